@@ -43,6 +43,11 @@ extern "C" {
 #define NERFX_PREC_FP32      0       /* v_mfma_f32_32x32x2_f32, exact fp32    */
 #define NERFX_PREC_BF16      1       /* v_mfma_f32_32x32x16_bf16, fp32 accum  */
 
+/* element types of the operators that take more than fp32 */
+#define NERFX_TYPE_F32       0
+#define NERFX_TYPE_BF16      1
+#define NERFX_TYPE_F16       2
+
 typedef struct nerfx_model nerfx_model_t;
 
 /* Shape of one radiance field -- the constructor arguments of
@@ -341,6 +346,44 @@ int nerfx_adam_step_scaled(float* param, const float* grad, float* exp_avg, floa
                            float lr, float beta1, float beta2, float eps, float weight_decay,
                            const float* grad_scale, const float* found_inf,
                            const float* step_in, float* step_out, void* stream);
+
+/* ---- orthogonalised updates (no counterpart in the reference) ------------------------------
+ * One matrix of a group, row-major and contiguous.  `grad` is read; `out` is written by
+ * nerfx_orthogonalize; `param` and `momentum` are updated by nerfx_muon_step. */
+typedef struct {
+    const void* grad;
+    void*   out;
+    float*  param;
+    float*  momentum;
+    int32_t rows, cols;  /* each 0..32768; an empty matrix is skipped */
+} nerfx_matrix_t;
+
+/* learning rate of one matrix: lr * sqrt(max(1, rows / cols)), or lr * 0.2 sqrt(max(rows, cols)) */
+#define NERFX_LR_ORIGINAL    0
+#define NERFX_LR_MATCH_RMS   1
+
+/* out = the matrix nearest to orthogonal that `steps` (1..32) Newton-Schulz steps make of grad:
+ * X = grad / max(|grad|_F, eps), then X <- a X + (b S + c S S) X with S = X X^T, (a, b, c) =
+ * coefficients[3 k ..] in step k (host array); a matrix with more rows than columns is worked on
+ * transposed.  Sums are fp32 (the norm fp64), products take both factors to 22 bits, whatever the
+ * `dtype` (NERFX_TYPE_*) of grad and out.  A zero matrix gives zeros; a matrix with an infinity or
+ * a NaN gives NaN.  `mats` is a host array; all matrices share the launches.  Coefficients
+ * that would let a singular value grow beyond 64 are refused.  `workspace`:
+ * nerfx_orthogonalize_workspace_bytes(mats, count) bytes, aligned to 16; it holds nothing between calls. */
+int64_t nerfx_orthogonalize_workspace_bytes(const nerfx_matrix_t* mats /* host */, int count);
+int nerfx_orthogonalize(const nerfx_matrix_t* mats /* host */, int count, int dtype,
+                        const float* coefficients /* host */, int steps, float eps,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+/* One optimisation step on a group of fp32 matrices:
+ *   momentum <- mu momentum + (1 - mu) g,   g = grad / *grad_scale (if given)
+ *   u = nesterov ? mu momentum + (1 - mu) g : momentum
+ *   param <- (1 - lr weight_decay) param - lr' orthogonalize(u),   lr' by `adjust_lr` (NERFX_LR_*)
+ * Nothing changes where *found_inf != 0 (device float, may be NULL).  No two matrices may share memory.
+ * The same workspace as nerfx_orthogonalize. */
+int nerfx_muon_step(const nerfx_matrix_t* mats /* host */, int count, double lr, double momentum, int nesterov,
+                    double weight_decay, int adjust_lr, const float* coefficients /* host */, int steps, float eps,
+                    const float* grad_scale, const float* found_inf,
+                    void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Distillation loss of distill.py:120-130 and its gradient w.r.t. the student's outputs:
  * loss = mean_i [ mean_j (alpha(s_sigma_i, delta_j) - alpha(t_sigma_i, delta_j))^2

@@ -14,6 +14,8 @@ LIB_PATH = os.environ.get("NERFX_LIB", os.path.join(_HERE, "libnerfx.so"))   # o
 ENC_POSITIONAL, ENC_FOURIER = 0, 1
 ACT_RELU, ACT_LEAKY_RELU, ACT_SILU = 0, 1, 2
 PREC_FP32, PREC_BF16 = 0, 1
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+LR_ORIGINAL, LR_MATCH_RMS = 0, 1
 
 
 class ModelDesc(C.Structure):
@@ -31,7 +33,12 @@ class DeviceInfo(C.Structure):
                 ("hbm_bytes", C.c_int64), ("arch", C.c_char * 32)]
 
 
-_p, _i, _l, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
+class Matrix(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("param", C.c_void_p), ("momentum", C.c_void_p),
+                ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
+_p, _i, _l, _f, _d = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double
 
 # name -> (restype, argtypes): exactly the declarations of include/nerfx.h
 SIGNATURES = {
@@ -69,6 +76,9 @@ SIGNATURES = {
     "nerfx_mse_loss_scaled": (_i, [_p, _p, _l, _p, _p, _p, _p, _p]),
     "nerfx_adam_step": (_i, [_p, _p, _p, _p, _l, _f, _f, _f, _f, _f, _p, _p, _p, _p, _p]),
     "nerfx_adam_step_scaled": (_i, [_p, _p, _p, _p, _l, _f, _f, _f, _f, _f, _p, _p, _p, _p, _p]),
+    "nerfx_orthogonalize_workspace_bytes": (_l, [C.POINTER(Matrix), _i]),
+    "nerfx_orthogonalize": (_i, [C.POINTER(Matrix), _i, _i, C.POINTER(_f), _i, _f, _p, _l, _p]),
+    "nerfx_muon_step": (_i, [C.POINTER(Matrix), _i, _d, _d, _i, _d, _i, C.POINTER(_f), _i, _f, _p, _p, _p, _l, _p]),
     "nerfx_voxel_sample": (_i, [_f, _f, _f, _f, _f, _f, _f, _f, _i, _i, C.c_uint64, C.c_uint64, _p, _p, _p, _p]),
     "nerfx_distill_loss": (_i, [_p, _p, _p, _p, _p, _l, _p, _p, _p, _p, _p]),
     "nerfx_debug_set_stamps": (None, [_p]),

@@ -722,6 +722,115 @@ def adam_step(param: Tensor, grad: Tensor, exp_avg: Tensor, exp_avg_sq: Tensor, 
                                       weight_decay, _p(inv_scale), _p(found_inf), _p(step_in), _p(step_out), _stream()))
 
 
+# ---- orthogonalised updates ------------------------------------------------------------------
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+_LR_RULES = {"original": _lib.LR_ORIGINAL, "match_rms_adamw": _lib.LR_MATCH_RMS}
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _ns_schedule(coefficients, steps: int):
+    """One (a, b, c) for all steps, or one for each -> the C array of 3 * steps floats."""
+    if not 1 <= steps <= 32:
+        raise ValueError(f"steps must be 1..32 (got {steps})")
+    rows = list(coefficients)
+    if len(rows) == 3 and not any(hasattr(r, "__len__") for r in rows):
+        rows = [tuple(rows)] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("coefficients: one (a, b, c), or one for each of the steps")
+    return (C.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def _ns_workspace(table, count: int, dev) -> Tuple[Tensor, int]:
+    need = lib.nerfx_orthogonalize_workspace_bytes(table, count)
+    if need < 0:
+        raise _lib.NerfxError(f"nerfx error: {lib.nerfx_last_error().decode()}")
+    return torch.empty((max(need, 1),), device=dev, dtype=torch.uint8), need
+
+
+def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7):
+    """The (semi-)orthogonal matrix near each of `mats` that `steps` Newton-Schulz steps reach: every
+    singular value of X = G / max(|G|, eps) goes through a s + b s^3 + c s^5 once per step, singular vectors stay.
+
+    `mats`: a matrix, a stack of them (b, r, c), or a list of matrices of any shapes (fp32, bf16 or fp16, one
+    type and device); all of them share the launches.  `coefficients`: (a, b, c), or one such triple per
+    step.  -> the same structure in the same type.  Results are held to fp32's precision before that
+    last rounding.  Not differentiable."""
+    listed = list(mats) if isinstance(mats, (list, tuple)) else list(mats.unbind(0)) if mats.dim() == 3 else [mats]
+    schedule = _ns_schedule(coefficients, steps)
+    for t in listed:
+        if not isinstance(t, Tensor):
+            raise TypeError("mats must be tensors")
+        if not t.is_cuda:
+            raise RuntimeError(f"nerf_amd runs on ROCm devices only: `mats` is on {t.device}")
+        if t.dtype not in _TYPES:
+            raise TypeError(f"orthogonalize takes fp32, bf16 or fp16 matrices (got {t.dtype})")
+        if t.dim() != 2:
+            raise ValueError(f"orthogonalize takes matrices (got a tensor of shape {tuple(t.shape)})")
+        if t.dtype != listed[0].dtype or t.device != listed[0].device:
+            raise ValueError("orthogonalize: all matrices of a call have one type and one device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("orthogonalize is not differentiable: pass detached matrices or call it under no_grad")
+    if not listed:
+        return torch.empty_like(mats) if isinstance(mats, Tensor) else []
+    dev = listed[0].device
+    srcs = [t.contiguous() for t in listed]
+    stacked = torch.empty(mats.shape, device=dev, dtype=mats.dtype) if isinstance(mats, Tensor) else None
+    outs = [torch.empty(t.shape, device=dev, dtype=t.dtype) for t in srcs] if stacked is None else \
+        list(stacked.unbind(0)) if stacked.dim() == 3 else [stacked]
+    table = (_lib.Matrix * len(srcs))(*[_lib.Matrix(s.data_ptr(), o.data_ptr(), None, None, *s.shape) for s, o in zip(srcs, outs)])
+    ws, need = _ns_workspace(table, len(srcs), dev)
+    with torch.cuda.device(dev):
+        check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[srcs[0].dtype], schedule, steps, eps, _p(ws), need, _stream()))
+    return outs if stacked is None else stacked
+
+
+def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+              steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, adjust_lr: str = "original",
+              grad_scale: Optional[Tensor] = None, found_inf: Optional[Tensor] = None) -> None:
+    """One step of momentum and orthogonalised updates on a list of matrices, in place:
+
+        momenta <- momentum * momenta + (1 - momentum) * grads            (grads / grad_scale where given)
+        u       =  momentum * momenta + (1 - momentum) * grads if nesterov else momenta
+        params  <- (1 - lr * weight_decay) * params - lr' * orthogonalize(u)
+
+    lr' = lr * sqrt(max(1, rows / cols)) ("original") or lr * 0.2 sqrt(max(rows, cols)) ("match_rms_adamw").
+    Where `found_inf` (one device float) is not zero nothing changes.  `params` and `momenta` are contiguous fp32
+    tensors that share no memory; all matrices share the launches and none of them waits for the host."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError("muon_step: params, grads and momenta pair up")
+    if adjust_lr not in _LR_RULES:
+        raise ValueError(f"adjust_lr must be one of {sorted(_LR_RULES)} (got {adjust_lr!r})")
+    schedule = _ns_schedule(coefficients, steps)
+    if not params:
+        return
+    dev = params[0].device
+    spans = []
+    for w, g, m in zip(params, grads, momenta):
+        for name, t in (("params", w), ("grads", g), ("momenta", m)):
+            if not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.dim() == 2 and t.shape == w.shape):
+                raise RuntimeError(f"muon_step: `{name}` must be fp32 matrices of one shape on one ROCm device")
+        for name, t in (("params", w), ("momenta", m)):
+            if not t.is_contiguous():
+                raise RuntimeError(f"muon_step: `{name}` must be contiguous (they are written in place)")
+            spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel()))
+    spans = sorted(s for s in spans if s[0] != s[1])
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise RuntimeError("muon_step: two of `params` and `momenta` share memory")
+    for name, t in (("grad_scale", grad_scale), ("found_inf", found_inf)):
+        if t is not None and not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.numel() == 1):
+            raise RuntimeError(f"muon_step: `{name}` must be one fp32 element on {dev}")
+    srcs = [g.detach().contiguous() for g in grads]
+    table = (_lib.Matrix * len(params))(*[_lib.Matrix(g.data_ptr(), None, w.data_ptr(), m.data_ptr(), *w.shape)
+                                          for w, g, m in zip(params, srcs, momenta)])
+    ws, need = _ns_workspace(table, len(params), dev)
+    with torch.cuda.device(dev):
+        check(lib.nerfx_muon_step(table, len(params), lr, momentum, int(nesterov), weight_decay, _LR_RULES[adjust_lr], schedule,
+                                  steps, eps, _p(grad_scale), _p(found_inf), _p(ws), need, _stream()))
+    for t in params + momenta:                              # written through raw pointers: tell autograd
+        torch.autograd.graph.increment_version(t)           # and the packed-weight cache of ModelHandle
+
+
 def voxel_sample(domain, voxels: int, samples: int, device, rng=None):
     """One distillation batch drawn by the sampling kernel: rx, rd (voxels * samples, 3), delta (voxels * samples)."""
     dev = _device(device)
