@@ -16,7 +16,7 @@ namespace nerfx {
 constexpr int ORTHO_GROUP = 32;                 // matrices per launch: the table has to fit the kernel arguments
 constexpr int ORTHO_MAX_SIDE = 32768;
 constexpr int ORTHO_MAX_STEPS = 32;
-constexpr int NORM_PARTS = 64;                  // partial sums of squares per matrix
+constexpr int NORM_PARTS = 512;                 // partial sums of squares per matrix
 constexpr int PREP_TILE = 64;
 
 struct OrthoMat {
@@ -32,6 +32,7 @@ struct OrthoMat {
 };
 struct OrthoArgs {
     OrthoMat mat[ORTHO_GROUP];
+    int32_t first[ORTHO_GROUP];                 // first block of each matrix in this launch; INT_MAX behind the last
     char* work;
     const float* grad_scale;
     const float* found_inf;
@@ -77,29 +78,32 @@ __device__ __forceinline__ float update_at(const OrthoArgs& a, const OrthoMat& q
     return a.nesterov ? fmaf(a.momentum, mom, a.rest * (g * unscale)) : mom;
 }
 
-// The matrix that block `b` of a launch works on, and the block's number within it.
-template <class Count>
-__device__ __forceinline__ int which_matrix(const OrthoArgs& a, int64_t& b, Count blocks_of) {
-    int k = 0;
-    for (; k < a.count - 1; ++k) {
-        const int64_t c = blocks_of(a.mat[k]);
-        if (b < c) break;
-        b -= c;
+// The matrix that this block works on, and the block's number within it.  (All of the table is read at once:
+// walking it would wait for each entry in turn.)
+__device__ __forceinline__ int which_matrix(const OrthoArgs& a, int& block) {
+    const int b = blockIdx.x;
+    int k = 0, start = 0;
+#pragma unroll
+    for (int i = 1; i < ORTHO_GROUP; ++i) {
+        const int f = a.first[i];
+        if (b >= f) { k = i; start = f; }
     }
+    block = b - start;
     return k;
 }
+enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
 
 // Momentum, and partial sums of squares of what is orthogonalised.  In double: a fp32 gradient's square
 // neither overflows nor vanishes there, and a sum of 2^30 of them keeps fp32's precision.
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoArgs a) {
-    int64_t b = blockIdx.x;
-    const OrthoMat q = a.mat[which_matrix(a, b, [](const OrthoMat& x) { return (int64_t)norm_parts(x); })];
+    int b;
+    const OrthoMat q = a.mat[which_matrix(a, b)];
     const int64_t total = (int64_t)q.rows * q.cols;
     const int parts = norm_parts(q);
     const bool skip = a.found_inf && *a.found_inf != 0.f;
     const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
     double acc = 0;
-    for (int64_t i = b * 256 + threadIdx.x; i < total; i += (int64_t)parts * 256) {
+    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < total; i += (int64_t)parts * 256) {
         if (a.muon && !skip)
             q.momentum[i] = fmaf(a.momentum, q.momentum[i], a.rest * (((const float*)q.grad)[i] * unscale));
         const double u = update_at(a, q, i, unscale);
@@ -115,13 +119,18 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoArgs a) {
 
 // X and X^T from what is orthogonalised: one 64 x 64 tile of X per block, through LDS, zeros in the padding.
 __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
-    int64_t b = blockIdx.x;
-    const OrthoMat q = a.mat[which_matrix(a, b, [](const OrthoMat& x) { return (int64_t)(x.m / PREP_TILE) * (x.n / PREP_TILE); })];
+    int b;
+    const OrthoMat q = a.mat[which_matrix(a, b)];
     __shared__ float tile[PREP_TILE][PREP_TILE + 1];
     const double* sums = (const double*)(a.work + ortho_sums_at(q));
+    __shared__ double part[4];
     double total = 0;
-    for (int k = 0; k < norm_parts(q); ++k) total += sums[k];
-    const double norm = sqrt(total);
+    for (int k = threadIdx.x; k < norm_parts(q); k += 256) total += sums[k];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = total;
+    __syncthreads();
+    const double norm = sqrt((part[0] + part[1]) + (part[2] + part[3]));
     double factor = (double)a.x_scale / (norm < (double)a.eps ? (double)a.eps : norm);                 // NaN stays NaN
     // A norm far below eps leaves X tiny, and f16 has few small numbers: X is then kept 2^lift larger, with room for
     // the growth of all steps.  (A, far smaller than 1 there, is stored as it is: X X^T / 4^lift.)
@@ -130,7 +139,7 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
     factor = ldexp(factor, lift);
     if (b == 0 && threadIdx.x == 0) *(int*)(a.work + ortho_lift_at(q)) = lift;
     const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
-    const int x0 = (int)(b / (q.n / PREP_TILE)) * PREP_TILE, y0 = (int)(b % (q.n / PREP_TILE)) * PREP_TILE;   // of X
+    const int x0 = b / (q.n / PREP_TILE) * PREP_TILE, y0 = b % (q.n / PREP_TILE) * PREP_TILE;   // of X
     // G's rows run along X's columns, or, if G is tall, along X's rows
     const int r0 = q.tall ? y0 : x0, c0 = q.tall ? x0 : y0;
     for (int e = threadIdx.x; e < PREP_TILE * PREP_TILE; e += 256) {
@@ -152,73 +161,112 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
 }
 
 // ---- the products ---------------------------------------------------------------------------------------------------
-// One T x T tile of P Q^T for two row-major split matrices with rows along K: 4 waves, each a quarter of the
-// tile.  Per step a workgroup brings one 32-wide block of K of both operands into LDS (the next one is on its
-// way in registers), 16-byte chunk c of row r at place c ^ (r & 7), so that the eight rows a ds_read_b128
-// phase touches lie on different banks.
-enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
+// One T x T tile of P Q^T for two row-major split matrices with rows along K: 2 x WAVES / 2 waves, each its part of
+// the tile.  A stage is one 32-wide block of K of both operands; STAGES of them lie in LDS, all but one of them on
+// their way while one is worked on (LDS-DMA: no registers hold them).  16-byte chunk c of row r lies at place
+// c ^ (r / 2 % 8), so that the sixteen rows a ds_read_b128 phase touches (256 bytes of banks) lie apart; LDS-DMA
+// writes lane after lane, so it is the source address that is permuted.
+// 64 lanes x 16 bytes from base + offset (per lane) to LDS at `lds` + 16 * lane.  The compiler does not know of the
+// load: whoever reads the LDS waits with landed().
+__device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+// All but the newest N of this wave's loads are done, and so are its LDS reads: then, behind the barrier, so are every wave's.
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
-template <int T>
+template <int T, int WAVES, int STAGES>
 struct SplitTile {
-    static constexpr int F = T / 64;                         // 32 x 32 fragments per wave and side
-    static constexpr int CHUNKS = T * 8 / 256;               // 16-byte chunks per thread and operand
-    float16_t_ acc[F][F];
+    static constexpr int FP = T / 64, FQ = T / (16 * WAVES); // 32 x 32 fragments per wave and side
+    static constexpr int LOADS = T / (8 * WAVES);            // per wave, stage and operand
+    static constexpr int STAGE_BYTES = 2 * T * SPLIT_BLOCK_BYTES;
+    static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
+    static_assert(STAGES >= 2 && STAGES <= 8 && 2 * LOADS * (STAGES - 1) < 64, "waits of landed()");
+    float16_t_ acc[FP][FQ];
 
-    __device__ __forceinline__ void run(char* lds, const char* P, const char* Q, int64_t p0, int64_t q0, int K) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-        const int64_t pitch = (int64_t)K / SPLIT_BLOCK * SPLIT_BLOCK_BYTES;
-        const int steps = K / SPLIT_BLOCK;
-        u32x4_t np[CHUNKS], nq[CHUNKS];
-        auto fetch = [&](int kb) {
+    // Until all stages but the newest `later` have landed.
+    static __device__ __forceinline__ void wait(int later) {
+        switch (later < STAGES - 1 ? later : STAGES - 1) {
+            case 0: landed<0>(); break;
+            case 1: landed<2 * LOADS>(); break;
+            case 2: landed<2 * LOADS * (STAGES > 2 ? 2 : 0)>(); break;
+            case 3: landed<2 * LOADS * (STAGES > 3 ? 3 : 0)>(); break;
+            case 4: landed<2 * LOADS * (STAGES > 4 ? 4 : 0)>(); break;
+            case 5: landed<2 * LOADS * (STAGES > 5 ? 5 : 0)>(); break;
+            case 6: landed<2 * LOADS * (STAGES > 6 ? 6 : 0)>(); break;
+            default: landed<2 * LOADS * (STAGES > 7 ? 7 : 0)>(); break;
+        }
+    }
+    struct Frags { half8_t ph[FP], pl[FP], qh[FQ], ql[FQ]; };
+    // half s of stage buffer `buf`: 16 of its 32 columns
+    static __device__ __forceinline__ void read(Frags& f, const char* buf, int s, int wave, int lane) {
+        auto frag = [&](int row, int chunk) {
+            return *(const half8_t*)(buf + row * SPLIT_BLOCK_BYTES + ((chunk ^ (row >> 1 & 7)) * 16));
+        };
+        const int p_row = row_of(wave) + (lane & 31), q_row = T + col_of(wave) + (lane & 31), c = 2 * s + (lane >> 5);
 #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const int chunk = tid + 256 * i, r = chunk >> 3, c = chunk & 7;
-                np[i] = *(const u32x4_t*)(P + (p0 + r) * pitch + (int64_t)kb * SPLIT_BLOCK_BYTES + c * 16);
-                nq[i] = *(const u32x4_t*)(Q + (q0 + r) * pitch + (int64_t)kb * SPLIT_BLOCK_BYTES + c * 16);
+        for (int i = 0; i < FP; ++i) { f.ph[i] = frag(p_row + 32 * i, c); f.pl[i] = frag(p_row + 32 * i, c + 4); }
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) { f.qh[j] = frag(q_row + 32 * j, c); f.ql[j] = frag(q_row + 32 * j, c + 4); }
+    }
+    // the three products of a fragment lie apart, so that no instruction waits for the one before
+    __device__ __forceinline__ void multiply(const Frags& f) {
+#pragma unroll
+        for (int t = 0; t < 3; ++t)
+#pragma unroll
+            for (int i = 0; i < FP; ++i)
+#pragma unroll
+                for (int j = 0; j < FQ; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(t == 1 ? f.pl[i] : f.ph[i], t == 0 ? f.ql[j] : f.qh[j],
+                                                                       acc[i][j], 0, 0, 0);
+    }
+
+    __device__ __forceinline__ void run(char* lds, const char* P, const char* Q, int K) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t pitch = (uint32_t)K / SPLIT_BLOCK * SPLIT_BLOCK_BYTES;
+        const int steps = K / SPLIT_BLOCK;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        // this lane's 16 bytes of the first of the rows that the wave's loads bring; the others lie 8 WAVES rows apart
+        const int row = 8 * wave + (lane >> 3);
+        const uint32_t offset = (uint32_t)row * pitch + ((lane & 7) ^ (row >> 1 & 7)) * 16;
+        auto fetch = [&](int kb) {
+            const uint32_t to = lds0 + (uint32_t)(kb % STAGES) * STAGE_BYTES + wave * 1024;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const uint32_t at = to + i * WAVES * 1024, from = offset + i * 8 * WAVES * pitch;
+                dma16(at, P + (int64_t)kb * SPLIT_BLOCK_BYTES, from);
+                dma16(at + T * SPLIT_BLOCK_BYTES, Q + (int64_t)kb * SPLIT_BLOCK_BYTES, from);
             }
         };
 #pragma unroll
-        for (int i = 0; i < F; ++i)
+        for (int i = 0; i < FP; ++i)
 #pragma unroll
-            for (int j = 0; j < F; ++j)
+            for (int j = 0; j < FQ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        fetch(0);
-        for (int kb = 0; kb < steps; ++kb) {
-            char* buf = lds + (kb & 1) * (2 * T * SPLIT_BLOCK_BYTES);
 #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const int chunk = tid + 256 * i, r = chunk >> 3, c = chunk & 7;
-                *(u32x4_t*)(buf + r * SPLIT_BLOCK_BYTES + ((c ^ (r & 7)) * 16)) = np[i];
-                *(u32x4_t*)(buf + (T + r) * SPLIT_BLOCK_BYTES + ((c ^ (r & 7)) * 16)) = nq[i];
-            }
-            __syncthreads();          // two buffers: the writes above and the reads of the step before lie apart
-            if (kb + 1 < steps) fetch(kb + 1);
-            auto frag = [&](int row, int chunk) {
-                return *(const half8_t*)(buf + row * SPLIT_BLOCK_BYTES + ((chunk ^ (row & 7)) * 16));
-            };
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                half8_t ph[F], pl[F], qh[F], ql[F];
-                const int c = 2 * s + (lane >> 5);
-#pragma unroll
-                for (int i = 0; i < F; ++i) {
-                    const int pr = (wave >> 1) * (T / 2) + 32 * i + (lane & 31);
-                    const int qr = T + (wave & 1) * (T / 2) + 32 * i + (lane & 31);
-                    ph[i] = frag(pr, c); pl[i] = frag(pr, c + 4);
-                    qh[i] = frag(qr, c); ql[i] = frag(qr, c + 4);
-                }
-#pragma unroll
-                for (int i = 0; i < F; ++i)
-#pragma unroll
-                    for (int j = 0; j < F; ++j) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-                    }
-            }
+        for (int kb = 0; kb < STAGES; ++kb)
+            if (kb < steps) fetch(kb);
+        Frags f0, f1;
+        wait(steps - 1);
+        read(f0, lds, 0, wave, lane);
+        for (int kb = 0; kb < steps - 1; ++kb) {             // fragments are read one half stage ahead of their use
+            read(f1, lds + (kb % STAGES) * STAGE_BYTES, 1, wave, lane);
+            multiply(f0);
+            wait(min(STAGES - 2, steps - 2 - kb));           // stage kb + 1 is there, and every wave has read all of stage kb,
+            if (kb + STAGES < steps) fetch(kb + STAGES);     // whose place this one takes
+            read(f0, lds + ((kb + 1) % STAGES) * STAGE_BYTES, 0, wave, lane);
+            multiply(f1);
         }
+        read(f1, lds + ((steps - 1) % STAGES) * STAGE_BYTES, 1, wave, lane);
+        multiply(f0);
+        multiply(f1);
     }
+    // where in the tile a wave's part begins
+    static __device__ __forceinline__ int row_of(int wave) { return wave / (WAVES / 2) * (T / 2); }
+    static __device__ __forceinline__ int col_of(int wave) { return wave % (WAVES / 2) * (2 * T / WAVES); }
 };
 
 // Number t of a lower triangle's tiles, row after row -> (row, column).
@@ -229,32 +277,42 @@ __device__ __forceinline__ void triangle_at(int64_t t, int& i, int& j) {
     j = (int)(t - (int64_t)i * (i + 1) / 2);
 }
 
-template <int T, int KIND>
-__global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoArgs a) {
-    __shared__ __align__(16) char lds[2 * 2 * T * SPLIT_BLOCK_BYTES];
+template <int T, int WAVES, int STAGES, int KIND>
+__global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoArgs a) {
+    extern __shared__ __align__(16) char lds[];
     constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;       // the result is symmetric: half of the tiles
-    int64_t b = blockIdx.x;
-    const OrthoMat q = a.mat[which_matrix(a, b, [](const OrthoMat& x) {
-        const int64_t mt = x.m / T;
-        return SYM ? mt * (mt + 1) / 2 : mt * (x.n / T);
-    })];
+    int b;
+    const OrthoMat q = a.mat[which_matrix(a, b)];
     int ti, tj;
     if constexpr (SYM) {
         triangle_at(b, ti, tj);
     } else {
-        ti = (int)(b % (q.m / T));
-        tj = (int)(b / (q.m / T));
+        ti = b % (q.m / T);
+        tj = b / (q.m / T);
     }
     char* X = a.work + q.base;
     char* A = a.work + ortho_a_at(q);
     char* B = a.work + ortho_b_at(q);
     const char* P = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : B;
     const char* Q = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : a.work + ortho_xt_at(q, a.from);
-    SplitTile<T> tile;
-    tile.run(lds, P, Q, (int64_t)ti * T, (int64_t)tj * T, KIND == ORTHO_GRAM ? q.n : q.m);
-
+    const int K = KIND == ORTHO_GRAM ? q.n : q.m;
+    using Tile = SplitTile<T, WAVES, STAGES>;
+    Tile tile;
     // element (row, col) of a 32 x 32 accumulator: col = lane % 32, row = 8 (e / 4) + 4 (lane / 32) + e % 4
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // the element itself, A[row][col] = A[col][row] or X[row][col] = X^T[col][row], is on its way from the start
+    Split4 own[Tile::FP][Tile::FQ][4];
+    if constexpr (KIND != ORTHO_GRAM) {
+#pragma unroll
+        for (int i = 0; i < Tile::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < Tile::FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    own[i][j][e] = split_load4(Q, tj * T + Tile::col_of(wave) + 32 * j + (lane & 31),
+                                               ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e, q.m);
+    }
+    tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K);
     float alpha = a.alpha, beta = a.beta;
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {            // see the kernel that made X
         const int lift = *(const int*)(a.work + ortho_lift_at(q));
@@ -263,11 +321,11 @@ __global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoArgs a) {
     }
     const bool skip = KIND == ORTHO_LAST && a.found_inf && *a.found_inf != 0.f;
 #pragma unroll
-    for (int i = 0; i < SplitTile<T>::F; ++i)
+    for (int i = 0; i < Tile::FP; ++i)
 #pragma unroll
-        for (int j = 0; j < SplitTile<T>::F; ++j) {
-            const int row0 = ti * T + (wave >> 1) * (T / 2) + 32 * i + 4 * (lane >> 5);
-            const int col = tj * T + (wave & 1) * (T / 2) + 32 * j + (lane & 31);
+        for (int j = 0; j < Tile::FQ; ++j) {
+            const int row0 = ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5);
+            const int col = tj * T + Tile::col_of(wave) + 32 * j + (lane & 31);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = row0 + 8 * e;
@@ -276,11 +334,9 @@ __global__ __launch_bounds__(256) void ortho_product_kernel(const OrthoArgs a) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[k] = beta * tile.acc[i][j][4 * e + k];
                 } else {
-                    // the element itself: A[row][col] = A[col][row], or X[row][col] = X^T[col][row]
-                    float own[4];
-                    split_load4(Q, col, row, q.m, own);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = fmaf(beta, tile.acc[i][j][4 * e + k], alpha * own[k]);
+                    for (int k = 0; k < 4; ++k)
+                        v[k] = fmaf(beta, tile.acc[i][j][4 * e + k], alpha * ((float)own[i][j][e].hi[k] + (float)own[i][j][e].lo[k]));
                 }
                 if constexpr (SYM) {
                     char* dst = KIND == ORTHO_GRAM ? A : B;
@@ -382,34 +438,46 @@ static int scales_for(const float* coef, int steps, OrthoScales& s) {
     return 0;
 }
 
-template <int T>
+template <int T, int WAVES, int STAGES>
 static int ortho_run(OrthoArgs& a, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
-    int64_t parts = 0, prep = 0, sym = 0, full = 0;
-    for (int k = 0; k < a.count; ++k) {
-        const int64_t mt = a.mat[k].m / T, nt = a.mat[k].n / T;
-        parts += norm_parts(a.mat[k]);
-        prep += (int64_t)(a.mat[k].m / PREP_TILE) * (a.mat[k].n / PREP_TILE);
-        sym += mt * (mt + 1) / 2;
-        full += mt * nt;
-    }
-    const dim3 block(256);
+    // a launch's grid is the matrices' blocks one after the other
+    auto grid = [&](auto blocks_of) {
+        int64_t at = 0;
+        for (int k = 0; k < ORTHO_GROUP; ++k) {
+            a.first[k] = k < a.count ? (int32_t)at : INT32_MAX;
+            if (k < a.count) at += blocks_of(a.mat[k]);
+        }
+        return dim3((unsigned)at);
+    };
+    auto symmetric = [](const OrthoMat& q) { return (int64_t)(q.m / T) * (q.m / T + 1) / 2; };
+    auto whole = [](const OrthoMat& q) { return (int64_t)(q.m / T) * (q.n / T); };
+    const dim3 block(256), product(64 * WAVES);
+    const size_t lds = SplitTile<T, WAVES, STAGES>::LDS_BYTES;
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_GRAM>), lds);
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_POLY>), lds);
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_APPLY>), lds);
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_LAST>), lds);
     a.x_scale = s.x;
     a.growth = s.growth;
-    hipLaunchKernelGGL(ortho_norm_kernel, dim3((unsigned)parts), block, 0, stream, a);
-    hipLaunchKernelGGL(ortho_prep_kernel, dim3((unsigned)prep), block, 0, stream, a);
+    dim3 g = grid([](const OrthoMat& q) { return (int64_t)norm_parts(q); });
+    hipLaunchKernelGGL(ortho_norm_kernel, g, block, 0, stream, a);
+    g = grid([](const OrthoMat& q) { return (int64_t)(q.m / PREP_TILE) * (q.n / PREP_TILE); });
+    hipLaunchKernelGGL(ortho_prep_kernel, g, block, 0, stream, a);
     for (int k = 0; k < steps; ++k) {
         const float ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
+        g = grid(symmetric);
         a.beta = s.a / (s.x * s.x);
-        hipLaunchKernelGGL((ortho_product_kernel<T, ORTHO_GRAM>), dim3((unsigned)sym), block, 0, stream, a);
+        hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_GRAM>), g, product, lds, stream, a);
         a.alpha = cb * (s.b / s.a);
         a.beta = cc * (s.b / s.a / s.a);
-        hipLaunchKernelGGL((ortho_product_kernel<T, ORTHO_POLY>), dim3((unsigned)sym), block, 0, stream, a);
+        hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_POLY>), g, product, lds, stream, a);
+        g = grid(whole);
         a.from = k & 1; a.to = a.from ^ 1;
         const bool last = k == steps - 1;
         a.alpha = last ? ca / s.x : ca;                       // the last step leaves the scale
         a.beta = last ? 1.0f / (s.b * s.x) : 1.0f / s.b;
-        if (last) hipLaunchKernelGGL((ortho_product_kernel<T, ORTHO_LAST>), dim3((unsigned)full), block, 0, stream, a);
-        else hipLaunchKernelGGL((ortho_product_kernel<T, ORTHO_APPLY>), dim3((unsigned)full), block, 0, stream, a);
+        if (last) hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_LAST>), g, product, lds, stream, a);
+        else hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_APPLY>), g, product, lds, stream, a);
     }
     return launch_status("orthogonalisation kernels");
 }
@@ -443,7 +511,7 @@ static int ortho_groups(const nerfx_matrix_t* mats, int count, OrthoArgs& a, con
             const double r = a.mat[i].rows, l = a.mat[i].cols;
             a.mat[i].lr = (float)(lr * (adjust == NERFX_LR_MATCH_RMS ? 0.2 * std::sqrt(std::max(r, l)) : std::sqrt(std::max(1.0, r / l))));
         }
-        if (int rc = tile == 128 ? ortho_run<128>(a, coef, steps, s, stream) : ortho_run<64>(a, coef, steps, s, stream)) return rc;
+        if (int rc = tile == 128 ? ortho_run<128, 8, 4>(a, coef, steps, s, stream) : ortho_run<64, 4, 8>(a, coef, steps, s, stream)) return rc;
     }
     return 0;
 }

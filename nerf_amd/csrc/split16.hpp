@@ -39,11 +39,10 @@ __device__ __forceinline__ void split_store4(char* base, int64_t r, int k, int n
     *(half4_t*)p = hi;
     *(half4_t*)(p + 64) = lo;
 }
-__device__ __forceinline__ void split_load4(const char* base, int64_t r, int k, int n_cols, float (&v)[4]) {
+struct Split4 { half4_t hi, lo; };
+__device__ __forceinline__ Split4 split_load4(const char* base, int64_t r, int k, int n_cols) {
     const char* p = split_at(const_cast<char*>(base), r, k, n_cols);
-    const half4_t hi = *(const half4_t*)p, lo = *(const half4_t*)(p + 64);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)hi[i] + (float)lo[i];
+    return {*(const half4_t*)p, *(const half4_t*)(p + 64)};
 }
 #endif
 
