@@ -36,6 +36,7 @@ extern "C" {
 #define NERFX_ENC_POSITIONAL 0       /* features.py:22-36  */
 #define NERFX_ENC_FOURIER    1       /* features.py:40-52  */
 /* hidden activations (model.py:28; train.py:235) */
+#define NERFX_ACT_NONE     (-1)      /* nerfx_mx4_linear only                 */
 #define NERFX_ACT_RELU       0
 #define NERFX_ACT_LEAKY_RELU 1       /* negative slope 0.01 (torch default)   */
 #define NERFX_ACT_SILU       2
@@ -47,6 +48,7 @@ extern "C" {
 #define NERFX_TYPE_F32       0
 #define NERFX_TYPE_BF16      1
 #define NERFX_TYPE_F16       2
+#define NERFX_TYPE_MX4       3       /* blocks of 32 4-bit codes, one scale each */
 
 typedef struct nerfx_model nerfx_model_t;
 
@@ -384,6 +386,25 @@ int nerfx_muon_step(const nerfx_matrix_t* mats /* host */, int count, double lr,
                     double weight_decay, int adjust_lr, const float* coefficients /* host */, int steps, float eps,
                     const float* grad_scale, const float* found_inf,
                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- microscaled 4-bit numbers (no counterpart in the reference) ---------------------------
+ * A row of k values is ceil(k / 32) blocks, the last one filled with zeros.  A block has 32 codes in 16
+ * bytes (value 2 i in the low half of byte i) and a scale byte s: its values are code * 2^(s - 127), code of
+ * +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, and s = 255 makes all of them NaN.  Arrays: codes (rows, 16 ceil(k / 32)),
+ * scales (rows, ceil(k / 32)), both contiguous.  1 <= k <= 2^20, rows < 2^31.
+ * quantize: s - 127 = floor(log2 max |x|) - 2 clamped to [-127, 127], codes rounded to nearest, ties to even,
+ * saturating; a block with an infinity or a NaN gets s = 255 and zero codes.  codes aligned to 4 bytes. */
+int nerfx_mx4_quantize(const void* x, int dtype, int64_t rows, int k, uint8_t* codes, uint8_t* scales, void* stream);
+int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k, int dtype, void* out,
+                         void* stream);
+/* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
+ * x_scales its scales; NULL otherwise), W (n, k) as codes and scales aligned to 16 bytes, bias (n) fp32 or NULL, sums in fp32,
+ * y in y_dtype (fp32, bf16 or f16), activ NERFX_ACT_*.
+ * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
+int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype);
+int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,
+                     const uint8_t* w_codes, const uint8_t* w_scales, int n, const float* bias, int activ,
+                     void* y, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Distillation loss of distill.py:120-130 and its gradient w.r.t. the student's outputs:
  * loss = mean_i [ mean_j (alpha(s_sigma_i, delta_j) - alpha(t_sigma_i, delta_j))^2

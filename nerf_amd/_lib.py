@@ -14,7 +14,8 @@ LIB_PATH = os.environ.get("NERFX_LIB", os.path.join(_HERE, "libnerfx.so"))   # o
 ENC_POSITIONAL, ENC_FOURIER = 0, 1
 ACT_RELU, ACT_LEAKY_RELU, ACT_SILU = 0, 1, 2
 PREC_FP32, PREC_BF16 = 0, 1
-TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_MX4 = 0, 1, 2, 3
+ACT_NONE = -1
 LR_ORIGINAL, LR_MATCH_RMS = 0, 1
 
 
@@ -79,6 +80,10 @@ SIGNATURES = {
     "nerfx_orthogonalize_workspace_bytes": (_l, [C.POINTER(Matrix), _i]),
     "nerfx_orthogonalize": (_i, [C.POINTER(Matrix), _i, _i, C.POINTER(_f), _i, _f, _p, _l, _p]),
     "nerfx_muon_step": (_i, [C.POINTER(Matrix), _i, _d, _d, _i, _d, _i, C.POINTER(_f), _i, _f, _p, _p, _p, _l, _p]),
+    "nerfx_mx4_quantize": (_i, [_p, _i, _l, _i, _p, _p, _p]),
+    "nerfx_mx4_dequantize": (_i, [_p, _p, _l, _i, _i, _p, _p]),
+    "nerfx_mx4_linear_workspace_bytes": (_l, [_l, _i, _i, _i]),
+    "nerfx_mx4_linear": (_i, [_p, _i, _p, _l, _i, _p, _p, _i, _p, _i, _p, _i, _p, _l, _p]),
     "nerfx_voxel_sample": (_i, [_f, _f, _f, _f, _f, _f, _f, _f, _i, _i, C.c_uint64, C.c_uint64, _p, _p, _p, _p]),
     "nerfx_distill_loss": (_i, [_p, _p, _p, _p, _p, _l, _p, _p, _p, _p, _p]),
     "nerfx_debug_set_stamps": (None, [_p]),

@@ -831,6 +831,124 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
         torch.autograd.graph.increment_version(t)           # and the packed-weight cache of ModelHandle
 
 
+# ---- microscaled 4-bit numbers -----------------------------------------------------------------
+_LINEAR_ACTS = {None: _lib.ACT_NONE, "relu": _lib.ACT_RELU, "leaky_relu": _lib.ACT_LEAKY_RELU, "silu": _lib.ACT_SILU}
+
+
+class Mx4:
+    """A matrix of microscaled 4-bit numbers: `codes` (rows, 16 * blocks) and `scales` (rows, blocks), uint8, for `k`
+    columns in blocks of 32 (include/nerfx.h has the format).  `mx4_quantize` makes one; it may also be built from stored
+    tensors.  Held as given: no copy."""
+
+    def __init__(self, codes: Tensor, scales: Tensor, k: int):
+        if not 1 <= k <= 1 << 20:
+            raise ValueError(f"Mx4: k must be 1..2^20 (got {k})")
+        blocks = (k + 31) // 32
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or \
+                tuple(scales.shape) != (codes.shape[0], blocks) or codes.shape[1] != 16 * blocks or codes.device != scales.device:
+            raise ValueError(f"Mx4: codes (rows, {16 * blocks}) and scales (rows, {blocks}) of type uint8 on one device hold {k} columns "
+                             f"(got {tuple(codes.shape)}, {tuple(scales.shape)})")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("Mx4: codes and scales must be contiguous")
+        if codes.data_ptr() % 16:
+            raise ValueError("Mx4: codes must be aligned to 16 bytes")
+        self.codes, self.scales, self.k = codes, scales, k
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.codes.shape[0], self.k
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to(self, device) -> "Mx4":
+        return Mx4(self.codes.to(device), self.scales.to(device), self.k)
+
+    def dequantize(self, dtype=torch.float32) -> Tensor:
+        """The values the codes stand for (exact in fp32 and bf16)."""
+        if dtype not in _TYPES:
+            raise TypeError(f"dequantize gives fp32, bf16 or fp16 (asked for {dtype})")
+        if not self.codes.is_cuda:
+            raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {self.codes.device}")
+        out = torch.empty(self.shape, device=self.device, dtype=dtype)
+        with torch.cuda.device(self.device):
+            check(lib.nerfx_mx4_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.k, _TYPES[dtype], _p(out), _stream()))
+        return out
+
+
+def _mx4_input(x: Tensor, name: str) -> Tensor:
+    if not isinstance(x, Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"nerf_amd runs on ROCm devices only: `{name}` is on {x.device}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{name} must be fp32, bf16 or fp16 (got {x.dtype})")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 20:
+        raise ValueError(f"{name}: the last dimension must hold 1..2^20 values (got {tuple(x.shape)})")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"4-bit numbers carry no gradient: detach `{name}` or call under no_grad")
+    return x.detach().contiguous()
+
+
+def mx4_quantize(x: Tensor) -> Mx4:
+    """x (rows, k) in fp32, bf16 or fp16 -> its microscaled 4-bit form: per block of 32 along a row the exponent of the largest
+    magnitude, codes rounded to nearest (ties to even, saturating).  A block with an infinity or a NaN becomes NaN."""
+    x = _mx4_input(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"mx4_quantize takes a matrix (got shape {tuple(x.shape)})")
+    rows, k = x.shape
+    blocks = (k + 31) // 32
+    codes = torch.empty((rows, 16 * blocks), device=x.device, dtype=torch.uint8)
+    scales = torch.empty((rows, blocks), device=x.device, dtype=torch.uint8)
+    with torch.cuda.device(x.device):
+        check(lib.nerfx_mx4_quantize(_p(x), _TYPES[x.dtype], rows, k, _p(codes), _p(scales), _stream()))
+    return Mx4(codes, scales, k)
+
+
+def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Optional[str] = None, out_dtype=None) -> Tensor:
+    """activation(Q(x) @ weight.T + bias) with both factors in 4 bits and fp32 sums: what a frozen Linear layer packed with
+    `mx4_quantize` answers.  `x` (..., k): fp32, bf16 or fp16, quantised as `mx4_quantize` does on its way, or an `Mx4`; `weight`
+    (n, k); `bias` (n) fp32; `activation` None, "relu", "leaky_relu" (slope 0.01) or "silu".  -> (..., n) in `out_dtype`
+    (default: x's type, fp32 for an `Mx4`).  No gradient."""
+    if not isinstance(weight, Mx4):
+        raise TypeError("weight must be an Mx4 (see mx4_quantize)")
+    if activation not in _LINEAR_ACTS:
+        raise ValueError(f"unknown activation {activation!r}")
+    n, k = weight.shape
+    if isinstance(x, Mx4):
+        lead, dt, src, scales, dev = (x.shape[0],), _lib.TYPE_MX4, x.codes, x.scales, x.device
+        if not x.codes.is_cuda:
+            raise RuntimeError(f"nerf_amd runs on ROCm devices only: `x` is on {dev}")
+        width, default = x.k, torch.float32
+    else:
+        src = _mx4_input(x, "x")
+        lead, dt, scales, dev, width, default = src.shape[:-1], _TYPES[src.dtype], None, src.device, src.shape[-1], src.dtype
+    if width != k:
+        raise ValueError(f"x has {width} columns, weight {k}")
+    if weight.device != dev:
+        raise ValueError(f"x is on {dev}, weight on {weight.device}")
+    if bias is not None:
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("4-bit numbers carry no gradient: detach `bias` or call under no_grad")
+        if tuple(bias.shape) != (n,) or bias.device != dev:
+            raise ValueError(f"bias must be ({n},) on {dev}")
+        bias = _dev(bias.detach(), "bias")
+    out_dtype = default if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES:
+        raise TypeError(f"mx4_linear gives fp32, bf16 or fp16 (asked for {out_dtype})")
+    m = 1
+    for s in lead:
+        m *= s
+    y = torch.empty((*lead, n), device=dev, dtype=out_dtype)
+    need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt)
+    ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
+    with torch.cuda.device(dev):
+        check(lib.nerfx_mx4_linear(_p(src), dt, _p(scales), m, k, _p(weight.codes), _p(weight.scales), n, _p(bias),
+                                   _LINEAR_ACTS[activation], _p(y), _TYPES[out_dtype], _p(ws), max(need, 0), _stream()))
+    return y
+
+
 def voxel_sample(domain, voxels: int, samples: int, device, rng=None):
     """One distillation batch drawn by the sampling kernel: rx, rd (voxels * samples, 3), delta (voxels * samples)."""
     dev = _device(device)
