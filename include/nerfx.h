@@ -398,8 +398,8 @@ int nerfx_mx4_quantize(const void* x, int dtype, int64_t rows, int k, uint8_t* c
 int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k, int dtype, void* out,
                          void* stream);
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
- * x_scales its scales; NULL otherwise), W (n, k) as codes and scales aligned to 16 bytes, bias (n) fp32 or NULL, sums in fp32,
- * y in y_dtype (fp32, bf16 or f16), activ NERFX_ACT_*.
+ * x_scales its scales; NULL otherwise), W (n, k) as codes and scales, bias (n) fp32 or NULL, sums in fp32,
+ * y in y_dtype (fp32, bf16 or f16), activ NERFX_ACT_*.  x and the weight's codes aligned to 16 bytes.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
 int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,

@@ -1,8 +1,9 @@
 // Microscaled 4-bit numbers (mx4.hpp): to them, back, and the product of two matrices of them.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
+#include <type_traits>
 
+#include "lds_dma.hpp"
 #include "mx4.hpp"
 #include "split16.hpp"
 
@@ -110,20 +111,30 @@ __device__ __forceinline__ float mx4_activate(float v, int activ) {
     return v;
 }
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ i32x8_t mx4_operand(u32x4_t c) { return {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0}; }
 
-// y for the 32 x 32 accumulator of rows n0 .. of W and rows m0 .. of x: a lane holds row m = m0 + lane % 32 and, with
-// h = lane / 32, columns n0 + 8 q + 4 h + i in element 4 q + i.
+// One activation for 16 values: the choice is made once, not in front of each of them.
+__device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = f(v[e]);
+    };
+    if (activ == NERFX_ACT_RELU) each([](float x) { return mx4_activate(x, NERFX_ACT_RELU); });
+    else if (activ == NERFX_ACT_LEAKY_RELU) each([](float x) { return mx4_activate(x, NERFX_ACT_LEAKY_RELU); });
+    else if (activ == NERFX_ACT_SILU) each([](float x) { return mx4_activate(x, NERFX_ACT_SILU); });
+}
+
+// y for the 32 x 32 accumulator (bias included) of rows n0 .. of W and rows m0 .. of x: a lane holds row m = m0 + lane % 32
+// and, with h = lane / 32, columns n0 + 8 q + 4 h + i in element 4 q + i.
 __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, const float16_t_& acc, int64_t m0, int n0) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int64_t m = m0 + (lane & 31);
     float v[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
-        v[e] = mx4_activate(acc[e] + (a.bias && n < a.n ? a.bias[n] : 0.f), a.activ);
-    }
+    for (int e = 0; e < 16; ++e) v[e] = acc[e];
+    mx4_activate16(v, a.activ);
     if (a.y_dtype == NERFX_TYPE_F32) {
         if (m >= a.m) return;
         float* y = (float*)a.y + m * a.n;
@@ -143,9 +154,11 @@ __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, const float16_
     // two 16-bit values a word; word 2 q + p holds columns 8 q + 4 h + 2 p, + 1
     uint32_t w[8];
 #pragma unroll
-    for (int p = 0; p < 8; ++p)
-        w[p] = a.y_dtype == NERFX_TYPE_BF16 ? __builtin_bit_cast(uint32_t, (bf16x2_t){(__bf16)v[2 * p], (__bf16)v[2 * p + 1]})
-                                            : __builtin_bit_cast(uint32_t, (f16x2_t){(_Float16)v[2 * p], (_Float16)v[2 * p + 1]});
+    for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (bf16x2_t){(__bf16)v[2 * p], (__bf16)v[2 * p + 1]});
+    if (a.y_dtype == NERFX_TYPE_F16) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (f16x2_t){(_Float16)v[2 * p], (_Float16)v[2 * p + 1]});
+    }
     if (!a.y_whole) {
         if (m >= a.m) return;
         uint16_t* y = (uint16_t*)a.y + m * a.n;
@@ -172,27 +185,104 @@ __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, const float16_
 }
 
 // A (32 FP WP) x (32 FQ WQ) tile of W x^T per workgroup of WP x WQ waves.  A stage is eight blocks (256 values) of every
-// row of both operands, 128 bytes a row, brought by LDS-DMA; block c of row r lies at place c ^ (r / 2 % 8), as in the
-// split16 products.  The scales, one byte a block, go straight into registers one stage ahead.
-template <int FP, int WP, int FQ, int WQ, int STAGES>
+// row of both operands, 128 bytes a row, brought by LDS-DMA while the stage before is worked on; block c of row r lies
+// at place c ^ (r / 2 % 8), so that the sixteen rows of a read phase touch different banks.  The scales, a byte a block, come
+// sixteen a row, two stages' worth, by way of registers: read in smaller pieces they would be most of the requests;
+// fragments are read one step (64 values) ahead of their use.  Rows behind
+// the last one and blocks behind a row's end are read from the last ones: the results of the former are not stored, the codes of
+// the latter are cleared on one side.
+template <int FP, int WP, int FQ, int WQ>
 struct Mx4Tile {
-    static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ;
+    static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ, STAGES = 2;
     static constexpr int STAGE_BLOCKS = 8, ROW_BYTES = STAGE_BLOCKS * MX4_BLOCK_BYTES;
-    static constexpr int STAGE_BYTES = (TP + TQ) * ROW_BYTES, LDS_BYTES = STAGES * STAGE_BYTES;
+    static constexpr int STAGE_BYTES = (TP + TQ) * ROW_BYTES;
+    // behind the stages: two chunks of scales, 16 bytes a row each, and the bias
+    static constexpr int SCALES_AT = STAGES * STAGE_BYTES, CHUNK_BYTES = (TP + TQ) * 16, BIAS_AT = SCALES_AT + 2 * CHUNK_BYTES;
+    static constexpr int LDS_BYTES = BIAS_AT + 4 * TP, CHUNK_ROWS = (TP + TQ) / (64 * WAVES);
     static constexpr int LOADS_P = TP / (8 * WAVES), LOADS_Q = TQ / (8 * WAVES);
-    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && LDS_BYTES <= 160 * 1024, "whole loads per wave");
+    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && WAVES % 2 == 0 && (TP + TQ) % (64 * WAVES) == 0 && LDS_BYTES <= 160 * 1024, "whole loads per wave");
+
+    struct Frags { u32x4_t p[FP], q[FQ]; };
+    // step s of the stage in `buf`
+    static __device__ __forceinline__ void read(Frags& f, const char* buf, int s, int p_row, int q_row, int h) {
+        auto frag = [&](int row) { return *(const u32x4_t*)(buf + row * ROW_BYTES + (((2 * s + h) ^ (row >> 1 & 7)) * 16)); };
+#pragma unroll
+        for (int i = 0; i < FP; ++i) f.p[i] = frag(p_row + 32 * i);
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) f.q[j] = frag(q_row + 32 * j);
+        __builtin_amdgcn_sched_barrier(0);                     // in front of the products of the step before, not behind them
+    }
+    // Scales of a row's blocks 16 chunk .. + 15; behind the row's end the last one again.
+    static __device__ __forceinline__ u32x4_t chunk(const uint8_t* row, int chunk, int nb) {
+        u32x4_t v = {0, 0, 0, 0};
+        if (16 * chunk + 16 <= nb) {
+            __builtin_memcpy(&v, row + 16 * chunk, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i / 4] |= (uint32_t)row[min(16 * chunk + i, nb - 1)] << (8 * (i % 4));
+        }
+        return v;
+    }
+    // From a chunk in LDS: those of blocks 2 s + h of stage st, one a byte.
+    static __device__ __forceinline__ uint32_t scales(const char* chunks, int row, int st, int h) {
+        const u32x2_t v = *(const u32x2_t*)(chunks + (st >> 1 & 1) * CHUNK_BYTES + row * 16 + (st & 1) * 8);
+        return __builtin_amdgcn_perm(v[1], v[0], h ? 0x07050301u : 0x06040200u);
+    }
 };
 
 template <int FP, int WP, int FQ, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearArgs a) {
-    using T = Mx4Tile<FP, WP, FQ, WQ, 1>;
+    using T = Mx4Tile<FP, WP, FQ, WQ>;
     extern __shared__ __align__(16) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int nb = mx4_blocks(a.k), stages = (nb + 7) / 8;
     const int n_tiles = (a.n + T::TP - 1) / T::TP;
     const int n0 = (int)(blockIdx.x % n_tiles) * T::TP;
     const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * T::TQ;
     const int wp = wave / WQ * 32 * FP, wq = wave % WQ * 32 * FQ;
+    const uint32_t pitch = (uint32_t)nb * MX4_BLOCK_BYTES, lds0 = lds_address(lds);
+    const char *P = (const char*)a.w + (int64_t)n0 * pitch, *Q = (const char*)a.x + m0 * pitch;
+    const int p_last = a.n - 1 - n0, q_last = (int)min((int64_t)T::TQ, a.m - m0) - 1;     // last row that is there
+    // this lane's part of a stage: one block of some rows
+    const int my_row = 8 * wave + (lane >> 3), my_block = (lane & 7) ^ (my_row >> 1 & 7);
+    uint32_t p_at[T::LOADS_P], q_at[T::LOADS_Q];
+#pragma unroll
+    for (int i = 0; i < T::LOADS_P; ++i) p_at[i] = (uint32_t)min(my_row + 8 * T::WAVES * i, p_last) * pitch;
+#pragma unroll
+    for (int i = 0; i < T::LOADS_Q; ++i) q_at[i] = (uint32_t)min(my_row + 8 * T::WAVES * i, q_last) * pitch;
+    auto fetch = [&](int st) {
+        const uint32_t to = lds0 + (uint32_t)(st % T::STAGES) * T::STAGE_BYTES + wave * 1024;
+        const uint32_t block = (uint32_t)min(st * 8 + my_block, nb - 1) * MX4_BLOCK_BYTES;
+#pragma unroll
+        for (int i = 0; i < T::LOADS_P; ++i) dma16(to + i * T::WAVES * 1024, P, p_at[i] + block);
+#pragma unroll
+        for (int i = 0; i < T::LOADS_Q; ++i) dma16(to + T::TP * T::ROW_BYTES + i * T::WAVES * 1024, Q, q_at[i] + block);
+    };
+    // this thread's rows of a chunk of scales
+    const uint8_t* scale_row[T::CHUNK_ROWS];
+    u32x4_t chunk[T::CHUNK_ROWS];
+#pragma unroll
+    for (int i = 0; i < T::CHUNK_ROWS; ++i) {
+        const int r = threadIdx.x + 64 * T::WAVES * i;
+        scale_row[i] = r < T::TP ? a.w_scales + (int64_t)(n0 + min(r, p_last)) * nb : a.x_scales + (m0 + min(r - T::TP, q_last)) * nb;
+    }
+    auto fetch_chunk = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < T::CHUNK_ROWS; ++i) chunk[i] = T::chunk(scale_row[i], c, nb);
+    };
+    auto store_chunk = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < T::CHUNK_ROWS; ++i)
+            *(u32x4_t*)(lds + T::SCALES_AT + (c & 1) * T::CHUNK_BYTES + (threadIdx.x + 64 * T::WAVES * i) * 16) = chunk[i];
+    };
+    const int p_row = wp + (lane & 31), q_row = T::TP + wq + (lane & 31);
+    uint32_t sp[FP], sq[FQ];
+    auto take_scales = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < FP; ++i) sp[i] = T::scales(lds + T::SCALES_AT, p_row + 32 * i, st, h);
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) sq[j] = T::scales(lds + T::SCALES_AT, q_row + 32 * j, st, h);
+    };
     float16_t_ acc[FP][FQ];
 #pragma unroll
     for (int i = 0; i < FP; ++i)
@@ -200,60 +290,310 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
         for (int j = 0; j < FQ; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    for (int st = 0; st < stages; ++st) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < (T::TP + T::TQ) * 8; c += 64 * T::WAVES) {
-            const int r = c >> 3, b = st * 8 + (c & 7);
-            u32x4_t v = {0, 0, 0, 0};
-            if (b < nb) {
-                if (r < T::TP) { if (n0 + r < a.n) v = *(const u32x4_t*)(a.w + ((int64_t)(n0 + r) * nb + b) * 16); }
-                else if (m0 + r - T::TP < a.m) v = *(const u32x4_t*)(a.x + ((m0 + r - T::TP) * nb + b) * 16);
-            }
-            *(u32x4_t*)(lds + r * T::ROW_BYTES + (((c & 7) ^ (r >> 1 & 7)) * 16)) = v;
-        }
-        __syncthreads();
-        uint32_t sp[FP][4], sq[FQ][4];
+    auto multiply = [&](const typename T::Frags& f, auto step) {
+        constexpr int s = decltype(step)::value;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int b = st * 8 + 2 * s + h;
+        for (int i = 0; i < FP; ++i)
 #pragma unroll
-            for (int i = 0; i < FP; ++i) {
-                const int r = n0 + wp + 32 * i + (lane & 31);
-                sp[i][s] = b < nb && r < a.n ? a.w_scales[(int64_t)r * nb + b] : 127u;
-            }
+            for (int j = 0; j < FQ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(f.p[i]), mx4_operand(f.q[j]), acc[i][j], 4, 4,
+                                                                           s, (int)sp[i], s, (int)sq[j]);
+    };
+    using S0 = std::integral_constant<int, 0>; using S1 = std::integral_constant<int, 1>;
+    using S2 = std::integral_constant<int, 2>; using S3 = std::integral_constant<int, 3>;
+    typename T::Frags f0, f1;
+    float* bias_lds = (float*)(lds + T::BIAS_AT);
+    for (int c = threadIdx.x; c < T::TP; c += 64 * T::WAVES) bias_lds[c] = a.bias && c <= p_last ? a.bias[n0 + c] : 0.f;
+    fetch_chunk(0);
+    store_chunk(0);
+    fetch(0);
+    landed<0>();
+    if (stages > 1) fetch(1);
+    take_scales(0);
+    T::read(f0, lds, 0, p_row, q_row, h);
+    for (int st = 0; st < stages - 1; ++st) {
+        const char* buf = lds + (st % T::STAGES) * T::STAGE_BYTES;
+        const bool new_chunk = (st & 1) && st + 1 < stages;    // the next stage begins a chunk
+        if (new_chunk) fetch_chunk((st + 1) >> 1);
+        __builtin_amdgcn_sched_barrier(0);                     // on its way for the whole stage
+        T::read(f1, buf, 1, p_row, q_row, h);
+        multiply(f0, S0{});
+        T::read(f0, buf, 2, p_row, q_row, h);
+        multiply(f1, S1{});
+        T::read(f1, buf, 3, p_row, q_row, h);
+        multiply(f0, S2{});
+        // The compiler does not know of the loads into LDS and waits for its own as if they were the only ones: the chunk has
+        // to be put away before the next of those are sent out, or it would wait for them all.
+        if (new_chunk) store_chunk((st + 1) >> 1);
+        landed<0>();                                           // the next stage is there, and every wave has read all of this one
+        if (st + 2 < stages) fetch(st + 2);
+        T::read(f0, lds + ((st + 1) % T::STAGES) * T::STAGE_BYTES, 0, p_row, q_row, h);
+        multiply(f1, S3{});
+        take_scales(st + 1);
+    }
+    const char* buf = lds + ((stages - 1) % T::STAGES) * T::STAGE_BYTES;
+    const int left = nb - 8 * (stages - 1);                    // blocks of the last stage
+    auto clear = [&](typename T::Frags& f, int s) {
+        if (2 * s + h >= left)
 #pragma unroll
-            for (int j = 0; j < FQ; ++j) {
-                const int64_t r = m0 + wq + 32 * j + (lane & 31);
-                sq[j][s] = b < nb && r < a.m ? a.x_scales[r * nb + b] : 127u;
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (st * 8 + 2 * s >= nb) break;
-            u32x4_t fp[FP], fq[FQ];
-#pragma unroll
-            for (int i = 0; i < FP; ++i) {
-                const int r = wp + 32 * i + (lane & 31);
-                fp[i] = *(const u32x4_t*)(lds + r * T::ROW_BYTES + (((2 * s + h) ^ (r >> 1 & 7)) * 16));
-            }
-#pragma unroll
-            for (int j = 0; j < FQ; ++j) {
-                const int r = T::TP + wq + 32 * j + (lane & 31);
-                fq[j] = *(const u32x4_t*)(lds + r * T::ROW_BYTES + (((2 * s + h) ^ (r >> 1 & 7)) * 16));
-            }
-#pragma unroll
-            for (int i = 0; i < FP; ++i)
-#pragma unroll
-                for (int j = 0; j < FQ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(fp[i]), mx4_operand(fq[j]), acc[i][j], 4, 4,
-                                                                               0, (int)sp[i][s], 0, (int)sq[j][s]);
+            for (int i = 0; i < FP; ++i) f.p[i] = {0, 0, 0, 0};
+    };
+    clear(f0, 0);
+    T::read(f1, buf, 1, p_row, q_row, h);
+    multiply(f0, S0{});
+    if (left > 2) {
+        clear(f1, 1);
+        multiply(f1, S1{});
+    }
+    if (left > 4) {
+        T::read(f0, buf, 2, p_row, q_row, h);
+        T::read(f1, buf, 3, p_row, q_row, h);
+        clear(f0, 2);
+        multiply(f0, S2{});
+        if (left > 6) {
+            clear(f1, 3);
+            multiply(f1, S3{});
         }
     }
+    // row by row of y: the runs of one row that neighbouring tiles write follow each other
 #pragma unroll
-    for (int i = 0; i < FP; ++i)
+    for (int j = 0; j < FQ; ++j)
 #pragma unroll
-        for (int j = 0; j < FQ; ++j)
-            if (n0 + wp + 32 * i < a.n) mx4_store(a, acc[i][j], m0 + wq + 32 * j, n0 + wp + 32 * i);
+        for (int i = 0; i < FP; ++i) {
+            const int n = n0 + wp + 32 * i;
+            if (n >= a.n) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_t b = *(const f32x4_t*)(bias_lds + wp + 32 * i + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += b[e];
+            }
+            mx4_store(a, acc[i][j], m0 + wq + 32 * j, n);
+        }
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------
+// Up to 64 rows of x: the weight is read once and nothing else counts.  A workgroup takes 16 rows of W, its waves parts
+// of K; each lane's 16-byte load is a block of W, which is an operand of the matrix instruction as it
+// is (16 x 16 x 128).  Rows of x in a float type are quantised by the workgroup into LDS, a block a thread, while the first
+// loads of W are on their way.
+constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024;
+
+// One block of x, 32 values: whole blocks from aligned memory (MX4_FULL), whole pieces of 16 bytes from aligned memory
+// (MX4_PIECES), or value by value; zeros behind k.
+enum { MX4_VALUES, MX4_PIECES, MX4_FULL };
+template <int DT>
+__device__ __forceinline__ Mx4Raw<DT, 32> mx4_load_block(const char* row, int at, int k, int how) {
+    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, PIECE = 16 / SIZE;
+    Mx4Raw<DT, 32> v;
+    if (how == MX4_FULL) {
+#pragma unroll
+        for (int i = 0; i < 32 / PIECE; ++i) {
+            const u32x4_t p = *(const u32x4_t*)(row + (at + i * PIECE) * SIZE);
+            v.w[4 * i] = p[0]; v.w[4 * i + 1] = p[1]; v.w[4 * i + 2] = p[2]; v.w[4 * i + 3] = p[3];
+        }
+    } else if (how == MX4_PIECES) {
+#pragma unroll
+        for (int i = 0; i < 32 / PIECE; ++i) {
+            u32x4_t p = {0, 0, 0, 0};
+            if (at + i * PIECE < k) p = *(const u32x4_t*)(row + (at + i * PIECE) * SIZE);
+            v.w[4 * i] = p[0]; v.w[4 * i + 1] = p[1]; v.w[4 * i + 2] = p[2]; v.w[4 * i + 3] = p[3];
+        }
+    } else if constexpr (SIZE == 4) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v.w[i] = at + i < k ? *(const uint32_t*)(row + (at + i) * 4) : 0u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t lo = at + 2 * i < k ? *(const uint16_t*)(row + (at + 2 * i) * 2) : 0u;
+            const uint32_t hi = at + 2 * i + 1 < k ? *(const uint16_t*)(row + (at + 2 * i + 1) * 2) : 0u;
+            v.w[i] = lo | hi << 16;
+        }
+    }
+    return v;
+}
+
+__device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
+    const float v = mx4_activate(acc + (a.bias ? a.bias[n] : 0.f), a.activ);
+    const int64_t at = m * a.n + n;
+    if (a.y_dtype == NERFX_TYPE_F32) ((float*)a.y)[at] = v;
+    else if (a.y_dtype == NERFX_TYPE_BF16) ((__bf16*)a.y)[at] = (__bf16)v;
+    else ((_Float16*)a.y)[at] = (_Float16)v;
+}
+
+template <int DT, int MT>
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4LinearArgs a, int how) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr bool FLOAT = DT != NERFX_TYPE_MX4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int nb = mx4_blocks(a.k), m = (int)a.m;
+    const int n0 = blockIdx.x * 16, row = min(n0 + l16, a.n - 1);
+    const int steps = (nb + 3) / 4, per = (steps + SKINNY_WAVES - 1) / SKINNY_WAVES;
+    const int first = min(wave * per, steps), last = min(first + per, steps);
+    const u32x4_t* w = (const u32x4_t*)a.w + (int64_t)row * nb;
+    const uint8_t* ws = a.w_scales + (int64_t)row * nb;
+    u32x4_t wc[SKINNY_AHEAD];
+    uint32_t wsc[SKINNY_AHEAD];
+    auto fetch = [&](int step, u32x4_t& c, uint32_t& s) {
+        const int b = min(4 * step + g, nb - 1);               // behind the last block x has zeros
+        c = __builtin_nontemporal_load(w + b);
+        s = ws[b];
+    };
+#pragma unroll
+    for (int u = 0; u < SKINNY_AHEAD; ++u)
+        if (first + u < last) fetch(first + u, wc[u], wsc[u]);
+    if constexpr (FLOAT) {
+        using Raw = Mx4Raw<DT, 32>;
+        for (int q = threadIdx.x; q < m * nb; q += 64 * SKINNY_WAVES) {
+            const int r = q / nb, b = q - r * nb;
+            const Raw v = mx4_load_block<DT>((const char*)a.x + (int64_t)r * a.k * (DT == NERFX_TYPE_F32 ? 4 : 2), b * 32, a.k, how);
+            const uint32_t byte = Raw::scale_byte(v.top_bits());
+            const float scale = Raw::scale_value(byte);
+            *(u32x4_t*)(lds + q * 16) = {v.codes(0, scale), v.codes(1, scale), v.codes(2, scale), v.codes(3, scale)};
+            *(uint8_t*)(lds + m * nb * 16 + q) = (uint8_t)byte;
+        }
+        __syncthreads();
+    }
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = {0.f, 0.f, 0.f, 0.f};
+    for (int base = first; base < last; base += SKINNY_AHEAD) {
+#pragma unroll
+        for (int u = 0; u < SKINNY_AHEAD; ++u) {
+            const int step = base + u;
+            if (step >= last) break;
+            const u32x4_t c = wc[u];
+            const uint32_t s = wsc[u];
+            if (step + SKINNY_AHEAD < last) fetch(step + SKINNY_AHEAD, wc[u], wsc[u]);
+            const int b = 4 * step + g;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int r = 16 * t + l16;
+                u32x4_t xc = {0, 0, 0, 0};
+                uint32_t xs = 127u;
+                if (r < m && b < nb) {
+                    const int q = r * nb + b;
+                    if constexpr (FLOAT) {
+                        xc = *(const u32x4_t*)(lds + q * 16);
+                        xs = *(const uint8_t*)(lds + m * nb * 16 + q);
+                    } else {
+                        xc = *((const u32x4_t*)a.x + q);
+                        xs = a.x_scales[q];
+                    }
+                }
+                acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx4_operand(c), mx4_operand(xc), acc[t], 4, 4, 0, (int)s, 0, (int)xs);
+            }
+        }
+    }
+    // sums of the waves' parts of K, in their order; element i of a lane: row m = lane % 16, column n = 4 (lane / 16) + i
+    __syncthreads();
+    f32x4_t* part = (f32x4_t*)lds;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[(wave * MT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    for (int o = threadIdx.x; o < MT * 64; o += 64 * SKINNY_WAVES) {
+        f32x4_t sum = part[o];
+#pragma unroll
+        for (int v = 1; v < SKINNY_WAVES; ++v) sum += part[v * MT * 64 + o];
+        const int r = 16 * (o >> 6) + (o & 15), n = n0 + 4 * ((o & 63) >> 4);
+        if (r >= m) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < a.n) mx4_store_one(a, r, n + i, sum[i]);
+    }
+}
+
+// ---- many rows, few columns ------------------------------------------------------------------------------------------
+// Up to 256 columns and 512 values a row: a layer of a field for a batch of samples.  Bound by memory: x is read once, in
+// whatever type it has, and y written once.  W stays in LDS (its rows (2 KS + 1) * 16 bytes apart: sixteen rows of a read on
+// sixteen different banks); a wave takes 32 rows of x, a lane two blocks of every 64 values of its row, quantises them in
+// registers, where they are operands of the matrix instruction as they are, and goes over W's columns.
+constexpr int STREAM_WAVES = 8, STREAM_ROWS = 32 * STREAM_WAVES;
+
+__host__ __device__ inline int stream_row_bytes(int ks) { return (2 * ks + 1) * 16; }
+__host__ __device__ inline int stream_scale_bytes(int ks) { return ks > 4 ? 16 : 8; }      // both halves of a row
+__host__ __device__ inline int stream_lds(int ks, int columns) {
+    return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4);
+}
+
+template <int DT, int KS>
+__global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4LinearArgs a, int columns) {
+    extern __shared__ __align__(16) char lds[];
+    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, SB = KS > 4 ? 8 : 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int nb = mx4_blocks(a.k), c0 = blockIdx.y * columns;
+    char* scale_lds = lds + columns * stream_row_bytes(KS);
+    float* bias_lds = (float*)(scale_lds + columns * stream_scale_bytes(KS));
+    for (int c = threadIdx.x; c < columns; c += 64 * STREAM_WAVES) bias_lds[c] = a.bias && c0 + c < a.n ? a.bias[c0 + c] : 0.f;
+    for (int c = threadIdx.x; c < columns * 2 * KS; c += 64 * STREAM_WAVES) {
+        const int r = c / (2 * KS), b = c - r * 2 * KS;
+        u32x4_t v = {0, 0, 0, 0};
+        uint32_t s = 127u;
+        if (c0 + r < a.n && b < nb) {
+            v = *((const u32x4_t*)a.w + (int64_t)(c0 + r) * nb + b);
+            s = a.w_scales[(int64_t)(c0 + r) * nb + b];
+        }
+        *(u32x4_t*)(lds + r * stream_row_bytes(KS) + b * 16) = v;
+        scale_lds[r * 2 * SB + (b & 1) * SB + (b >> 1)] = (char)s;
+    }
+    __syncthreads();
+    for (int64_t m0 = (int64_t)blockIdx.x * STREAM_ROWS + 32 * wave; m0 < a.m; m0 += (int64_t)gridDim.x * STREAM_ROWS) {
+        const int64_t m = min(m0 + (lane & 31), a.m - 1);
+        u32x4_t xc[KS];
+        uint32_t xs[(KS + 3) / 4] = {};
+        if constexpr (DT == NERFX_TYPE_MX4) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                xc[s] = {0, 0, 0, 0};
+                uint32_t byte = 127u;
+                if (2 * s + h < nb) {
+                    xc[s] = *((const u32x4_t*)a.x + m * nb + 2 * s + h);
+                    byte = a.x_scales[m * nb + 2 * s + h];
+                }
+                xs[s / 4] |= byte << (8 * (s & 3));
+            }
+        } else {
+            using Raw = Mx4Raw<DT, 32>;
+            constexpr int AT_ONCE = DT == NERFX_TYPE_F32 ? 2 : 4;          // as many loads in flight as registers allow
+#pragma unroll
+            for (int s0 = 0; s0 < KS; s0 += AT_ONCE) {
+                Raw raw[AT_ONCE];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u)
+                    if (s0 + u < KS) raw[u] = mx4_load_block<DT>((const char*)a.x + m * a.k * SIZE, (2 * (s0 + u) + h) * 32, a.k, MX4_FULL);
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    if (s0 + u >= KS) break;
+                    const int s = s0 + u;
+                    const uint32_t byte = Raw::scale_byte(raw[u].top_bits());
+                    const float scale = Raw::scale_value(byte);
+                    xc[s] = {raw[u].codes(0, scale), raw[u].codes(1, scale), raw[u].codes(2, scale), raw[u].codes(3, scale)};
+                    xs[s / 4] |= byte << (8 * (s & 3));
+                }
+                if (KS > AT_ONCE) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        for (int n = 0; n < columns; n += 32) {
+            const int r = n + (lane & 31);
+            const char* wr = lds + r * stream_row_bytes(KS) + h * 16;
+            uint32_t ws[SB / 4];
+            ws[0] = *(const uint32_t*)(scale_lds + r * 2 * SB + h * SB);
+            if constexpr (SB == 8) ws[1] = *(const uint32_t*)(scale_lds + r * 2 * SB + h * SB + 4);
+            float16_t_ acc;                                        // begins as the bias
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_t b = *(const f32x4_t*)(bias_lds + n + 8 * q + 4 * h);
+                acc[4 * q] = b[0]; acc[4 * q + 1] = b[1]; acc[4 * q + 2] = b[2]; acc[4 * q + 3] = b[3];
+            }
+#define NERFX_STEP(s)                                                                                                                  \
+            if constexpr (s < KS)                                                                                                      \
+                acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(*(const u32x4_t*)(wr + s * 32)), mx4_operand(xc[s < KS ? s : 0]), acc, \
+                                                                      4, 4, s & 3, (int)ws[s / 4 < SB / 4 ? s / 4 : 0], s & 3, (int)xs[s / 4 < (KS + 3) / 4 ? s / 4 : 0]);
+            NERFX_STEP(0) NERFX_STEP(1) NERFX_STEP(2) NERFX_STEP(3) NERFX_STEP(4) NERFX_STEP(5) NERFX_STEP(6) NERFX_STEP(7)
+#undef NERFX_STEP
+            mx4_store(a, acc, m0, c0 + n);
+        }
+    }
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -272,12 +612,80 @@ static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_
 
 template <int FP, int WP, int FQ, int WQ>
 static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
-    using T = Mx4Tile<FP, WP, FQ, WQ, 1>;
+    using T = Mx4Tile<FP, WP, FQ, WQ>;
     const int64_t tiles = ((a.n + T::TP - 1) / T::TP) * ((a.m + T::TQ - 1) / T::TQ);
     NERFX_REQUIRE(tiles <= 1 << 22, "%lld x %d results are too many for one launch", (long long)a.m, a.n);
     NERFX_OPT_IN_LDS((mx4_tile_kernel<FP, WP, FQ, WQ>), T::LDS_BYTES);
     hipLaunchKernelGGL((mx4_tile_kernel<FP, WP, FQ, WQ>), dim3((unsigned)tiles), dim3(64 * T::WAVES), T::LDS_BYTES, stream, a);
     return launch_status("mx4_tile_kernel");
+}
+
+// How a product is done, by its sizes:
+//  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes: W is read once, by as many workgroups as it has
+//          rows (one row by 4096 x 4096: 62 us with tiles);
+//  stream  otherwise up to 256 columns and 512 values a row: float rows of 64, 128, 192, 256, 320 or 512 values are quantised in
+//          registers, others into the workspace first;
+//  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.
+enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
+// Steps of 64 values that a row is worked on in: what the stream kernel is made for.
+static int stream_steps(int k) {
+    const int ks = (k + 63) / 64;
+    return ks <= 5 ? ks : 8;
+}
+static int mx4_plan(int64_t m, int n, int k, int x_dtype, bool& stage) {
+    const bool is_float = x_dtype != NERFX_TYPE_MX4;
+    stage = false;
+    if (m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
+    if (n <= 256 && k <= 512 && m > SKINNY_ROWS) {
+        stage = is_float && k != 64 * stream_steps(k);
+        return MX4_STREAM;
+    }
+    stage = is_float;
+    return m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
+}
+
+template <int DT>
+static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
+    const int mt = (int)(a.m + 15) / 16, nb = mx4_blocks(a.k);
+    const size_t codes = DT == NERFX_TYPE_MX4 ? 0 : (size_t)a.m * nb * 17, sums = (size_t)SKINNY_WAVES * mt * 1024;
+    const size_t lds = std::max(codes, sums);
+    const int how = a.k % 32 == 0 ? MX4_FULL : a.k % (DT == NERFX_TYPE_F32 ? 4 : 8) == 0 ? MX4_PIECES : MX4_VALUES;
+    const dim3 grid((unsigned)((a.n + 15) / 16)), block(64 * SKINNY_WAVES);
+    auto go = [&](auto kernel) {
+        NERFX_OPT_IN_LDS(kernel, lds);
+        hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, how);
+        return launch_status("mx4_skinny_kernel");
+    };
+    switch (mt) {
+        case 1: return go(mx4_skinny_kernel<DT, 1>);
+        case 2: return go(mx4_skinny_kernel<DT, 2>);
+        case 3: return go(mx4_skinny_kernel<DT, 3>);
+        default: return go(mx4_skinny_kernel<DT, 4>);
+    }
+}
+
+template <int DT>
+static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
+    const int64_t row_tiles = (a.m + STREAM_ROWS - 1) / STREAM_ROWS;
+    // few rows: the columns are spread over workgroups until the device is full
+    const int tiles = (a.n + 31) / 32;
+    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, row_tiles * tiles / 256));
+    const int columns = 32 * per;
+    const dim3 grid((unsigned)std::min<int64_t>(row_tiles, 512), (unsigned)((tiles + per - 1) / per)), block(64 * STREAM_WAVES);
+    auto go = [&](auto kernel, int ks) {
+        const size_t lds = stream_lds(ks, columns);
+        NERFX_OPT_IN_LDS(kernel, lds);
+        hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, columns);
+        return launch_status("mx4_stream_kernel");
+    };
+    switch (stream_steps(a.k)) {
+        case 1: return go(mx4_stream_kernel<DT, 1>, 1);
+        case 2: return go(mx4_stream_kernel<DT, 2>, 2);
+        case 3: return go(mx4_stream_kernel<DT, 3>, 3);
+        case 4: return go(mx4_stream_kernel<DT, 4>, 4);
+        case 5: return go(mx4_stream_kernel<DT, 5>, 5);
+        default: return go(mx4_stream_kernel<DT, 8>, 8);
+    }
 }
 
 static int check_mx4(int64_t rows, int k) {
@@ -319,7 +727,9 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
 
 extern "C" int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype) {
     if (check_mx4(m, k) || check_mx4(n, k) || !(float_type(x_dtype) || x_dtype == NERFX_TYPE_MX4)) return -1;
-    if (x_dtype == NERFX_TYPE_MX4) return 0;
+    bool stage;
+    mx4_plan(m, n, k, x_dtype, stage);
+    if (!stage) return 0;
     return (m * mx4_blocks(k) * 17 + 15) / 16 * 16;
 }
 
@@ -333,7 +743,7 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
     NERFX_REQUIRE(activ >= NERFX_ACT_NONE && activ <= NERFX_ACT_SILU, "unknown activation %d", activ);
     if (m == 0 || n == 0) return 0;
     NERFX_REQUIRE(x && w_codes && w_scales && y && (x_dtype != NERFX_TYPE_MX4 || x_scales), "a required pointer is NULL");
-    NERFX_REQUIRE(aligned16(w_codes) && (x_dtype != NERFX_TYPE_MX4 || aligned16(x)), "codes are not aligned to 16 bytes");
+    NERFX_REQUIRE(aligned16(w_codes) && aligned16(x), "x or the weight's codes are not aligned to 16 bytes");
     const int64_t need = nerfx_mx4_linear_workspace_bytes(m, n, k, x_dtype);
     NERFX_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
                   "workspace NULL, not aligned to 16 bytes, or of %lld bytes with %lld needed", (long long)workspace_bytes, (long long)need);
@@ -342,11 +752,25 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
     a.m = m; a.n = n; a.k = k; a.activ = activ; a.y_dtype = y_dtype;
     a.y_whole = aligned16(y) && n % (y_dtype == NERFX_TYPE_F32 ? 4 : 8) == 0;
     a.x = (const uint8_t*)x; a.x_scales = x_scales;
-    if (x_dtype != NERFX_TYPE_MX4) {
+    const hipStream_t st = (hipStream_t)stream;
+    bool stage;
+    const int plan = mx4_plan(m, n, k, x_dtype, stage);
+    if (stage) {
         uint8_t* codes = (uint8_t*)workspace;
         uint8_t* scales = codes + m * mx4_blocks(k) * 16;
-        if (int rc = quantize_launch(x, x_dtype, m, k, codes, scales, (hipStream_t)stream)) return rc;
+        if (int rc = quantize_launch(x, x_dtype, m, k, codes, scales, st)) return rc;
         a.x = codes; a.x_scales = scales;
+        x_dtype = NERFX_TYPE_MX4;
     }
-    return tile_launch<2, 2, 2, 2>(a, (hipStream_t)stream);
+    if (plan == MX4_TILE) {
+        const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+        return big >= 192 ? tile_launch<4, 2, 2, 4>(a, st) : tile_launch<2, 2, 2, 2>(a, st);
+    }
+    auto by_type = [&](auto skinny, auto str) { return plan == MX4_SKINNY ? skinny(a, st) : str(a, st); };
+    switch (x_dtype) {
+        case NERFX_TYPE_F32: return by_type(skinny_launch<NERFX_TYPE_F32>, stream_launch<NERFX_TYPE_F32>);
+        case NERFX_TYPE_BF16: return by_type(skinny_launch<NERFX_TYPE_BF16>, stream_launch<NERFX_TYPE_BF16>);
+        case NERFX_TYPE_F16: return by_type(skinny_launch<NERFX_TYPE_F16>, stream_launch<NERFX_TYPE_F16>);
+        default: return by_type(skinny_launch<NERFX_TYPE_MX4>, stream_launch<NERFX_TYPE_MX4>);
+    }
 }

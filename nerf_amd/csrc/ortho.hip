@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "lds_dma.hpp"
 #include "split16.hpp"
 
 namespace nerfx {
@@ -166,17 +167,6 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
 // their way while one is worked on (LDS-DMA: no registers hold them).  16-byte chunk c of row r lies at place
 // c ^ (r / 2 % 8), so that the sixteen rows a ds_read_b128 phase touches (256 bytes of banks) lie apart; LDS-DMA
 // writes lane after lane, so it is the source address that is permuted.
-// 64 lanes x 16 bytes from base + offset (per lane) to LDS at `lds` + 16 * lane.  The compiler does not know of the
-// load: whoever reads the LDS waits with landed().
-__device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
-}
-// All but the newest N of this wave's loads are done, and so are its LDS reads: then, behind the barrier, so are every wave's.
-template <int N>
-__device__ __forceinline__ void landed() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
 template <int T, int WAVES, int STAGES>
 struct SplitTile {
     static constexpr int FP = T / 64, FQ = T / (16 * WAVES); // 32 x 32 fragments per wave and side
@@ -210,6 +200,7 @@ struct SplitTile {
         for (int i = 0; i < FP; ++i) { f.ph[i] = frag(p_row + 32 * i, c); f.pl[i] = frag(p_row + 32 * i, c + 4); }
 #pragma unroll
         for (int j = 0; j < FQ; ++j) { f.qh[j] = frag(q_row + 32 * j, c); f.ql[j] = frag(q_row + 32 * j, c + 4); }
+        __builtin_amdgcn_sched_barrier(0);                   // in front of the products of the half before, not behind them
     }
     // the three products of a fragment lie apart, so that no instruction waits for the one before
     __device__ __forceinline__ void multiply(const Frags& f) {
@@ -227,7 +218,7 @@ struct SplitTile {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t pitch = (uint32_t)K / SPLIT_BLOCK * SPLIT_BLOCK_BYTES;
         const int steps = K / SPLIT_BLOCK;
-        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        const uint32_t lds0 = lds_address(lds);
         // this lane's 16 bytes of the first of the rows that the wave's loads bring; the others lie 8 WAVES rows apart
         const int row = 8 * wave + (lane >> 3);
         const uint32_t offset = (uint32_t)row * pitch + ((lane & 7) ^ (row >> 1 & 7)) * 16;
