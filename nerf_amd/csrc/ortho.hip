@@ -200,7 +200,6 @@ struct SplitTile {
         for (int i = 0; i < FP; ++i) { f.ph[i] = frag(p_row + 32 * i, c); f.pl[i] = frag(p_row + 32 * i, c + 4); }
 #pragma unroll
         for (int j = 0; j < FQ; ++j) { f.qh[j] = frag(q_row + 32 * j, c); f.ql[j] = frag(q_row + 32 * j, c + 4); }
-        __builtin_amdgcn_sched_barrier(0);                   // in front of the products of the half before, not behind them
     }
     // the three products of a fragment lie apart, so that no instruction waits for the one before
     __device__ __forceinline__ void multiply(const Frags& f) {
@@ -365,7 +364,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoAr
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-// Tile side: 128 halves the operand traffic of 64, but only pays where its tiles fill the device.
+// Sides are padded to whole tiles: of 128 where there is enough work for them somewhere, else of 64.
 static int tile_side(const nerfx_matrix_t* mats, int count) {
     int64_t big = 0;
     for (int k = 0; k < count; ++k) {
@@ -429,46 +428,68 @@ static int scales_for(const float* coef, int steps, OrthoScales& s) {
     return 0;
 }
 
-template <int T, int WAVES, int STAGES>
-static int ortho_run(OrthoArgs& a, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
-    // a launch's grid is the matrices' blocks one after the other
-    auto grid = [&](auto blocks_of) {
-        int64_t at = 0;
-        for (int k = 0; k < ORTHO_GROUP; ++k) {
-            a.first[k] = k < a.count ? (int32_t)at : INT32_MAX;
-            if (k < a.count) at += blocks_of(a.mat[k]);
-        }
-        return dim3((unsigned)at);
-    };
-    auto symmetric = [](const OrthoMat& q) { return (int64_t)(q.m / T) * (q.m / T + 1) / 2; };
-    auto whole = [](const OrthoMat& q) { return (int64_t)(q.m / T) * (q.n / T); };
-    const dim3 block(256), product(64 * WAVES);
-    const size_t lds = SplitTile<T, WAVES, STAGES>::LDS_BYTES;
-    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_GRAM>), lds);
-    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_POLY>), lds);
-    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_APPLY>), lds);
-    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, ORTHO_LAST>), lds);
+// A launch's grid is the matrices' blocks one after the other.
+template <class F>
+static int64_t lay_out(OrthoArgs& a, F blocks_of) {
+    int64_t at = 0;
+    for (int k = 0; k < ORTHO_GROUP; ++k) {
+        a.first[k] = k < a.count ? (int32_t)at : INT32_MAX;
+        if (k < a.count) at += blocks_of(a.mat[k]);
+    }
+    return at;
+}
+
+template <int KIND>
+static int64_t product_blocks(OrthoArgs& a, int tile) {
+    return lay_out(a, [tile](const OrthoMat& q) {
+        const int64_t mt = q.m / tile;
+        return KIND == ORTHO_GRAM || KIND == ORTHO_POLY ? mt * (mt + 1) / 2 : mt * (q.n / tile);
+    });
+}
+
+template <int T, int WAVES, int STAGES, int KIND>
+static int product_as(const OrthoArgs& a, int64_t blocks, hipStream_t stream) {
+    constexpr size_t lds = SplitTile<T, WAVES, STAGES>::LDS_BYTES;
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, KIND>), lds);
+    hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, KIND>), dim3((unsigned)blocks), dim3(64 * WAVES), lds, stream, a);
+    return 0;
+}
+
+// The tile a product takes, by how many of them there are:
+//  128  where whole rounds of them fill at least four fifths of the 256 CUs: half of the operand traffic of 64
+//       (2048 x 2048 by 2048: 50 us; 55 in tiles of 64);
+//  64   with two stages, five workgroups to a CU, where they would not: of a symmetric result 136 tiles of 128 take as long as
+//       all 256 (50 us), 528 of 64 take 41; three and four stages hold fewer workgroups and take 44 and 50;
+//  64   with eight stages where there is at most one to a CU: all of a K of 256 is on its way at once.
+template <int KIND>
+static int product(OrthoArgs& a, int pad, hipStream_t stream) {
+    if (pad == 128) {
+        const int64_t blocks = product_blocks<KIND>(a, 128), rounds = (blocks + 255) / 256;
+        if (blocks * 5 >= rounds * 256 * 4) return product_as<128, 8, 4, KIND>(a, blocks, stream);
+    }
+    const int64_t blocks = product_blocks<KIND>(a, 64);
+    return blocks <= 256 ? product_as<64, 4, 8, KIND>(a, blocks, stream) : product_as<64, 4, 2, KIND>(a, blocks, stream);
+}
+
+static int ortho_run(OrthoArgs& a, int pad, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
     a.x_scale = s.x;
     a.growth = s.growth;
-    dim3 g = grid([](const OrthoMat& q) { return (int64_t)norm_parts(q); });
-    hipLaunchKernelGGL(ortho_norm_kernel, g, block, 0, stream, a);
-    g = grid([](const OrthoMat& q) { return (int64_t)(q.m / PREP_TILE) * (q.n / PREP_TILE); });
-    hipLaunchKernelGGL(ortho_prep_kernel, g, block, 0, stream, a);
+    int64_t blocks = lay_out(a, [](const OrthoMat& q) { return (int64_t)norm_parts(q); });
+    hipLaunchKernelGGL(ortho_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    blocks = lay_out(a, [](const OrthoMat& q) { return (int64_t)(q.m / PREP_TILE) * (q.n / PREP_TILE); });
+    hipLaunchKernelGGL(ortho_prep_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
     for (int k = 0; k < steps; ++k) {
         const float ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
-        g = grid(symmetric);
         a.beta = s.a / (s.x * s.x);
-        hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_GRAM>), g, product, lds, stream, a);
+        if (int rc = product<ORTHO_GRAM>(a, pad, stream)) return rc;
         a.alpha = cb * (s.b / s.a);
         a.beta = cc * (s.b / s.a / s.a);
-        hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_POLY>), g, product, lds, stream, a);
-        g = grid(whole);
+        if (int rc = product<ORTHO_POLY>(a, pad, stream)) return rc;
         a.from = k & 1; a.to = a.from ^ 1;
         const bool last = k == steps - 1;
         a.alpha = last ? ca / s.x : ca;                       // the last step leaves the scale
         a.beta = last ? 1.0f / (s.b * s.x) : 1.0f / s.b;
-        if (last) hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_LAST>), g, product, lds, stream, a);
-        else hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, ORTHO_APPLY>), g, product, lds, stream, a);
+        if (int rc = last ? product<ORTHO_LAST>(a, pad, stream) : product<ORTHO_APPLY>(a, pad, stream)) return rc;
     }
     return launch_status("orthogonalisation kernels");
 }
@@ -502,7 +523,7 @@ static int ortho_groups(const nerfx_matrix_t* mats, int count, OrthoArgs& a, con
             const double r = a.mat[i].rows, l = a.mat[i].cols;
             a.mat[i].lr = (float)(lr * (adjust == NERFX_LR_MATCH_RMS ? 0.2 * std::sqrt(std::max(r, l)) : std::sqrt(std::max(1.0, r / l))));
         }
-        if (int rc = tile == 128 ? ortho_run<128, 8, 4>(a, coef, steps, s, stream) : ortho_run<64, 4, 8>(a, coef, steps, s, stream)) return rc;
+        if (int rc = ortho_run(a, tile, coef, steps, s, stream)) return rc;
     }
     return 0;
 }
