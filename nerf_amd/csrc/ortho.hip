@@ -4,8 +4,11 @@
 // per step   A = X X^T,   B = b A + c A A,   X <- a X + B X
 // which takes every singular value s to a s + b s^3 + c s^5 and leaves the singular vectors.  The result goes
 // back in G's own orientation.  A whole group of matrices of any shapes shares every launch: a launch's grid
-// is the concatenation of the matrices' tiles, and a workgroup finds its matrix by walking the (short) table
-// in the kernel's arguments, so nothing is copied to the device and the call can be captured.
+// is the concatenation of the matrices' tiles, and a workgroup finds its matrix in a table.  The first launch has the
+// table in its arguments and leaves it in the workspace, so nothing is copied to the device and the call can be captured;
+// the others read it there.
+//
+// Groups of small matrices (sides up to 64 and 256) take one launch altogether: see ortho_small_kernel.
 #include <algorithm>
 #include <cmath>
 
@@ -31,19 +34,22 @@ struct OrthoMat {
     float lr;                                   // optimiser step: learning rate with its shape factor
     int32_t tall;                               // rows > cols: X is the transpose
 };
-struct OrthoArgs {
-    OrthoMat mat[ORTHO_GROUP];
-    int32_t first[ORTHO_GROUP];                 // first block of each matrix in this launch; INT_MAX behind the last
-    char* work;
+struct OrthoCall {
     const float* grad_scale;
     const float* found_inf;
     float momentum, rest, decay;                // rest: 1 - momentum, decay: 1 - lr * weight_decay
+    float eps, x_scale;
     int32_t growth;                             // the steps together grow a singular value by at most 2^growth
-    float eps, alpha, beta, x_scale;            // alpha, beta: factors of the epilogue's element and accumulator
     int32_t count, nesterov, dtype, muon;
-    int32_t from, to;                           // which of the two X^T copies is read and written
 };
-static_assert(sizeof(OrthoArgs) <= 4096, "the group's table has to fit the kernel arguments");
+enum { ORTHO_NORM_GRID, ORTHO_PREP_GRID, ORTHO_SYM_GRID, ORTHO_FULL_GRID, ORTHO_GRIDS };
+struct OrthoTable {
+    OrthoMat mat[ORTHO_GROUP];
+    int32_t first[ORTHO_GRIDS][ORTHO_GROUP];    // first block of each matrix in a launch; INT_MAX behind the last
+    OrthoCall call;
+};
+static_assert(sizeof(OrthoTable) <= 3584, "the table has to fit the kernel arguments");
+constexpr int64_t ORTHO_TABLE_BYTES = 3584;     // at the start of the workspace
 
 // Parts of a matrix's workspace: X (m x n), two copies of X^T (n x m), A and B (m x m), partial sums.
 __host__ __device__ inline int64_t ortho_x_bytes(const OrthoMat& q) { return (int64_t)q.m * q.n * 4; }
@@ -72,21 +78,21 @@ __device__ __forceinline__ void store_from_float(void* p, int64_t i, float v, in
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 // What is orthogonalised, at flat index i: the gradient, or the optimiser's mix of it and the (new) momentum.
-__device__ __forceinline__ float update_at(const OrthoArgs& a, const OrthoMat& q, int64_t i, float unscale) {
+__device__ __forceinline__ float update_at(const OrthoCall& a, const OrthoMat& q, int64_t i, float unscale) {
     const float g = load_as_float(q.grad, i, a.dtype);
     if (!a.muon) return g;
     const float mom = q.momentum[i];
     return a.nesterov ? fmaf(a.momentum, mom, a.rest * (g * unscale)) : mom;
 }
 
-// The matrix that this block works on, and the block's number within it.  (All of the table is read at once:
-// walking it would wait for each entry in turn.)
-__device__ __forceinline__ int which_matrix(const OrthoArgs& a, int& block) {
+// The matrix that this block works on, and the block's number within it.  (All of a row of the table is read at
+// once: walking it would wait for each entry in turn.)
+__device__ __forceinline__ int which_matrix(const OrthoTable& t, int grid, int& block) {
     const int b = blockIdx.x;
     int k = 0, start = 0;
 #pragma unroll
     for (int i = 1; i < ORTHO_GROUP; ++i) {
-        const int f = a.first[i];
+        const int f = t.first[grid][i];
         if (b >= f) { k = i; start = f; }
     }
     block = b - start;
@@ -96,9 +102,12 @@ enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
 
 // Momentum, and partial sums of squares of what is orthogonalised.  In double: a fp32 gradient's square
 // neither overflows nor vanishes there, and a sum of 2^30 of them keeps fp32's precision.
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoArgs a) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable t, char* work) {
     int b;
-    const OrthoMat q = a.mat[which_matrix(a, b)];
+    const OrthoMat q = t.mat[which_matrix(t, ORTHO_NORM_GRID, b)];
+    const OrthoCall& a = t.call;
+    if (blockIdx.x == 0)                                       // for the launches behind this one
+        for (int i = threadIdx.x; i < (int)(sizeof(OrthoTable) / 4); i += 256) ((uint32_t*)work)[i] = ((const uint32_t*)&t)[i];
     const int64_t total = (int64_t)q.rows * q.cols;
     const int parts = norm_parts(q);
     const bool skip = a.found_inf && *a.found_inf != 0.f;
@@ -115,15 +124,16 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoArgs a) {
     for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
     __syncthreads();
-    if (threadIdx.x == 0) ((double*)(a.work + ortho_sums_at(q)))[b] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (threadIdx.x == 0) ((double*)(work + ortho_sums_at(q)))[b] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // X and X^T from what is orthogonalised: one 64 x 64 tile of X per block, through LDS, zeros in the padding.
-__global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
+__global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __restrict__ t, char* __restrict__ work) {
     int b;
-    const OrthoMat q = a.mat[which_matrix(a, b)];
+    const OrthoMat q = t->mat[which_matrix(*t, ORTHO_PREP_GRID, b)];
+    const OrthoCall a = t->call;
     __shared__ float tile[PREP_TILE][PREP_TILE + 1];
-    const double* sums = (const double*)(a.work + ortho_sums_at(q));
+    const double* sums = (const double*)(work + ortho_sums_at(q));
     __shared__ double part[4];
     double total = 0;
     for (int k = threadIdx.x; k < norm_parts(q); k += 256) total += sums[k];
@@ -138,7 +148,7 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
     int lift = 0;
     if (norm < (double)a.eps) lift = max(0, min(120, norm > 0 ? ilogb((double)a.eps / norm) - a.growth : 0));
     factor = ldexp(factor, lift);
-    if (b == 0 && threadIdx.x == 0) *(int*)(a.work + ortho_lift_at(q)) = lift;
+    if (b == 0 && threadIdx.x == 0) *(int*)(work + ortho_lift_at(q)) = lift;
     const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
     const int x0 = b / (q.n / PREP_TILE) * PREP_TILE, y0 = b % (q.n / PREP_TILE) * PREP_TILE;   // of X
     // G's rows run along X's columns, or, if G is tall, along X's rows
@@ -150,8 +160,8 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoArgs a) {
         if (q.tall) tile[c][r] = v; else tile[r][c] = v;
     }
     __syncthreads();
-    char* x = a.work + q.base;
-    char* xt = a.work + ortho_xt_at(q, 0);
+    char* x = work + q.base;
+    char* xt = work + ortho_xt_at(q, 0);
     for (int e = threadIdx.x; e < PREP_TILE * PREP_TILE / 4; e += 256) {
         const int r = e / (PREP_TILE / 4), k = (e % (PREP_TILE / 4)) * 4;
         const float row[4] = {tile[r][k], tile[r][k + 1], tile[r][k + 2], tile[r][k + 3]};
@@ -268,11 +278,12 @@ __device__ __forceinline__ void triangle_at(int64_t t, int& i, int& j) {
 }
 
 template <int T, int WAVES, int STAGES, int KIND>
-__global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTable* __restrict__ t, char* __restrict__ work, float alpha,
+                                                                float beta, int from) {
     extern __shared__ __align__(16) char lds[];
     constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;       // the result is symmetric: half of the tiles
     int b;
-    const OrthoMat q = a.mat[which_matrix(a, b)];
+    const OrthoMat q = t->mat[which_matrix(*t, SYM ? ORTHO_SYM_GRID : ORTHO_FULL_GRID, b)];
     int ti, tj;
     if constexpr (SYM) {
         triangle_at(b, ti, tj);
@@ -280,11 +291,11 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoAr
         ti = b % (q.m / T);
         tj = b / (q.m / T);
     }
-    char* X = a.work + q.base;
-    char* A = a.work + ortho_a_at(q);
-    char* B = a.work + ortho_b_at(q);
+    char* X = work + q.base;
+    char* A = work + ortho_a_at(q);
+    char* B = work + ortho_b_at(q);
     const char* P = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : B;
-    const char* Q = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : a.work + ortho_xt_at(q, a.from);
+    const char* Q = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : work + ortho_xt_at(q, from);
     const int K = KIND == ORTHO_GRAM ? q.n : q.m;
     using Tile = SplitTile<T, WAVES, STAGES>;
     Tile tile;
@@ -303,12 +314,12 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoAr
                                                ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e, q.m);
     }
     tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K);
-    float alpha = a.alpha, beta = a.beta;
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {            // see the kernel that made X
-        const int lift = *(const int*)(a.work + ortho_lift_at(q));
+        const int lift = *(const int*)(work + ortho_lift_at(q));
         beta = ldexpf(beta, KIND == ORTHO_GRAM ? -2 * lift : -lift);
         alpha = ldexpf(alpha, -lift);
     }
+    const OrthoCall a = t->call;
     const bool skip = KIND == ORTHO_LAST && a.found_inf && *a.found_inf != 0.f;
 #pragma unroll
     for (int i = 0; i < Tile::FP; ++i)
@@ -340,7 +351,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoAr
                         *(_Float16*)(p + 64) = lo;
                     }
                 } else if constexpr (KIND == ORTHO_APPLY) {
-                    split_store4(a.work + ortho_xt_at(q, a.to), col, row, q.m, v);
+                    split_store4(work + ortho_xt_at(q, from ^ 1), col, row, q.m, v);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         _Float16 hi, lo;
@@ -363,6 +374,187 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoAr
         }
 }
 
+// ---- small matrices: one launch ---------------------------------------------------------------------------------------
+// A matrix whose smaller side is at most 64 and whose larger one is at most 256 fits in LDS with everything that the steps
+// need (X, X^T, A and B: 160 KB), so that a workgroup takes all of its steps by itself.  What bounds the other way there is
+// the number of launches: 17 of 5 us each.  Only for groups of nothing but such matrices; in a group with a larger one they
+// ride along in its launches.
+//
+// A row takes 128 bytes for every 32 of its columns, as in memory; 16-byte chunk c (of a pair of blocks: 0 .. 15) of row r lies at
+// place c ^ (r % 16), so that the sixteen rows of a read phase touch different banks.  Every matrix and row begins at a multiple
+// of 256 bytes, so that an address is a per-lane one with a constant's bits flipped.
+constexpr int SMALL_M = 64, SMALL_N = 256, SMALL_WAVES = 8;
+
+__device__ __forceinline__ int small_at(int r, int k, int pitch) {             // of the hi half; the lo half: ^ 64
+    return r * pitch + (k >> 6) * 256 + ((((k >> 5 & 1) * 8 + (k >> 3 & 3)) ^ (r & 15)) * 16) + (k & 7) * 2;
+}
+__device__ __forceinline__ void small_put(char* m, int at, float v) {
+    _Float16 hi, lo;
+    split16(v, hi, lo);
+    *(_Float16*)(m + at) = hi;
+    *(_Float16*)(m + (at ^ 64)) = lo;
+}
+// 32 x 32 of P Q^T from rows p0 .. of P and q0 .. of Q; K a multiple of 64.
+__device__ __forceinline__ float16_t_ small_product(const char* P, int p0, int p_pitch, const char* Q, int q0, int q_pitch, int K) {
+    const int lane = threadIdx.x & 63, p = p0 + (lane & 31), q = q0 + (lane & 31), h = lane >> 5;
+    const int pv = p * p_pitch + ((h ^ (p & 15)) * 16), qv = q * q_pitch + ((h ^ (q & 15)) * 16);
+    float16_t_ main, cross;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) main[e] = cross[e] = 0.f;
+    for (int kb = 0; kb < K / 64; ++kb) {
+        half8_t ph[4], pl[4], qh[4], ql[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int c = (s >> 1) * 128 + (s & 1) * 32;
+            ph[s] = *(const half8_t*)(P + kb * 256 + (pv ^ c)); pl[s] = *(const half8_t*)(P + kb * 256 + (pv ^ (c + 64)));
+            qh[s] = *(const half8_t*)(Q + kb * 256 + (qv ^ c)); ql[s] = *(const half8_t*)(Q + kb * 256 + (qv ^ (c + 64)));
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {                                          // two chains: neither waits for the other
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[s], ql[s], cross, 0, 0, 0);
+            main = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[s], qh[s], main, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[s], qh[s], cross, 0, 0, 0);
+        }
+    }
+    return main + cross;
+}
+
+struct OrthoSteps { float coef[3 * ORTHO_MAX_STEPS]; int32_t steps; float sx, sa, sb; };
+
+__global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoTable t, const OrthoSteps c) {
+    extern __shared__ __align__(256) char lds[];
+    const OrthoMat q = t.mat[blockIdx.x];
+    const OrthoCall& a = t.call;
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int total = q.rows * q.cols, threads = 64 * SMALL_WAVES, xp = q.n * 4, side = min(q.rows, q.cols);
+    char *A = lds, *B = lds + SMALL_M * 256, *XT = lds + 2 * SMALL_M * 256, *X = XT + q.n * 256;
+    const bool skip = a.found_inf && *a.found_inf != 0.f;
+    const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
+    // zeros: what lies behind the matrix's sides stays as it is
+    for (int i = tid; i < (2 * SMALL_M * 256 + q.n * 512) / 16; i += threads) *(u32x4_t*)(lds + 16 * i) = (u32x4_t){0, 0, 0, 0};
+    // momentum and norm, as in the kernels above
+    double acc = 0;
+    for (int i = tid; i < total; i += threads) {
+        if (a.muon && !skip)
+            q.momentum[i] = fmaf(a.momentum, q.momentum[i], a.rest * (((const float*)q.grad)[i] * unscale));
+        const double u = update_at(a, q, i, unscale);
+        acc = fma(u, u, acc);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+    __syncthreads();
+    double* part = (double*)B;
+    if (lane == 0) part[wave] = acc;
+    __syncthreads();
+    double sum = 0;
+#pragma unroll
+    for (int w = 0; w < SMALL_WAVES; ++w) sum += part[w];
+    const double norm = sqrt(sum);
+    double factor = (double)a.x_scale / (norm < (double)a.eps ? (double)a.eps : norm);
+    int lift = 0;
+    if (norm < (double)a.eps) lift = max(0, min(120, norm > 0 ? ilogb((double)a.eps / norm) - a.growth : 0));
+    factor = ldexp(factor, lift);
+    __syncthreads();
+    if (tid < SMALL_WAVES) part[tid] = 0;
+    for (int i = tid; i < total; i += threads) {
+        const int r = i / q.cols, k = i - r * q.cols;
+        const float v = (float)(update_at(a, q, i, unscale) * factor);
+        small_put(X, small_at(q.tall ? k : r, q.tall ? r : k, xp), v);
+        small_put(XT, small_at(q.tall ? r : k, q.tall ? k : r, 256), v);
+    }
+    __syncthreads();
+    // a wave's 32 x 32 part of A and B: four waves have one, those behind the matrix's side none
+    const int row0 = 32 * (wave >> 1 & 1), col0 = 32 * (wave & 1);
+    const bool square = wave < 4 && row0 < side && col0 < side;
+    const float gram = ldexpf(c.sa / (c.sx * c.sx), -2 * lift);
+    // elements row .. row + 3 of column `col`, as a run of a symmetric matrix's row or of X^T's: 8 (e / 4) + 4 h rows on
+    auto run_at = [&](int col, int row) { return ((col * 256 + (col & 15) * 16) ^ (row / 32 * 128)) + 8 * h; };
+    auto put4 = [&](char* at, int e, const float (&v)[4]) {
+        half4_t hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { _Float16 f, l; split16(v[i], f, l); hi[i] = f; lo[i] = l; }
+        *(half4_t*)(lds + ((int)(at - lds) ^ (e / 4 * 16))) = hi;
+        *(half4_t*)(lds + ((int)(at - lds) ^ (e / 4 * 16 + 64))) = lo;
+        return Split4{hi, lo};
+    };
+    auto get4 = [&](const char* at, int e) {
+        return Split4{*(const half4_t*)(lds + ((int)(at - lds) ^ (e / 4 * 16))), *(const half4_t*)(lds + ((int)(at - lds) ^ (e / 4 * 16 + 64)))};
+    };
+    const int tiles = q.n / 32 * 2;                                            // of X: 64 rows
+    for (int step = 0; step < c.steps; ++step) {
+        const float ca = c.coef[3 * step], cb = c.coef[3 * step + 1], cc = c.coef[3 * step + 2];
+        const bool last = step == c.steps - 1;
+        const int run = run_at(col0 + (lane & 31), row0);
+        if (square) {
+            const float16_t_ v = small_product(X, row0, xp, X, col0, xp, q.n);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) put4(A + run, e, {gram * v[e], gram * v[e + 1], gram * v[e + 2], gram * v[e + 3]});
+        }
+        __syncthreads();
+        if (square) {
+            const float16_t_ v = small_product(A, row0, 256, A, col0, 256, SMALL_M);
+            const float pa = cb * (c.sb / c.sa), pb = cc * (c.sb / c.sa / c.sa);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const Split4 own = get4(A + run, e);
+                float w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = fmaf(pb, v[e + k], pa * ((float)own.hi[k] + (float)own.lo[k]));
+                put4(B + run, e, w);
+            }
+        }
+        __syncthreads();
+        constexpr int MOST = SMALL_N / 32 * 2 / SMALL_WAVES;
+        float16_t_ x[MOST];
+        const float xa = last ? ldexpf(ca / c.sx, -lift) : ca, xb = last ? ldexpf(1.0f / (c.sb * c.sx), -lift) : 1.0f / c.sb;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            const int tile = wave + SMALL_WAVES * i, r0 = 32 * (tile & 1), n0 = 32 * (tile >> 1);
+            if (tile >= tiles || r0 >= side) continue;
+            x[i] = small_product(B, r0, 256, XT, n0, 256, SMALL_M);
+            const char* at = XT + run_at(n0 + (lane & 31), r0);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const Split4 own = get4(at, e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][e + k] = fmaf(xb, x[i][e + k], xa * ((float)own.hi[k] + (float)own.lo[k]));
+            }
+        }
+        __syncthreads();                                                       // X^T has been read
+        float* out = (float*)X;                                                // X as well: the last step's result goes there
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) {
+            const int tile = wave + SMALL_WAVES * i, r0 = 32 * (tile & 1), n0 = 32 * (tile >> 1), k = n0 + (lane & 31);
+            if (tile >= tiles || r0 >= side) continue;
+            if (last) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) out[(r0 + 4 * h + 8 * (e / 4) + e % 4) * q.n + k] = x[i][e];
+                continue;
+            }
+            char* at = XT + run_at(k, r0);
+            const int xv = (r0 + 4 * h) * xp + (k >> 6) * 256 + ((((k >> 5 & 1) * 8 + (k >> 3 & 3)) ^ 4 * h) * 16) + (k & 7) * 2;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const Split4 v = put4(at, e, {x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3]});
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {                                  // row r0 + 4 h + 2 e + j of X
+                    char* to = X + (2 * e + j) * xp;
+                    *(_Float16*)(to + (xv ^ ((2 * e & 8) + j) * 16)) = v.hi[j];
+                    *(_Float16*)(to + (xv ^ (((2 * e & 8) + j) * 16 + 64))) = v.lo[j];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (skip) return;
+    for (int i = tid; i < total; i += threads) {
+        const int r = i / q.cols, k = i - r * q.cols;
+        const float v = ((const float*)X)[q.tall ? k * q.n + r : r * q.n + k];
+        if (a.muon) q.param[i] = fmaf(-q.lr, v, q.param[i] * a.decay);
+        else store_from_float(q.out, i, v, a.dtype);
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------------------------------
 // Sides are padded to whole tiles: of 128 where there is enough work for them somewhere, else of 64.
 static int tile_side(const nerfx_matrix_t* mats, int count) {
@@ -374,12 +566,12 @@ static int tile_side(const nerfx_matrix_t* mats, int count) {
     return big >= 192 ? 128 : 64;
 }
 
-static int64_t fill_group(const nerfx_matrix_t* mats, int count, int tile, OrthoArgs& a) {
-    int64_t at = 0;
-    a.count = 0;
+static int64_t fill_group(const nerfx_matrix_t* mats, int count, int tile, OrthoTable& a) {
+    int64_t at = ORTHO_TABLE_BYTES;
+    a.call.count = 0;
     for (int k = 0; k < count; ++k) {
         if (mats[k].rows == 0 || mats[k].cols == 0) continue;
-        OrthoMat& q = a.mat[a.count++];
+        OrthoMat& q = a.mat[a.call.count++];
         q = OrthoMat{};
         q.grad = mats[k].grad; q.momentum = mats[k].momentum; q.param = mats[k].param; q.out = mats[k].out;
         q.rows = mats[k].rows; q.cols = mats[k].cols;
@@ -430,29 +622,13 @@ static int scales_for(const float* coef, int steps, OrthoScales& s) {
 
 // A launch's grid is the matrices' blocks one after the other.
 template <class F>
-static int64_t lay_out(OrthoArgs& a, F blocks_of) {
+static int64_t lay_out(OrthoTable& t, int grid, F blocks_of) {
     int64_t at = 0;
     for (int k = 0; k < ORTHO_GROUP; ++k) {
-        a.first[k] = k < a.count ? (int32_t)at : INT32_MAX;
-        if (k < a.count) at += blocks_of(a.mat[k]);
+        t.first[grid][k] = k < t.call.count ? (int32_t)at : INT32_MAX;
+        if (k < t.call.count) at += blocks_of(t.mat[k]);
     }
     return at;
-}
-
-template <int KIND>
-static int64_t product_blocks(OrthoArgs& a, int tile) {
-    return lay_out(a, [tile](const OrthoMat& q) {
-        const int64_t mt = q.m / tile;
-        return KIND == ORTHO_GRAM || KIND == ORTHO_POLY ? mt * (mt + 1) / 2 : mt * (q.n / tile);
-    });
-}
-
-template <int T, int WAVES, int STAGES, int KIND>
-static int product_as(const OrthoArgs& a, int64_t blocks, hipStream_t stream) {
-    constexpr size_t lds = SplitTile<T, WAVES, STAGES>::LDS_BYTES;
-    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, KIND>), lds);
-    hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, KIND>), dim3((unsigned)blocks), dim3(64 * WAVES), lds, stream, a);
-    return 0;
 }
 
 // The tile a product takes, by how many of them there are:
@@ -461,69 +637,112 @@ static int product_as(const OrthoArgs& a, int64_t blocks, hipStream_t stream) {
 //  64   with two stages, five workgroups to a CU, where they would not: of a symmetric result 136 tiles of 128 take as long as
 //       all 256 (50 us), 528 of 64 take 41; three and four stages hold fewer workgroups and take 44 and 50;
 //  64   with eight stages where there is at most one to a CU: all of a K of 256 is on its way at once.
-template <int KIND>
-static int product(OrthoArgs& a, int pad, hipStream_t stream) {
+enum { ORTHO_TILE_128, ORTHO_TILE_64, ORTHO_TILE_64_DEEP };
+struct OrthoShape { int kind; int64_t blocks; };
+static OrthoShape choose(OrthoTable& t, int grid, int pad) {
+    auto blocks = [&](int tile) {
+        return lay_out(t, grid, [=](const OrthoMat& q) {
+            const int64_t mt = q.m / tile;
+            return grid == ORTHO_SYM_GRID ? mt * (mt + 1) / 2 : mt * (q.n / tile);
+        });
+    };
     if (pad == 128) {
-        const int64_t blocks = product_blocks<KIND>(a, 128), rounds = (blocks + 255) / 256;
-        if (blocks * 5 >= rounds * 256 * 4) return product_as<128, 8, 4, KIND>(a, blocks, stream);
+        const int64_t big = blocks(128);
+        if (big * 5 >= (big + 255) / 256 * 256 * 4) return {ORTHO_TILE_128, big};
     }
-    const int64_t blocks = product_blocks<KIND>(a, 64);
-    return blocks <= 256 ? product_as<64, 4, 8, KIND>(a, blocks, stream) : product_as<64, 4, 2, KIND>(a, blocks, stream);
+    const int64_t small = blocks(64);
+    return {small <= 256 ? ORTHO_TILE_64_DEEP : ORTHO_TILE_64, small};
 }
 
-static int ortho_run(OrthoArgs& a, int pad, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
-    a.x_scale = s.x;
-    a.growth = s.growth;
-    int64_t blocks = lay_out(a, [](const OrthoMat& q) { return (int64_t)norm_parts(q); });
-    hipLaunchKernelGGL(ortho_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
-    blocks = lay_out(a, [](const OrthoMat& q) { return (int64_t)(q.m / PREP_TILE) * (q.n / PREP_TILE); });
-    hipLaunchKernelGGL(ortho_prep_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+template <int T, int WAVES, int STAGES, int KIND>
+static int product_as(int64_t blocks, char* work, float alpha, float beta, int from, hipStream_t stream) {
+    constexpr size_t lds = SplitTile<T, WAVES, STAGES>::LDS_BYTES;
+    NERFX_OPT_IN_LDS((ortho_product_kernel<T, WAVES, STAGES, KIND>), lds);
+    hipLaunchKernelGGL((ortho_product_kernel<T, WAVES, STAGES, KIND>), dim3((unsigned)blocks), dim3(64 * WAVES), lds, stream,
+                       (const OrthoTable*)work, work, alpha, beta, from);
+    return 0;
+}
+template <int KIND>
+static int product(const OrthoShape& s, char* work, float alpha, float beta, int from, hipStream_t stream) {
+    if (s.kind == ORTHO_TILE_128) return product_as<128, 8, 4, KIND>(s.blocks, work, alpha, beta, from, stream);
+    if (s.kind == ORTHO_TILE_64) return product_as<64, 4, 2, KIND>(s.blocks, work, alpha, beta, from, stream);
+    return product_as<64, 4, 8, KIND>(s.blocks, work, alpha, beta, from, stream);
+}
+
+static bool all_small(const OrthoTable& t) {
+    for (int k = 0; k < t.call.count; ++k)
+        if (t.mat[k].m > SMALL_M || t.mat[k].n > SMALL_N) return false;
+    return true;
+}
+
+static int small_run(OrthoTable& t, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
+    t.call.x_scale = s.x;
+    t.call.growth = s.growth;
+    OrthoSteps c{};
+    std::copy(coef, coef + 3 * steps, c.coef);
+    c.steps = steps; c.sx = s.x; c.sa = s.a; c.sb = s.b;
+    int n = 0;
+    for (int k = 0; k < t.call.count; ++k) n = std::max(n, t.mat[k].n);
+    const size_t lds = 2 * SMALL_M * 256 + (size_t)n * 512;
+    NERFX_OPT_IN_LDS(ortho_small_kernel, lds);
+    hipLaunchKernelGGL(ortho_small_kernel, dim3((unsigned)t.call.count), dim3(64 * SMALL_WAVES), lds, stream, t, c);
+    return launch_status("ortho_small_kernel");
+}
+
+static int ortho_run(OrthoTable& t, char* work, int pad, const float* coef, int steps, const OrthoScales& s, hipStream_t stream) {
+    t.call.x_scale = s.x;
+    t.call.growth = s.growth;
+    const int64_t norm = lay_out(t, ORTHO_NORM_GRID, [](const OrthoMat& q) { return (int64_t)norm_parts(q); });
+    const int64_t prep = lay_out(t, ORTHO_PREP_GRID, [](const OrthoMat& q) { return (int64_t)(q.m / PREP_TILE) * (q.n / PREP_TILE); });
+    const OrthoShape sym = choose(t, ORTHO_SYM_GRID, pad), full = choose(t, ORTHO_FULL_GRID, pad);
+    hipLaunchKernelGGL(ortho_norm_kernel, dim3((unsigned)norm), dim3(256), 0, stream, t, work);
+    hipLaunchKernelGGL(ortho_prep_kernel, dim3((unsigned)prep), dim3(256), 0, stream, (const OrthoTable*)work, work);
     for (int k = 0; k < steps; ++k) {
         const float ca = coef[3 * k], cb = coef[3 * k + 1], cc = coef[3 * k + 2];
-        a.beta = s.a / (s.x * s.x);
-        if (int rc = product<ORTHO_GRAM>(a, pad, stream)) return rc;
-        a.alpha = cb * (s.b / s.a);
-        a.beta = cc * (s.b / s.a / s.a);
-        if (int rc = product<ORTHO_POLY>(a, pad, stream)) return rc;
-        a.from = k & 1; a.to = a.from ^ 1;
-        const bool last = k == steps - 1;
-        a.alpha = last ? ca / s.x : ca;                       // the last step leaves the scale
-        a.beta = last ? 1.0f / (s.b * s.x) : 1.0f / s.b;
-        if (int rc = last ? product<ORTHO_LAST>(a, pad, stream) : product<ORTHO_APPLY>(a, pad, stream)) return rc;
+        if (int rc = product<ORTHO_GRAM>(sym, work, 0.f, s.a / (s.x * s.x), 0, stream)) return rc;
+        if (int rc = product<ORTHO_POLY>(sym, work, cb * (s.b / s.a), cc * (s.b / s.a / s.a), 0, stream)) return rc;
+        // the last step leaves the scales
+        if (int rc = k == steps - 1 ? product<ORTHO_LAST>(full, work, ca / s.x, 1.0f / (s.b * s.x), k & 1, stream)
+                                    : product<ORTHO_APPLY>(full, work, ca, 1.0f / s.b, k & 1, stream)) return rc;
     }
     return launch_status("orthogonalisation kernels");
 }
 
+static_assert(sizeof(OrthoTable) + sizeof(OrthoSteps) <= 4096, "kernel arguments");
 // Groups of at most ORTHO_GROUP matrices, one after the other in the same workspace (same stream: in order).
 static int64_t group_bytes(const nerfx_matrix_t* mats, int count) {
     int64_t most = 0;
-    OrthoArgs a;
+    OrthoTable a;
     for (int k = 0; k < count; k += ORTHO_GROUP) {
         const int c = std::min(ORTHO_GROUP, count - k);
-        most = std::max(most, fill_group(mats + k, c, tile_side(mats + k, c), a));
+        const int64_t bytes = fill_group(mats + k, c, tile_side(mats + k, c), a);
+        if (a.call.count && !all_small(a)) most = std::max(most, bytes);
     }
     return most;
 }
 
-static int ortho_groups(const nerfx_matrix_t* mats, int count, OrthoArgs& a, const float* coef, int steps, void* workspace,
+static int ortho_groups(const nerfx_matrix_t* mats, int count, OrthoTable& a, const float* coef, int steps, void* workspace,
                         int64_t workspace_bytes, double lr, int adjust, hipStream_t stream) {
     NERFX_REQUIRE(steps >= 1 && steps <= ORTHO_MAX_STEPS && coef, "steps %d outside 1..%d, or no coefficients", steps, ORTHO_MAX_STEPS);
-    NERFX_REQUIRE(a.eps > 0.f && std::isfinite(a.eps), "eps must be positive and finite");
+    NERFX_REQUIRE(a.call.eps > 0.f && std::isfinite(a.call.eps), "eps must be positive and finite");
     OrthoScales s;
     if (int rc = scales_for(coef, steps, s)) return rc;
     const int64_t need = group_bytes(mats, count);
     NERFX_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "workspace is NULL or not aligned to 16 bytes");
     NERFX_REQUIRE(workspace_bytes >= need, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-    a.work = (char*)workspace;
     for (int k = 0; k < count; k += ORTHO_GROUP) {
         const int c = std::min(ORTHO_GROUP, count - k), tile = tile_side(mats + k, c);
         fill_group(mats + k, c, tile, a);
-        if (a.count == 0) continue;
-        for (int i = 0; i < a.count; ++i) {
+        if (a.call.count == 0) continue;
+        for (int i = 0; i < a.call.count; ++i) {
             const double r = a.mat[i].rows, l = a.mat[i].cols;
             a.mat[i].lr = (float)(lr * (adjust == NERFX_LR_MATCH_RMS ? 0.2 * std::sqrt(std::max(r, l)) : std::sqrt(std::max(1.0, r / l))));
         }
-        if (int rc = ortho_run(a, tile, coef, steps, s, stream)) return rc;
+        if (all_small(a)) {
+            if (int rc = small_run(a, coef, steps, s, stream)) return rc;
+            continue;
+        }
+        if (int rc = ortho_run(a, (char*)workspace, tile, coef, steps, s, stream)) return rc;
     }
     return 0;
 }
@@ -543,8 +762,8 @@ extern "C" int nerfx_orthogonalize(const nerfx_matrix_t* mats, int count, int dt
     NERFX_REQUIRE(dtype == NERFX_TYPE_F32 || dtype == NERFX_TYPE_BF16 || dtype == NERFX_TYPE_F16, "unknown type %d", dtype);
     for (int k = 0; k < count; ++k)
         NERFX_REQUIRE(mats[k].rows == 0 || mats[k].cols == 0 || (mats[k].grad && mats[k].out), "matrix %d: grad / out is NULL", k);
-    OrthoArgs a{};
-    a.dtype = dtype; a.eps = eps;
+    OrthoTable a{};
+    a.call.dtype = dtype; a.call.eps = eps;
     return ortho_groups(mats, count, a, coefficients, steps, workspace, workspace_bytes, 0, 0, (hipStream_t)stream);
 }
 
@@ -558,9 +777,10 @@ extern "C" int nerfx_muon_step(const nerfx_matrix_t* mats, int count, double lr,
     for (int k = 0; k < count; ++k)
         NERFX_REQUIRE(mats[k].rows == 0 || mats[k].cols == 0 || (mats[k].grad && mats[k].momentum && mats[k].param),
                       "matrix %d: grad / momentum / param is NULL", k);
-    OrthoArgs a{};
-    a.muon = 1; a.nesterov = nesterov != 0; a.momentum = (float)momentum; a.rest = (float)(1 - momentum);
-    a.decay = (float)(1 - lr * weight_decay); a.eps = eps;
-    a.grad_scale = grad_scale; a.found_inf = found_inf;
+    OrthoTable a{};
+    OrthoCall& c = a.call;
+    c.muon = 1; c.nesterov = nesterov != 0; c.momentum = (float)momentum; c.rest = (float)(1 - momentum);
+    c.decay = (float)(1 - lr * weight_decay); c.eps = eps;
+    c.grad_scale = grad_scale; c.found_inf = found_inf;
     return ortho_groups(mats, count, a, coefficients, steps, workspace, workspace_bytes, lr, adjust_lr, (hipStream_t)stream);
 }

@@ -1,7 +1,10 @@
 """Tensor-level wrappers over the C ABI: validate, allocate outputs with torch,
 pass raw device pointers and the current HIP stream.  No arithmetic happens here.
 """
+import contextlib
 import ctypes as C
+import functools
+import struct
 import weakref
 from typing import Optional, Tuple
 
@@ -728,23 +731,50 @@ _LR_RULES = {"original": _lib.LR_ORIGINAL, "match_rms_adamw": _lib.LR_MATCH_RMS}
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+_AS_IT_IS = contextlib.nullcontext()
+
+
+def _on(dev):
+    """torch.cuda.device(dev), or nothing where that is the current one."""
+    return _AS_IT_IS if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object around it
+
+
+def _stream_on(dev):
+    """_stream() of `dev`, for calls whose own time is that of a few Python objects."""
+    return _stream() if _RAW_STREAM is None else _RAW_STREAM(dev.index)
+
+
 def _ns_schedule(coefficients, steps: int):
     """One (a, b, c) for all steps, or one for each -> the C array of 3 * steps floats."""
     if not 1 <= steps <= 32:
         raise ValueError(f"steps must be 1..32 (got {steps})")
-    rows = list(coefficients)
-    if len(rows) == 3 and not any(hasattr(r, "__len__") for r in rows):
-        rows = [tuple(rows)] * steps
-    if len(rows) != steps or any(len(r) != 3 for r in rows):
+    rows = tuple(tuple(r) if hasattr(r, "__len__") else r for r in coefficients)
+    if len(rows) == 3 and not any(isinstance(r, tuple) for r in rows):
+        rows = (rows,) * steps
+    if len(rows) != steps or any(not isinstance(r, tuple) or len(r) != 3 for r in rows):
         raise ValueError("coefficients: one (a, b, c), or one for each of the steps")
-    return (C.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+    return _ns_array(rows)
 
 
-def _ns_workspace(table, count: int, dev) -> Tuple[Tensor, int]:
+@functools.lru_cache(maxsize=64)
+def _ns_array(rows):
+    return (C.c_float * (3 * len(rows)))(*[float(v) for r in rows for v in r])
+
+
+def _matrix_table(rows):
+    """rows of (grad, out, param, momentum, rows, cols) -> the C array of nerfx_matrix_t."""
+    n = len(rows)
+    return (_lib.Matrix * n).from_buffer_copy(struct.pack("QQQQii" * n, *[v for r in rows for v in r]))
+
+
+def _ns_workspace(table, count: int, dev):
     need = lib.nerfx_orthogonalize_workspace_bytes(table, count)
     if need < 0:
         raise _lib.NerfxError(f"nerfx error: {lib.nerfx_last_error().decode()}")
-    return torch.empty((max(need, 1),), device=dev, dtype=torch.uint8), need
+    return (torch.empty((need,), device=dev, dtype=torch.uint8) if need else None), need
 
 
 def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7):
@@ -757,30 +787,30 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
     last rounding.  Not differentiable."""
     listed = list(mats) if isinstance(mats, (list, tuple)) else list(mats.unbind(0)) if mats.dim() == 3 else [mats]
     schedule = _ns_schedule(coefficients, steps)
+    if not listed:
+        return torch.empty_like(mats) if isinstance(mats, Tensor) else []
+    if not all(isinstance(t, Tensor) for t in listed):
+        raise TypeError("mats must be tensors")
+    dtype, dev, grad = listed[0].dtype, listed[0].device, torch.is_grad_enabled()
     for t in listed:
-        if not isinstance(t, Tensor):
-            raise TypeError("mats must be tensors")
         if not t.is_cuda:
             raise RuntimeError(f"nerf_amd runs on ROCm devices only: `mats` is on {t.device}")
         if t.dtype not in _TYPES:
             raise TypeError(f"orthogonalize takes fp32, bf16 or fp16 matrices (got {t.dtype})")
         if t.dim() != 2:
             raise ValueError(f"orthogonalize takes matrices (got a tensor of shape {tuple(t.shape)})")
-        if t.dtype != listed[0].dtype or t.device != listed[0].device:
+        if t.dtype != dtype or t.device != dev:
             raise ValueError("orthogonalize: all matrices of a call have one type and one device")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise RuntimeError("orthogonalize is not differentiable: pass detached matrices or call it under no_grad")
-    if not listed:
-        return torch.empty_like(mats) if isinstance(mats, Tensor) else []
-    dev = listed[0].device
     srcs = [t.contiguous() for t in listed]
     stacked = torch.empty(mats.shape, device=dev, dtype=mats.dtype) if isinstance(mats, Tensor) else None
     outs = [torch.empty(t.shape, device=dev, dtype=t.dtype) for t in srcs] if stacked is None else \
         list(stacked.unbind(0)) if stacked.dim() == 3 else [stacked]
-    table = (_lib.Matrix * len(srcs))(*[_lib.Matrix(s.data_ptr(), o.data_ptr(), None, None, *s.shape) for s, o in zip(srcs, outs)])
+    table = _matrix_table([(s.data_ptr(), o.data_ptr(), 0, 0, *s.shape) for s, o in zip(srcs, outs)])
     ws, need = _ns_workspace(table, len(srcs), dev)
-    with torch.cuda.device(dev):
-        check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[srcs[0].dtype], schedule, steps, eps, _p(ws), need, _stream()))
+    with _on(dev):
+        check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[dtype], schedule, steps, eps, _p(ws), need, _stream_on(dev)))
     return outs if stacked is None else stacked
 
 
@@ -805,28 +835,31 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     if not params:
         return
     dev = params[0].device
+    if not params[0].is_cuda:
+        raise RuntimeError(f"nerf_amd runs on ROCm devices only: `params` is on {dev}")
     spans = []
     for w, g, m in zip(params, grads, momenta):
+        shape = w.shape
         for name, t in (("params", w), ("grads", g), ("momenta", m)):
-            if not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.dim() == 2 and t.shape == w.shape):
+            if t.device != dev or t.dtype != torch.float32 or t.dim() != 2 or t.shape != shape:
                 raise RuntimeError(f"muon_step: `{name}` must be fp32 matrices of one shape on one ROCm device")
-        for name, t in (("params", w), ("momenta", m)):
-            if not t.is_contiguous():
-                raise RuntimeError(f"muon_step: `{name}` must be contiguous (they are written in place)")
-            spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel()))
-    spans = sorted(s for s in spans if s[0] != s[1])
+        if not (w.is_contiguous() and m.is_contiguous()):
+            raise RuntimeError("muon_step: params and momenta must be contiguous (they are written in place)")
+        size = 4 * shape[0] * shape[1]
+        if size:
+            spans += [(w.data_ptr(), w.data_ptr() + size), (m.data_ptr(), m.data_ptr() + size)]
+    spans.sort()
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise RuntimeError("muon_step: two of `params` and `momenta` share memory")
     for name, t in (("grad_scale", grad_scale), ("found_inf", found_inf)):
         if t is not None and not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.numel() == 1):
             raise RuntimeError(f"muon_step: `{name}` must be one fp32 element on {dev}")
     srcs = [g.detach().contiguous() for g in grads]
-    table = (_lib.Matrix * len(params))(*[_lib.Matrix(g.data_ptr(), None, w.data_ptr(), m.data_ptr(), *w.shape)
-                                          for w, g, m in zip(params, srcs, momenta)])
+    table = _matrix_table([(g.data_ptr(), 0, w.data_ptr(), m.data_ptr(), *w.shape) for w, g, m in zip(params, srcs, momenta)])
     ws, need = _ns_workspace(table, len(params), dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(lib.nerfx_muon_step(table, len(params), lr, momentum, int(nesterov), weight_decay, _LR_RULES[adjust_lr], schedule,
-                                  steps, eps, _p(grad_scale), _p(found_inf), _p(ws), need, _stream()))
+                                  steps, eps, _p(grad_scale), _p(found_inf), _p(ws), need, _stream_on(dev)))
     for t in params + momenta:                              # written through raw pointers: tell autograd
         torch.autograd.graph.increment_version(t)           # and the packed-weight cache of ModelHandle
 
@@ -872,8 +905,9 @@ class Mx4:
         if not self.codes.is_cuda:
             raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {self.codes.device}")
         out = torch.empty(self.shape, device=self.device, dtype=dtype)
-        with torch.cuda.device(self.device):
-            check(lib.nerfx_mx4_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.k, _TYPES[dtype], _p(out), _stream()))
+        with _on(self.device):
+            check(lib.nerfx_mx4_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.k, _TYPES[dtype], _p(out),
+                                           _stream_on(self.device)))
         return out
 
 
@@ -901,8 +935,8 @@ def mx4_quantize(x: Tensor) -> Mx4:
     blocks = (k + 31) // 32
     codes = torch.empty((rows, 16 * blocks), device=x.device, dtype=torch.uint8)
     scales = torch.empty((rows, blocks), device=x.device, dtype=torch.uint8)
-    with torch.cuda.device(x.device):
-        check(lib.nerfx_mx4_quantize(_p(x), _TYPES[x.dtype], rows, k, _p(codes), _p(scales), _stream()))
+    with _on(x.device):
+        check(lib.nerfx_mx4_quantize(_p(x), _TYPES[x.dtype], rows, k, _p(codes), _p(scales), _stream_on(x.device)))
     return Mx4(codes, scales, k)
 
 
@@ -945,9 +979,9 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
     y = torch.empty((*lead, n), device=dev, dtype=out_dtype)
     need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt)
     ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         check(lib.nerfx_mx4_linear(_p(src), dt, _p(scales), m, k, _p(weight.codes), _p(weight.scales), n, _p(bias),
-                                   _LINEAR_ACTS[activation], _p(y), _TYPES[out_dtype], _p(ws), max(need, 0), _stream()))
+                                   _LINEAR_ACTS[activation], _p(y), _TYPES[out_dtype], _p(ws), max(need, 0), _stream_on(dev)))
     return y
 
 

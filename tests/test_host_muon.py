@@ -22,10 +22,13 @@ def test_workspace_bytes():
     from nerf_amd import _lib
     size = _lib.lib.nerfx_orthogonalize_workspace_bytes
     assert size(None, 0) == 0 and size(_table(_lib, (0, 5), (5, 0)), 2) == 0
-    assert size(_table(_lib, (1, 1)), 1) >= 5 * 64 * 64 * 4
+    assert size(_table(_lib, (300, 300)), 1) >= 5 * 300 * 300 * 4
     # matrices of one group lie side by side; a 33rd starts a group that reuses the space
-    one = size(_table(_lib, (64, 64)), 1)
-    assert size(_table(_lib, *[(64, 64)] * 32), 32) == 32 * one == size(_table(_lib, *[(64, 64)] * 33), 33)
+    three = size(_table(_lib, *[(300, 300)] * 3), 3)
+    assert size(_table(_lib, (300, 300)), 1) < three < size(_table(_lib, *[(300, 300)] * 32), 32)
+    assert size(_table(_lib, *[(300, 300)] * 32), 32) == size(_table(_lib, *[(300, 300)] * 33), 33)
+    # small matrices by themselves stay inside their workgroups
+    assert size(_table(_lib, (64, 256), (1, 1)), 2) == 0 and size(_table(_lib, (65, 65)), 1) > 0
     assert size(_table(_lib, (256, 39)), 1) == size(_table(_lib, (39, 256)), 1)
     assert size(None, 1) == -1
     assert size(_table(_lib, (-1, 4)), 1) == -1 and size(_table(_lib, (4, 32769)), 1) == -1
@@ -42,7 +45,7 @@ def test_c_refusals_of_orthogonalize(change, text):
     lib = _lib.lib
     coef = change.get("coef", COEF * change.get("steps", 1) or COEF)
     arr = None if coef is None else (C.c_float * max(3, len(coef)))(*coef)
-    rc = lib.nerfx_orthogonalize(_table(_lib, (8, 8), ptr=change.get("ptr", 4096)), 1, change.get("dtype", 0), arr, change.get("steps", 1),
+    rc = lib.nerfx_orthogonalize(_table(_lib, (80, 80), ptr=change.get("ptr", 4096)), 1, change.get("dtype", 0), arr, change.get("steps", 1),
                                  change.get("eps", 1e-7), C.c_void_p(change.get("ws", 4096)), change.get("bytes", 1 << 40), None)
     assert rc == -1 and text in lib.nerfx_last_error(), lib.nerfx_last_error()
 
