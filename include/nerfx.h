@@ -399,12 +399,13 @@ int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
                          void* stream);
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
  * x_scales its scales; NULL otherwise), W (n, k) as codes and scales, bias (n) fp32 or NULL, sums in fp32,
- * y in y_dtype (fp32, bf16 or f16), activ NERFX_ACT_*.  x and the weight's codes aligned to 16 bytes.
+ * activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as above along n, y its codes and
+ * y_scales its scales; NULL otherwise).  x, the weight's codes and y's codes aligned to 16 bytes.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
-int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype);
+int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,
                      const uint8_t* w_codes, const uint8_t* w_scales, int n, const float* bias, int activ,
-                     void* y, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+                     void* y, int y_dtype, uint8_t* y_scales, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Distillation loss of distill.py:120-130 and its gradient w.r.t. the student's outputs:
  * loss = mean_i [ mean_j (alpha(s_sigma_i, delta_j) - alpha(t_sigma_i, delta_j))^2

@@ -82,8 +82,8 @@ SIGNATURES = {
     "nerfx_muon_step": (_i, [C.POINTER(Matrix), _i, _d, _d, _i, _d, _i, C.POINTER(_f), _i, _f, _p, _p, _p, _l, _p]),
     "nerfx_mx4_quantize": (_i, [_p, _i, _l, _i, _p, _p, _p]),
     "nerfx_mx4_dequantize": (_i, [_p, _p, _l, _i, _i, _p, _p]),
-    "nerfx_mx4_linear_workspace_bytes": (_l, [_l, _i, _i, _i]),
-    "nerfx_mx4_linear": (_i, [_p, _i, _p, _l, _i, _p, _p, _i, _p, _i, _p, _i, _p, _l, _p]),
+    "nerfx_mx4_linear_workspace_bytes": (_l, [_l, _i, _i, _i, _i]),
+    "nerfx_mx4_linear": (_i, [_p, _i, _p, _l, _i, _p, _p, _i, _p, _i, _p, _i, _p, _p, _l, _p]),
     "nerfx_voxel_sample": (_i, [_f, _f, _f, _f, _f, _f, _f, _f, _i, _i, C.c_uint64, C.c_uint64, _p, _p, _p, _p]),
     "nerfx_distill_loss": (_i, [_p, _p, _p, _p, _p, _l, _p, _p, _p, _p, _p]),
     "nerfx_debug_set_stamps": (None, [_p]),

@@ -135,6 +135,26 @@ __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, const float16_
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = acc[e];
     mx4_activate16(v, a.activ);
+    if (a.y_dtype == NERFX_TYPE_MX4) {                         // the tile's 32 columns are a block of y
+        using Raw = Mx4Raw<NERFX_TYPE_F32, 16>;
+        Raw raw;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) raw.w[e] = n0 + 8 * (e >> 2) + 4 * h + (e & 3) < a.n ? __builtin_bit_cast(uint32_t, v[e]) : 0u;
+        uint32_t top = raw.top_bits();
+        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        const uint32_t byte = Raw::scale_byte(max(both[0], both[1]));
+        const float scale = Raw::scale_value(byte);
+        // this lane's codes are the lower (h = 0) or upper halves of the block's four words: after the exchange the lower lane
+        // has all of the first two, the upper lane of the other two
+        const auto half = __builtin_amdgcn_permlane32_swap(raw.codes(0, scale), raw.codes(1, scale), false, false);
+        u32x2_t w = {__builtin_amdgcn_perm(half[1], half[0], 0x05040100u), __builtin_amdgcn_perm(half[1], half[0], 0x07060302u)};
+        if (byte == 255u) w = {0, 0};
+        if (m >= a.m) return;
+        const int64_t block = m * mx4_blocks(a.n) + n0 / MX4_BLOCK;
+        *(u32x2_t*)((char*)a.y + block * MX4_BLOCK_BYTES + 8 * h) = w;
+        if (h == 0) a.y_scales[block] = (uint8_t)byte;
+        return;
+    }
     if (a.y_dtype == NERFX_TYPE_F32) {
         if (m >= a.m) return;
         float* y = (float*)a.y + m * a.n;
@@ -621,8 +641,9 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 }
 
 // How a product is done, by its sizes:
-//  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes: W is read once, by as many workgroups as it has
-//          rows (one row by 4096 x 4096: 62 us with tiles);
+//  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes (else by way of the workspace): W is read once, by
+//          as many workgroups as it has 16 rows (one row by 4096 x 4096: 62 us with tiles).  Not for a result in blocks, which
+//          are of 32 columns;
 //  stream  otherwise up to 256 columns and 512 values a row: float rows of 64, 128, 192, 256, 320 or 512 values are quantised in
 //          registers, others into the workspace first;
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.
@@ -632,16 +653,16 @@ static int stream_steps(int k) {
     const int ks = (k + 63) / 64;
     return ks <= 5 ? ks : 8;
 }
-static int mx4_plan(int64_t m, int n, int k, int x_dtype, bool& stage) {
-    const bool is_float = x_dtype != NERFX_TYPE_MX4;
+static int mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype, bool& stage) {
+    const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
     stage = false;
-    if (m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
-    if (n <= 256 && k <= 512 && m > SKINNY_ROWS) {
+    if (!blocks_out && m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
+    if (n <= 256 && k <= 512 && (blocks_out || m > SKINNY_ROWS)) {
         stage = is_float && k != 64 * stream_steps(k);
         return MX4_STREAM;
     }
     stage = is_float;
-    return m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
+    return !blocks_out && m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
 }
 
 template <int DT>
@@ -725,36 +746,40 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
     return launch_status("mx4_dequantize_kernel");
 }
 
-extern "C" int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype) {
-    if (check_mx4(m, k) || check_mx4(n, k) || !(float_type(x_dtype) || x_dtype == NERFX_TYPE_MX4)) return -1;
+static bool mx4_type(int dtype) { return float_type(dtype) || dtype == NERFX_TYPE_MX4; }
+
+extern "C" int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype) {
+    if (check_mx4(m, k) || check_mx4(n, k) || !mx4_type(x_dtype) || !mx4_type(y_dtype)) return -1;
     bool stage;
-    mx4_plan(m, n, k, x_dtype, stage);
+    mx4_plan(m, n, k, x_dtype, y_dtype, stage);
     if (!stage) return 0;
     return (m * mx4_blocks(k) * 17 + 15) / 16 * 16;
 }
 
 extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k, const uint8_t* w_codes,
                                 const uint8_t* w_scales, int n, const float* bias, int activ, void* y, int y_dtype,
-                                void* workspace, int64_t workspace_bytes, void* stream) {
+                                uint8_t* y_scales, void* workspace, int64_t workspace_bytes, void* stream) {
     if (int rc = check_mx4(m, k)) return rc;
     if (int rc = check_mx4(n, k)) return rc;
-    NERFX_REQUIRE(float_type(x_dtype) || x_dtype == NERFX_TYPE_MX4, "unknown type %d of x", x_dtype);
-    NERFX_REQUIRE(float_type(y_dtype), "unknown type %d of y", y_dtype);
+    NERFX_REQUIRE(mx4_type(x_dtype), "unknown type %d of x", x_dtype);
+    NERFX_REQUIRE(mx4_type(y_dtype), "unknown type %d of y", y_dtype);
     NERFX_REQUIRE(activ >= NERFX_ACT_NONE && activ <= NERFX_ACT_SILU, "unknown activation %d", activ);
     if (m == 0 || n == 0) return 0;
-    NERFX_REQUIRE(x && w_codes && w_scales && y && (x_dtype != NERFX_TYPE_MX4 || x_scales), "a required pointer is NULL");
+    NERFX_REQUIRE(x && w_codes && w_scales && y && (x_dtype != NERFX_TYPE_MX4 || x_scales) && (y_dtype != NERFX_TYPE_MX4 || y_scales),
+                  "a required pointer is NULL");
+    NERFX_REQUIRE(y_dtype != NERFX_TYPE_MX4 || aligned16(y), "y's codes are not aligned to 16 bytes");
     NERFX_REQUIRE(aligned16(w_codes) && aligned16(x), "x or the weight's codes are not aligned to 16 bytes");
-    const int64_t need = nerfx_mx4_linear_workspace_bytes(m, n, k, x_dtype);
+    const int64_t need = nerfx_mx4_linear_workspace_bytes(m, n, k, x_dtype, y_dtype);
     NERFX_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
                   "workspace NULL, not aligned to 16 bytes, or of %lld bytes with %lld needed", (long long)workspace_bytes, (long long)need);
     Mx4LinearArgs a{};
-    a.w = w_codes; a.w_scales = w_scales; a.bias = bias; a.y = y;
+    a.w = w_codes; a.w_scales = w_scales; a.bias = bias; a.y = y; a.y_scales = y_scales;
     a.m = m; a.n = n; a.k = k; a.activ = activ; a.y_dtype = y_dtype;
     a.y_whole = aligned16(y) && n % (y_dtype == NERFX_TYPE_F32 ? 4 : 8) == 0;
     a.x = (const uint8_t*)x; a.x_scales = x_scales;
     const hipStream_t st = (hipStream_t)stream;
     bool stage;
-    const int plan = mx4_plan(m, n, k, x_dtype, stage);
+    const int plan = mx4_plan(m, n, k, x_dtype, y_dtype, stage);
     if (stage) {
         uint8_t* codes = (uint8_t*)workspace;
         uint8_t* scales = codes + m * mx4_blocks(k) * 16;

@@ -895,6 +895,13 @@ class Mx4:
     def device(self):
         return self.codes.device
 
+    @staticmethod
+    def cat(parts) -> "Mx4":
+        """Columns side by side; every part but the last has to end with a whole block."""
+        if any(p.k % 32 for p in parts[:-1]):
+            raise ValueError(f"Mx4.cat: widths {[p.k for p in parts]}: all but the last must be multiples of 32")
+        return Mx4(torch.cat([p.codes for p in parts], 1), torch.cat([p.scales for p in parts], 1), sum(p.k for p in parts))
+
     def to(self, device) -> "Mx4":
         return Mx4(self.codes.to(device), self.scales.to(device), self.k)
 
@@ -940,11 +947,12 @@ def mx4_quantize(x: Tensor) -> Mx4:
     return Mx4(codes, scales, k)
 
 
-def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Optional[str] = None, out_dtype=None) -> Tensor:
+def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Optional[str] = None, out_dtype=None):
     """activation(Q(x) @ weight.T + bias) with both factors in 4 bits and fp32 sums: what a frozen Linear layer packed with
     `mx4_quantize` answers.  `x` (..., k): fp32, bf16 or fp16, quantised as `mx4_quantize` does on its way, or an `Mx4`; `weight`
     (n, k); `bias` (n) fp32; `activation` None, "relu", "leaky_relu" (slope 0.01) or "silu".  -> (..., n) in `out_dtype`
-    (default: x's type, fp32 for an `Mx4`).  No gradient."""
+    (default: x's type, fp32 for an `Mx4`), or, with out_dtype="mx4", the result quantised on its way out: an `Mx4` of
+    prod(...) rows, what the next layer takes.  No gradient."""
     if not isinstance(weight, Mx4):
         raise TypeError("weight must be an Mx4 (see mx4_quantize)")
     if activation not in _LINEAR_ACTS:
@@ -970,19 +978,25 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
         if tuple(bias.shape) != (n,) or bias.device != dev:
             raise ValueError(f"bias must be ({n},) on {dev}")
         bias = _dev(bias.detach(), "bias")
-    out_dtype = default if out_dtype is None else out_dtype
-    if out_dtype not in _TYPES:
-        raise TypeError(f"mx4_linear gives fp32, bf16 or fp16 (asked for {out_dtype})")
     m = 1
     for s in lead:
         m *= s
-    y = torch.empty((*lead, n), device=dev, dtype=out_dtype)
-    need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt)
+    if out_dtype == "mx4":
+        out = Mx4(torch.empty((m, 16 * ((n + 31) // 32)), device=dev, dtype=torch.uint8),
+                  torch.empty((m, (n + 31) // 32), device=dev, dtype=torch.uint8), n)
+        y, y_scales, yt = out.codes, out.scales, _lib.TYPE_MX4
+    else:
+        out_dtype = default if out_dtype is None else out_dtype
+        if out_dtype not in _TYPES:
+            raise TypeError(f"mx4_linear gives fp32, bf16, fp16 or \"mx4\" (asked for {out_dtype})")
+        out = y = torch.empty((*lead, n), device=dev, dtype=out_dtype)
+        y_scales, yt = None, _TYPES[out_dtype]
+    need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt, yt)
     ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
     with _on(dev):
         check(lib.nerfx_mx4_linear(_p(src), dt, _p(scales), m, k, _p(weight.codes), _p(weight.scales), n, _p(bias),
-                                   _LINEAR_ACTS[activation], _p(y), _TYPES[out_dtype], _p(ws), max(need, 0), _stream_on(dev)))
-    return y
+                                   _LINEAR_ACTS[activation], _p(y), yt, _p(y_scales), _p(ws), max(need, 0), _stream_on(dev)))
+    return out
 
 
 def voxel_sample(domain, voxels: int, samples: int, device, rng=None):

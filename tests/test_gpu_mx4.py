@@ -181,6 +181,25 @@ def test_linear_of_a_quantized_input(ops, m, n, k):
     assert ops.mx4_linear(q, ops.mx4_quantize(w)).dtype == torch.float32
 
 
+@pytest.mark.parametrize("act", [None, "relu", "silu"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (3, 40, 39), (64, 256, 256), (129, 256, 295), (300, 31, 96), (300, 256, 256), (500, 300, 64),
+                                   (515, 700, 1032), (200, 64, 600)])
+def test_linear_into_blocks(ops, m, n, k, act):
+    """A result quantised on its way out is the fp32 result, which the same product gives, quantised."""
+    for dtype in TYPES:
+        x, w, bias = pair(m, n, k, dtype, 8)
+        x[m // 2, k // 2] = float("nan") if m > 100 else 1.0
+        qw, qx = ops.mx4_quantize(w), ops.mx4_quantize(x)
+        got = ops.mx4_linear(qx, qw, bias, act, "mx4")
+        assert got.shape == (m, n)
+        plain = ops.mx4_linear(torch.cat((qx.dequantize(), torch.zeros(100, k, device="cuda"))), qw, bias, act)[:m]
+        want = ops.mx4_quantize(plain)                                  # more rows: the same kernels as for blocks
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+        again = ops.mx4_linear(x, qw, bias, act, "mx4")
+        assert torch.equal(got.codes, again.codes) and torch.equal(got.scales, again.scales)
+    assert ops.mx4_linear(x.view(1, m, k), qw, bias, act, "mx4").shape == (m, n)
+
+
 def test_linear_shapes_views_and_empty(ops):
     x, w, bias = pair(24, 40, 64, torch.float32, 3)
     qw = ops.mx4_quantize(w)
@@ -228,10 +247,10 @@ def test_linear_writes_nothing_beside_its_result(ops):
         qw = ops.mx4_quantize(w)
         buf = torch.full((m * n + 512,), 3.0, device="cuda", dtype=dt)
         y = buf[256:256 + m * n]
-        need = _lib.lib.nerfx_mx4_linear_workspace_bytes(m, n, k, code)
+        need = _lib.lib.nerfx_mx4_linear_workspace_bytes(m, n, k, code, code)
         ws = torch.empty(max(need, 1), device="cuda", dtype=torch.uint8)
         p = lambda t: C.c_void_p(t.data_ptr())
-        _lib.check(_lib.lib.nerfx_mx4_linear(p(x), code, None, m, k, p(qw.codes), p(qw.scales), n, p(bias), 0, p(y), code, p(ws), need,
+        _lib.check(_lib.lib.nerfx_mx4_linear(p(x), code, None, m, k, p(qw.codes), p(qw.scales), n, p(bias), 0, p(y), code, None, p(ws), need,
                                              C.c_void_p(torch.cuda.current_stream().cuda_stream)))
         assert bool((buf[:256] == 3).all()) and bool((buf[256 + m * n:] == 3).all())
         assert torch.equal(y.view(m, n), ops.mx4_linear(x, qw, bias, "relu"))

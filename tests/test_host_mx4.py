@@ -16,10 +16,11 @@ def _mx4(ops, rows=4, k=64):
 def test_workspace_bytes():
     from nerf_amd import _lib
     size = _lib.lib.nerfx_mx4_linear_workspace_bytes
-    assert size(10, 4, 33, _lib.TYPE_MX4) == 0
-    assert size(-1, 4, 4, 0) == size(4, -1, 4, 0) == size(4, 4, 0, 0) == size(4, 4, (1 << 20) + 1, 0) == size(4, 4, 4, 9) == -1
-    assert size(1 << 31, 4, 4, 0) == -1
-    assert size(524288, 256, 256, _lib.TYPE_BF16) >= 0
+    assert size(10, 4, 33, _lib.TYPE_MX4, 0) == 0
+    assert size(-1, 4, 4, 0, 0) == size(4, -1, 4, 0, 0) == size(4, 4, 0, 0, 0) == size(4, 4, (1 << 20) + 1, 0, 0) == -1
+    assert size(4, 4, 4, 9, 0) == size(4, 4, 4, 0, 9) == size(1 << 31, 4, 4, 0, 0) == -1
+    assert size(524288, 256, 256, _lib.TYPE_BF16, _lib.TYPE_BF16) == 0          # quantised in registers
+    assert size(524288, 256, 295, _lib.TYPE_BF16, _lib.TYPE_MX4) >= 524288 * 10 * 17
 
 
 def test_c_refusals():
@@ -41,14 +42,18 @@ def test_c_refusals():
     refused(lib.nerfx_mx4_dequantize(p, p, 4, (1 << 20) + 1, 0, p, None), b"k ")
     refused(lib.nerfx_mx4_dequantize(p + 1, p, 4, 8, 0, p, None), b"aligned")
 
-    def linear(x=p, xt=0, xs=None, m=4, k=64, w=p, ws=p, n=4, act=0, y=p, yt=0, work=p, size=1 << 40):
-        return lib.nerfx_mx4_linear(x, xt, xs, m, k, w, ws, n, None, act, y, yt, work, size, None)
+    def linear(x=p, xt=0, xs=None, m=4, k=64, w=p, ws=p, n=4, act=0, y=p, yt=0, ys=None, work=p, size=1 << 40):
+        return lib.nerfx_mx4_linear(x, xt, xs, m, k, w, ws, n, None, act, y, yt, ys, work, size, None)
 
     refused(linear(m=-1), b"rows")
     refused(linear(n=-1), b"rows")
     refused(linear(k=0), b"k 0")
     refused(linear(xt=4), b"of x")
-    refused(linear(yt=3), b"of y")
+    refused(linear(yt=4), b"of y")
+    refused(linear(yt=3), b"NULL")                                     # codes without scales
+    refused(linear(yt=3, ys=p, y=p + 8), b"aligned")
+    refused(linear(m=100, k=65, size=0), b"workspace")
+    refused(linear(m=100, k=65, work=None), b"workspace")
     refused(linear(act=3), b"activation")
     refused(linear(act=-2), b"activation")
     for name in ("x", "w", "ws", "y"):
@@ -67,6 +72,10 @@ def test_mx4_checks_its_parts(ops):
                 (codes[0], scales, 64), (codes, scales[:3], 64), (codes.t(), scales, 64), (codes[:, :16], scales, 32)):
         with pytest.raises(ValueError):
             ops.Mx4(*bad)
+    both = ops.Mx4.cat([t, _mx4(ops, 4, 39)])
+    assert both.shape == (4, 103) and both.codes.shape == (4, 64)
+    with pytest.raises(ValueError, match="32"):
+        ops.Mx4.cat([_mx4(ops, 4, 39), t])
     flat = torch.zeros(200, dtype=torch.uint8)
     start = next(i for i in range(16) if (flat.data_ptr() + i) % 16 == 8)
     with pytest.raises(ValueError, match="aligned"):
