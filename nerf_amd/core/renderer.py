@@ -10,6 +10,7 @@ import torch
 from torch import Tensor
 
 from .. import ops
+from .mx4 import Mx4NeRF
 
 
 class BoundedVolumeRaymarcher:
@@ -44,6 +45,10 @@ class BoundedVolumeRaymarcher:
         inference_mode / no_grad (infer.py:13, train.py:71 for the val and test splits,
         bench.py:149); a caller that wants gradients passes train=True."""
         nc, nf = self.samples_c, self.samples_f
+        if isinstance(coarse, Mx4NeRF) or (nf > 0 and isinstance(fine, Mx4NeRF)):
+            if train:
+                raise RuntimeError("[NeRF] a 4-bit field is frozen: render it with train=False")
+            return self._render_fields(coarse, fine, ro, rd, perturb)
         rng = ops.next_rng(ro.device) if (perturb and ro.is_cuda) else None
         if train:
             if nf > 0:
@@ -53,3 +58,26 @@ class BoundedVolumeRaymarcher:
             hc = ops.handle_for(coarse)
             hf = ops.handle_for(fine) if nf > 0 else None
             return ops.render(hc, hf, ro, rd, self.tn, self.tf, nc, nf, rng=rng)
+
+    @torch.no_grad()
+    def _render_fields(self, coarse, fine, ro: Tensor, rd: Tensor, perturb: bool):
+        """The stages of `ops.render` one after the other, where a field has no kernel to be called inside of them."""
+        nc, nf = self.samples_c, self.samples_f
+        ro, rd = ops._dev(ro, "ro"), ops._dev(rd, "rd")
+        u_c = u_f = None
+        if perturb:
+            rng = ops.next_rng(ro.device)
+            u_c = ops.rng_uniform(rng, 0, ro.size(0) * nc, ro.device).view(-1, nc)
+            u_f = ops.rng_uniform(rng, 1, ro.size(0) * nf, ro.device).view(-1, nf) if nf > 0 else None
+
+        def field(model, t: Tensor, density_only: bool = False):
+            if isinstance(model, Mx4NeRF):
+                return model.rays(ro, rd, t, density_only)
+            return ops.mlp_rays(ops.handle_for(model), ro, rd, t, density_only)
+
+        t = ops.sample_encode(ro, rd, self.tn, self.tf, nc, u_c, want_rx=False)["t"]
+        if nf > 0:
+            t = ops.coarse_pdf_sample(field(coarse, t, True)[0], t, rd, nf, u_f)
+        sigma, rgb = field(fine if nf > 0 else coarse, t)
+        weights, rgb_map, depth = ops.composite_fwd(sigma, rgb, t, rd)
+        return t, weights, depth, rgb_map

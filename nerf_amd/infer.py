@@ -4,6 +4,7 @@ from torch import Tensor
 
 from . import ops
 from .core.model import NeRF
+from .core.mx4 import Mx4NeRF
 from .core.renderer import BoundedVolumeRaymarcher as BVR
 from .utils.pbar import tqdm
 
@@ -60,3 +61,4 @@ def orbit(coarse: NeRF, fine: NeRF, raymarcher: BVR, poses: Tensor, H: int, W: i
 
 
 NeRF.infer = infer
+Mx4NeRF.infer = infer
