@@ -184,7 +184,7 @@ struct SplitTile {
     static constexpr int STAGE_BYTES = 2 * T * SPLIT_BLOCK_BYTES;
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
     static_assert(STAGES >= 2 && STAGES <= 8 && 2 * LOADS * (STAGES - 1) < 64, "waits of landed()");
-    float16_t_ acc[FP][FQ];
+    float16_t_ acc[FP][FQ], cross[FP][FQ];
 
     // Until all stages but the newest `later` have landed.
     static __device__ __forceinline__ void wait(int later) {
@@ -211,16 +211,19 @@ struct SplitTile {
 #pragma unroll
         for (int j = 0; j < FQ; ++j) { f.qh[j] = frag(q_row + 32 * j, c); f.ql[j] = frag(q_row + 32 * j, c + 4); }
     }
-    // the three products of a fragment lie apart, so that no instruction waits for the one before
+    // hi hi goes into sums of its own: what rounds each time is then K / 16 additions at the result's size, and the two thirds
+    // that the cross terms are round at theirs, 2^-11 of it.  (In one sum a Gram matrix of rows of 1,500 was 1e-6 off.)
     __device__ __forceinline__ void multiply(const Frags& f) {
 #pragma unroll
         for (int t = 0; t < 3; ++t)
 #pragma unroll
             for (int i = 0; i < FP; ++i)
 #pragma unroll
-                for (int j = 0; j < FQ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(t == 1 ? f.pl[i] : f.ph[i], t == 0 ? f.ql[j] : f.qh[j],
-                                                                       acc[i][j], 0, 0, 0);
+                for (int j = 0; j < FQ; ++j) {
+                    if (t == 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.qh[j], acc[i][j], 0, 0, 0);
+                    else cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(t == 2 ? f.pl[i] : f.ph[i], t == 0 ? f.ql[j] : f.qh[j],
+                                                                              cross[i][j], 0, 0, 0);
+                }
     }
 
     __device__ __forceinline__ void run(char* lds, const char* P, const char* Q, int K) {
@@ -245,7 +248,7 @@ struct SplitTile {
 #pragma unroll
             for (int j = 0; j < FQ; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = cross[i][j][e] = 0.f;
 #pragma unroll
         for (int kb = 0; kb < STAGES; ++kb)
             if (kb < steps) fetch(kb);
@@ -263,6 +266,10 @@ struct SplitTile {
         read(f1, lds + ((steps - 1) % STAGES) * STAGE_BYTES, 1, wave, lane);
         multiply(f0);
         multiply(f1);
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) acc[i][j] += cross[i][j];
     }
     // where in the tile a wave's part begins
     static __device__ __forceinline__ int row_of(int wave) { return wave / (WAVES / 2) * (T / 2); }
@@ -398,9 +405,9 @@ __device__ __forceinline__ void small_put(char* m, int at, float v) {
 __device__ __forceinline__ float16_t_ small_product(const char* P, int p0, int p_pitch, const char* Q, int q0, int q_pitch, int K) {
     const int lane = threadIdx.x & 63, p = p0 + (lane & 31), q = q0 + (lane & 31), h = lane >> 5;
     const int pv = p * p_pitch + ((h ^ (p & 15)) * 16), qv = q * q_pitch + ((h ^ (q & 15)) * 16);
-    float16_t_ main, cross;
+    float16_t_ main, cross, low;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) main[e] = cross[e] = 0.f;
+    for (int e = 0; e < 16; ++e) main[e] = cross[e] = low[e] = 0.f;
     for (int kb = 0; kb < K / 64; ++kb) {
         half8_t ph[4], pl[4], qh[4], ql[4];
 #pragma unroll
@@ -410,13 +417,16 @@ __device__ __forceinline__ float16_t_ small_product(const char* P, int p0, int p
             qh[s] = *(const half8_t*)(Q + kb * 256 + (qv ^ c)); ql[s] = *(const half8_t*)(Q + kb * 256 + (qv ^ (c + 64)));
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {                                          // two chains: neither waits for the other
+        // Here lo lo is not left out: it costs nothing (latency bounds these products), and with a few elements to a sum there
+        // is little for its 2^-24 to average out in.
+        for (int s = 0; s < 4; ++s) {
             cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[s], ql[s], cross, 0, 0, 0);
             main = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[s], qh[s], main, 0, 0, 0);
             cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[s], qh[s], cross, 0, 0, 0);
+            low = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[s], ql[s], low, 0, 0, 0);
         }
     }
-    return main + cross;
+    return main + (cross + low);
 }
 
 struct OrthoSteps { float coef[3 * ORTHO_MAX_STEPS]; int32_t steps; float sx, sa, sb; };
