@@ -10,22 +10,30 @@
 namespace nerfx {
 
 // ---- to and from -----------------------------------------------------------------------------------------------------
-// Four lanes make a block, eight values each: every load and store of a wave is one run of memory.  Bound by
-// memory: x is read once, 4.25 bits a value are written.
+// Four lanes make a block, eight values each: every load and store of a wave is one run of memory.  Bound by memory (524,288 x
+// 256 bf16: 5.4 TB/s to, 5.4 TB/s from), as long as nothing but the conversion instructions touches the values: where rows are
+// whole blocks the matrix is one run (MX4_FULL), and no division finds the row.
+enum { MX4_VALUES, MX4_PIECES, MX4_FULL };     // rows value by value; whole 16-byte pieces, aligned; whole blocks as well
+
+// Value eight of part `q` begins at `at` of `row`; its place in memory is row * k + at.
+__device__ __forceinline__ int64_t mx4_place(uint64_t q, int k, int how, int& at) {
+    if (how == MX4_FULL) { at = 0; return (int64_t)q * 8; }    // at: only compared with k, and every part is whole
+    const uint32_t nb = mx4_blocks(k);
+    const uint64_t block = q >> 2, row = block >> 32 ? block / nb : (uint32_t)block / nb;
+    at = (int)(block - row * nb) * MX4_BLOCK + (int)(q & 3) * 8;
+    return (int64_t)row * k + at;
+}
+
 template <int DT>
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t rows, int k, int whole,
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t parts, int k, int how,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     using Raw = Mx4Raw<DT, 8>;
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
-    const int nb = mx4_blocks(k);
-    const int64_t total = rows * nb * 4;
-    const int part = threadIdx.x & 3;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-        const int64_t block = q >> 2, row = block / nb;
-        const int at = (int)(block - row * nb) * MX4_BLOCK + part * 8;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
+        int at;
+        const char* src = (const char*)x + mx4_place(q, k, how, at) * SIZE;
         Raw v;
-        const char* src = (const char*)x + (row * k + at) * SIZE;
-        if (whole && at + 8 <= k) {                            // 16-byte pieces; k is a multiple of 8
+        if (how != MX4_VALUES && at + 8 <= k) {
 #pragma unroll
             for (int i = 0; i < Raw::WORDS / 4; ++i) {
                 const u32x4_t p = *(const u32x4_t*)(src + 16 * i);
@@ -48,41 +56,41 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restric
         top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
         const uint32_t byte = Raw::scale_byte(top);
         codes[q] = byte == 255u ? 0u : v.codes(0, Raw::scale_value(byte));
-        if (part == 0) scales[block] = (uint8_t)byte;
+        if ((q & 3) == 0) scales[q >> 2] = (uint8_t)byte;
     }
 }
 
 template <int DT>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                             int64_t rows, int k, int whole, void* __restrict__ out) {
+                                                             int64_t parts, int k, int how, void* __restrict__ out) {
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
-    const int nb = mx4_blocks(k);
-    const int64_t total = rows * nb * 4;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-        const int64_t block = q >> 2, row = block / nb;
-        const int at = (int)(block - row * nb) * MX4_BLOCK + (int)(q & 3) * 8;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
+        int at;
+        char* dst = (char*)out + mx4_place(q, k, how, at) * SIZE;
         if (at >= k) continue;
-        const uint32_t c = codes[q], byte = scales[block];
+        const uint32_t c = codes[q], byte = scales[q >> 2];
+        const float scale = Mx4Raw<DT, 8>::scale_value(byte);
         uint32_t w[8 * SIZE / 4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t code = c >> (4 * i) & 15u, m = code & 7u;
-            // 0, 0.5 apart, code m is (2 + m % 2) 2^(m / 2 - 3) ... as a float; then times 2^(byte - 127)
-            const float grid = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (126u + (m >> 1)) << 23 | (m & 1u) << 22);
-            float v = byte == 255u ? __builtin_nanf("") : ldexpf(grid, (int)byte - 127);
-            v = code & 8u ? -v : v;
-            if constexpr (DT == NERFX_TYPE_F32) {
-                w[i] = __builtin_bit_cast(uint32_t, v);
-            } else {
-                const uint32_t h = DT == NERFX_TYPE_F16 ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v)
-                                                        : (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
-                if (i & 1) w[i / 2] |= h << 16; else w[i / 2] = h;
-            }
+#define NERFX_PAIR(s)                                                                                                                  \
+        if constexpr (DT == NERFX_TYPE_F32) {                                                                                          \
+            const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, s);                                                      \
+            const float lo = v[0], hi = v[1];                                                                                          \
+            w[2 * s] = __builtin_bit_cast(uint32_t, lo); w[2 * s + 1] = __builtin_bit_cast(uint32_t, hi);                              \
+        } else if constexpr (DT == NERFX_TYPE_BF16) {                                                                                  \
+            w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, s));                               \
+        } else {                                                                                                                       \
+            w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, s));                                \
         }
-        char* dst = (char*)out + (row * k + at) * SIZE;
-        if (whole && at + 8 <= k) {
+        NERFX_PAIR(0) NERFX_PAIR(1) NERFX_PAIR(2) NERFX_PAIR(3)
+#undef NERFX_PAIR
+        if (byte == 255u) {
 #pragma unroll
-            for (int i = 0; i < SIZE / 2; ++i) *(u32x4_t*)(dst + 16 * i) = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+            for (int i = 0; i < 2 * SIZE; ++i) w[i] = DT == NERFX_TYPE_F32 ? 0x7fc00000u : DT == NERFX_TYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+        }
+        if (how != MX4_VALUES && at + 8 <= k) {
+#pragma unroll
+            for (int i = 0; i < SIZE / 2; ++i)
+                __builtin_nontemporal_store((u32x4_t){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]}, (u32x4_t*)(dst + 16 * i));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -401,7 +409,6 @@ constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS =
 
 // One block of x, 32 values: whole blocks from aligned memory (MX4_FULL), whole pieces of 16 bytes from aligned memory
 // (MX4_PIECES), or value by value; zeros behind k.
-enum { MX4_VALUES, MX4_PIECES, MX4_FULL };
 template <int DT>
 __device__ __forceinline__ Mx4Raw<DT, 32> mx4_load_block(const char* row, int at, int k, int how) {
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, PIECE = 16 / SIZE;
@@ -619,15 +626,22 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
 // ---- host side -------------------------------------------------------------------------------------------------------
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// How the rows of a matrix in a float type can be read or written: see the kernels.
+static int mx4_rows(const void* p, int k, int dtype) {
+    if (!aligned16(p) || k % (dtype == NERFX_TYPE_F32 ? 4 : 8) != 0) return MX4_VALUES;
+    return k % MX4_BLOCK == 0 ? MX4_FULL : MX4_PIECES;
+}
+static dim3 mx4_grid(int64_t parts) { return dim3((unsigned)std::min<int64_t>((parts + 255) / 256, 256 * 32)); }
+
 static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_t* codes, uint8_t* scales, hipStream_t stream) {
-    const int64_t threads = rows * mx4_blocks(k) * 4;
-    const dim3 grid((unsigned)std::min<int64_t>((threads + 255) / 256, 256 * 32));
-    const int whole = k % 8 == 0 && aligned16(x);
-    uint32_t* c = (uint32_t*)codes;
-    if (dtype == NERFX_TYPE_F32) hipLaunchKernelGGL(mx4_quantize_kernel<NERFX_TYPE_F32>, grid, dim3(256), 0, stream, x, rows, k, whole, c, scales);
-    else if (dtype == NERFX_TYPE_BF16) hipLaunchKernelGGL(mx4_quantize_kernel<NERFX_TYPE_BF16>, grid, dim3(256), 0, stream, x, rows, k, whole, c, scales);
-    else hipLaunchKernelGGL(mx4_quantize_kernel<NERFX_TYPE_F16>, grid, dim3(256), 0, stream, x, rows, k, whole, c, scales);
-    return launch_status("mx4_quantize_kernel");
+    const int64_t parts = rows * mx4_blocks(k) * 4;
+    const int how = mx4_rows(x, k, dtype);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, stream, x, parts, k, how, (uint32_t*)codes, scales);
+        return launch_status("mx4_quantize_kernel");
+    };
+    return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32>)
+         : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16>) : go(mx4_quantize_kernel<NERFX_TYPE_F16>);
 }
 
 template <int FP, int WP, int FQ, int WQ>
@@ -670,7 +684,7 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     const int mt = (int)(a.m + 15) / 16, nb = mx4_blocks(a.k);
     const size_t codes = DT == NERFX_TYPE_MX4 ? 0 : (size_t)a.m * nb * 17, sums = (size_t)SKINNY_WAVES * mt * 1024;
     const size_t lds = std::max(codes, sums);
-    const int how = a.k % 32 == 0 ? MX4_FULL : a.k % (DT == NERFX_TYPE_F32 ? 4 : 8) == 0 ? MX4_PIECES : MX4_VALUES;
+    const int how = mx4_rows(a.x, a.k, DT);
     const dim3 grid((unsigned)((a.n + 15) / 16)), block(64 * SKINNY_WAVES);
     auto go = [&](auto kernel) {
         NERFX_OPT_IN_LDS(kernel, lds);
@@ -735,15 +749,14 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
     if (rows == 0) return 0;
     NERFX_REQUIRE(codes && scales && out, "codes / scales / out is NULL");
     NERFX_REQUIRE(((uintptr_t)codes & 3) == 0, "codes are not aligned to 4 bytes");
-    const int64_t threads = rows * mx4_blocks(k) * 4;
-    const dim3 grid((unsigned)std::min<int64_t>((threads + 255) / 256, 256 * 32));
-    const int whole = k % 8 == 0 && aligned16(out);
-    const uint32_t* c = (const uint32_t*)codes;
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == NERFX_TYPE_F32) hipLaunchKernelGGL(mx4_dequantize_kernel<NERFX_TYPE_F32>, grid, dim3(256), 0, s, c, scales, rows, k, whole, out);
-    else if (dtype == NERFX_TYPE_BF16) hipLaunchKernelGGL(mx4_dequantize_kernel<NERFX_TYPE_BF16>, grid, dim3(256), 0, s, c, scales, rows, k, whole, out);
-    else hipLaunchKernelGGL(mx4_dequantize_kernel<NERFX_TYPE_F16>, grid, dim3(256), 0, s, c, scales, rows, k, whole, out);
-    return launch_status("mx4_dequantize_kernel");
+    const int64_t parts = rows * mx4_blocks(k) * 4;
+    const int how = mx4_rows(out, k, dtype);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)codes, scales, parts, k, how, out);
+        return launch_status("mx4_dequantize_kernel");
+    };
+    return dtype == NERFX_TYPE_F32 ? go(mx4_dequantize_kernel<NERFX_TYPE_F32>)
+         : dtype == NERFX_TYPE_BF16 ? go(mx4_dequantize_kernel<NERFX_TYPE_BF16>) : go(mx4_dequantize_kernel<NERFX_TYPE_F16>);
 }
 
 static bool mx4_type(int dtype) { return float_type(dtype) || dtype == NERFX_TYPE_MX4; }

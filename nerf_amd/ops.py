@@ -747,6 +747,10 @@ def _stream_on(dev):
     return _stream() if _RAW_STREAM is None else _RAW_STREAM(dev.index)
 
 
+def _at(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 def _ns_schedule(coefficients, steps: int):
     """One (a, b, c) for all steps, or one for each -> the C array of 3 * steps floats."""
     if not 1 <= steps <= 32:
@@ -805,12 +809,12 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
             raise RuntimeError("orthogonalize is not differentiable: pass detached matrices or call it under no_grad")
     srcs = [t.contiguous() for t in listed]
     stacked = torch.empty(mats.shape, device=dev, dtype=mats.dtype) if isinstance(mats, Tensor) else None
-    outs = [torch.empty(t.shape, device=dev, dtype=t.dtype) for t in srcs] if stacked is None else \
+    outs = [torch.empty_like(t) for t in srcs] if stacked is None else \
         list(stacked.unbind(0)) if stacked.dim() == 3 else [stacked]
     table = _matrix_table([(s.data_ptr(), o.data_ptr(), 0, 0, *s.shape) for s, o in zip(srcs, outs)])
     ws, need = _ns_workspace(table, len(srcs), dev)
     with _on(dev):
-        check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[dtype], schedule, steps, eps, _p(ws), need, _stream_on(dev)))
+        check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[dtype], schedule, steps, eps, _at(ws), need, _stream_on(dev)))
     return outs if stacked is None else stacked
 
 
@@ -859,7 +863,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     ws, need = _ns_workspace(table, len(params), dev)
     with _on(dev):
         check(lib.nerfx_muon_step(table, len(params), lr, momentum, int(nesterov), weight_decay, _LR_RULES[adjust_lr], schedule,
-                                  steps, eps, _p(grad_scale), _p(found_inf), _p(ws), need, _stream_on(dev)))
+                                  steps, eps, _at(grad_scale), _at(found_inf), _at(ws), need, _stream_on(dev)))
     for t in params + momenta:                              # written through raw pointers: tell autograd
         torch.autograd.graph.increment_version(t)           # and the packed-weight cache of ModelHandle
 
@@ -887,6 +891,16 @@ class Mx4:
             raise ValueError("Mx4: codes must be aligned to 16 bytes")
         self.codes, self.scales, self.k = codes, scales, k
 
+    @classmethod
+    def _new(cls, rows: int, k: int, dev) -> "Mx4":
+        """An unwritten one."""
+        self = object.__new__(cls)
+        blocks = (k + 31) // 32
+        self.codes = torch.empty((rows, 16 * blocks), device=dev, dtype=torch.uint8)
+        self.scales = torch.empty((rows, blocks), device=dev, dtype=torch.uint8)
+        self.k = k
+        return self
+
     @property
     def shape(self) -> Tuple[int, int]:
         return self.codes.shape[0], self.k
@@ -911,10 +925,12 @@ class Mx4:
             raise TypeError(f"dequantize gives fp32, bf16 or fp16 (asked for {dtype})")
         if not self.codes.is_cuda:
             raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {self.codes.device}")
-        out = torch.empty(self.shape, device=self.device, dtype=dtype)
-        with _on(self.device):
-            check(lib.nerfx_mx4_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.k, _TYPES[dtype], _p(out),
-                                           _stream_on(self.device)))
+        codes, dev = self.codes, self.codes.device
+        rows = codes.shape[0]
+        out = torch.empty((rows, self.k), device=dev, dtype=dtype)
+        with _on(dev):
+            check(lib.nerfx_mx4_dequantize(codes.data_ptr(), self.scales.data_ptr(), rows, self.k, _TYPES[dtype], out.data_ptr(),
+                                           _stream_on(dev)))
         return out
 
 
@@ -939,12 +955,12 @@ def mx4_quantize(x: Tensor) -> Mx4:
     if x.dim() != 2:
         raise ValueError(f"mx4_quantize takes a matrix (got shape {tuple(x.shape)})")
     rows, k = x.shape
-    blocks = (k + 31) // 32
-    codes = torch.empty((rows, 16 * blocks), device=x.device, dtype=torch.uint8)
-    scales = torch.empty((rows, blocks), device=x.device, dtype=torch.uint8)
-    with _on(x.device):
-        check(lib.nerfx_mx4_quantize(_p(x), _TYPES[x.dtype], rows, k, _p(codes), _p(scales), _stream_on(x.device)))
-    return Mx4(codes, scales, k)
+    dev = x.device
+    out = Mx4._new(rows, k, dev)
+    with _on(dev):
+        check(lib.nerfx_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, out.codes.data_ptr(), out.scales.data_ptr(),
+                                     _stream_on(dev)))
+    return out
 
 
 def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Optional[str] = None, out_dtype=None):
@@ -982,8 +998,7 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
     for s in lead:
         m *= s
     if out_dtype == "mx4":
-        out = Mx4(torch.empty((m, 16 * ((n + 31) // 32)), device=dev, dtype=torch.uint8),
-                  torch.empty((m, (n + 31) // 32), device=dev, dtype=torch.uint8), n)
+        out = Mx4._new(m, n, dev)
         y, y_scales, yt = out.codes, out.scales, _lib.TYPE_MX4
     else:
         out_dtype = default if out_dtype is None else out_dtype
@@ -994,8 +1009,8 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
     need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt, yt)
     ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
     with _on(dev):
-        check(lib.nerfx_mx4_linear(_p(src), dt, _p(scales), m, k, _p(weight.codes), _p(weight.scales), n, _p(bias),
-                                   _LINEAR_ACTS[activation], _p(y), yt, _p(y_scales), _p(ws), max(need, 0), _stream_on(dev)))
+        check(lib.nerfx_mx4_linear(src.data_ptr(), dt, _at(scales), m, k, weight.codes.data_ptr(), weight.scales.data_ptr(), n, _at(bias),
+                                   _LINEAR_ACTS[activation], y.data_ptr(), yt, _at(y_scales), _at(ws), max(need, 0), _stream_on(dev)))
     return out
 
 
