@@ -134,83 +134,113 @@ __device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
     else if (activ == NERFX_ACT_SILU) each([](float x) { return mx4_activate(x, NERFX_ACT_SILU); });
 }
 
-// y for the 32 x 32 accumulator (bias included) of rows n0 .. of W and rows m0 .. of x: a lane holds row m = m0 + lane % 32
-// and, with h = lane / 32, columns n0 + 8 q + 4 h + i in element 4 q + i.
-__device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, const float16_t_& acc, int64_t m0, int n0) {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    const int64_t m = m0 + (lane & 31);
-    float v[16];
+// y from 32 x 32 accumulators (bias included) of rows m0 .. of x and, tile after tile, of neighbouring columns.  A lane holds row
+// m0 + lane % 32 and, with h = lane / 32, columns n0 + 8 q + 4 h + i of it in element 4 q + i: written from there, a store would
+// touch 32 rows with 32 bytes each.  So a wave collects 128 bytes of each of its rows in LDS (one tile of fp32, two of 16 bits,
+// eight of blocks) and writes them as lines (524,288 x 256 by 256 x 256, bf16: 138 -> 114 us).  Rows lie 144 bytes apart there: a phase's
+// sixteen on different banks.  Where y's rows are not whole 16-byte pieces every value is stored by itself.
+struct Mx4Lines {
+    static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
+    char* lds;
+    int begin = 0, end = 0;                                    // bytes of y's rows that are collected
+
+    __device__ __forceinline__ void add(const Mx4LinearArgs& a, const float16_t_& acc, int64_t m0, int n0) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const int64_t m = m0 + (lane & 31);
+        float v[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = acc[e];
-    mx4_activate16(v, a.activ);
-    if (a.y_dtype == NERFX_TYPE_MX4) {                         // the tile's 32 columns are a block of y
-        using Raw = Mx4Raw<NERFX_TYPE_F32, 16>;
-        Raw raw;
+        for (int e = 0; e < 16; ++e) v[e] = acc[e];
+        mx4_activate16(v, a.activ);
+        char* row = lds + (lane & 31) * PITCH;
+        if (a.y_dtype == NERFX_TYPE_MX4) {                     // the tile's 32 columns are a block of y
+            using Raw = Mx4Raw<NERFX_TYPE_F32, 16>;
+            Raw raw;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) raw.w[e] = n0 + 8 * (e >> 2) + 4 * h + (e & 3) < a.n ? __builtin_bit_cast(uint32_t, v[e]) : 0u;
-        uint32_t top = raw.top_bits();
-        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        const uint32_t byte = Raw::scale_byte(max(both[0], both[1]));
-        const float scale = Raw::scale_value(byte);
-        // this lane's codes are the lower (h = 0) or upper halves of the block's four words: after the exchange the lower lane
-        // has all of the first two, the upper lane of the other two
-        const auto half = __builtin_amdgcn_permlane32_swap(raw.codes(0, scale), raw.codes(1, scale), false, false);
-        u32x2_t w = {__builtin_amdgcn_perm(half[1], half[0], 0x05040100u), __builtin_amdgcn_perm(half[1], half[0], 0x07060302u)};
-        if (byte == 255u) w = {0, 0};
-        if (m >= a.m) return;
-        const int64_t block = m * mx4_blocks(a.n) + n0 / MX4_BLOCK;
-        *(u32x2_t*)((char*)a.y + block * MX4_BLOCK_BYTES + 8 * h) = w;
-        if (h == 0) a.y_scales[block] = (uint8_t)byte;
-        return;
-    }
-    if (a.y_dtype == NERFX_TYPE_F32) {
-        if (m >= a.m) return;
-        float* y = (float*)a.y + m * a.n;
+            for (int e = 0; e < 16; ++e) raw.w[e] = n0 + 8 * (e >> 2) + 4 * h + (e & 3) < a.n ? __builtin_bit_cast(uint32_t, v[e]) : 0u;
+            uint32_t top = raw.top_bits();
+            const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            const uint32_t byte = Raw::scale_byte(max(both[0], both[1]));
+            const float scale = Raw::scale_value(byte);
+            // this lane's codes are the lower (h = 0) or upper halves of the block's four words: after the exchange the lower
+            // lane has all of the first two, the upper lane of the other two
+            const auto half = __builtin_amdgcn_permlane32_swap(raw.codes(0, scale), raw.codes(1, scale), false, false);
+            u32x2_t w = {__builtin_amdgcn_perm(half[1], half[0], 0x05040100u), __builtin_amdgcn_perm(half[1], half[0], 0x07060302u)};
+            if (byte == 255u) w = {0, 0};
+            if (h == 0 && m < a.m) a.y_scales[m * mx4_blocks(a.n) + n0 / MX4_BLOCK] = (uint8_t)byte;
+            open(n0 / 2);
+            *(u32x2_t*)(row + n0 / 2 - begin + 8 * h) = w;
+            close(a, m0, n0 / 2 + 16, mx4_blocks(a.n) * 16);
+        } else if (a.y_dtype == NERFX_TYPE_F32) {
+            if (!a.y_whole) {
+                float* y = (float*)a.y + m * a.n;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = n0 + 8 * q + 4 * h;
-            if (a.y_whole) {
-                if (n < a.n) *(u32x4_t*)(y + n) = __builtin_bit_cast(u32x4_t, (float __attribute__((ext_vector_type(4)))){v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]});
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n + i < a.n) y[n + i] = v[4 * q + i];
+                for (int e = 0; e < 16; ++e) {
+                    const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    if (m < a.m && n < a.n) y[n] = v[e];
+                }
+                return;
             }
+            open(4 * n0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(f32x4_t*)(row + 32 * q + 16 * h) = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            close(a, m0, 4 * n0 + 128, 4 * a.n);
+        } else {
+            // two 16-bit values a word; word 2 q + p holds columns 8 q + 4 h + 2 p, + 1
+            uint32_t w[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (bf16x2_t){(__bf16)v[2 * p], (__bf16)v[2 * p + 1]});
+            if (a.y_dtype == NERFX_TYPE_F16) {
+#pragma unroll
+                for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (f16x2_t){(_Float16)v[2 * p], (_Float16)v[2 * p + 1]});
+            }
+            if (!a.y_whole) {
+                uint16_t* y = (uint16_t*)a.y + m * a.n;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    if (m < a.m && n < a.n) y[n] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                }
+                return;
+            }
+            // exchange halves between lanes l and l + 32, so that one lane has 16 columns in a row: the lower lane
+            // q = 0, 1 (columns 0 .. 15), the upper one q = 2, 3
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const auto r = __builtin_amdgcn_permlane32_swap(w[p], w[p + 4], false, false);
+                w[p] = r[0];
+                w[p + 4] = r[1];
+            }
+            open(2 * n0);
+            *(u32x4_t*)(row + 2 * n0 - begin + 32 * h) = {w[0], w[1], w[4], w[5]};
+            *(u32x4_t*)(row + 2 * n0 - begin + 32 * h + 16) = {w[2], w[3], w[6], w[7]};
+            close(a, m0, 2 * n0 + 64, 2 * a.n);
         }
-        return;
     }
-    // two 16-bit values a word; word 2 q + p holds columns 8 q + 4 h + 2 p, + 1
-    uint32_t w[8];
-#pragma unroll
-    for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (bf16x2_t){(__bf16)v[2 * p], (__bf16)v[2 * p + 1]});
-    if (a.y_dtype == NERFX_TYPE_F16) {
-#pragma unroll
-        for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (f16x2_t){(_Float16)v[2 * p], (_Float16)v[2 * p + 1]});
+
+private:
+    __device__ __forceinline__ void open(int at) { if (end == 0) begin = at; }
+    // Bytes up to `to` are there: out with them, if they make lines or the rows (of row_bytes) end.
+    __device__ __forceinline__ void close(const Mx4LinearArgs& a, int64_t m0, int to, int row_bytes) {
+        end = to;
+        if (to - begin == 128 || to >= row_bytes) flush(a, m0, row_bytes);
     }
-    if (!a.y_whole) {
-        if (m >= a.m) return;
-        uint16_t* y = (uint16_t*)a.y + m * a.n;
+
+public:
+    // Also needed behind the last tile of some columns, where they end in the middle of a row's line.
+    __device__ __forceinline__ void flush(const Mx4LinearArgs& a, int64_t m0, int row_bytes) {
+        const int lane = threadIdx.x & 63, at = begin + 16 * (lane & 7);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (n < a.n) y[n] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 3);
+            const u32x4_t v = *(const u32x4_t*)(lds + r * PITCH + 16 * (lane & 7));
+            if (m0 + r < a.m && at < min(end, row_bytes)) *(u32x4_t*)((char*)a.y + (m0 + r) * row_bytes + at) = v;
         }
-        return;
+        end = 0;
     }
-    // exchange halves between lanes l and l + 32, so that one lane has 16 columns in a row: the lower lane
-    // q = 0, 1 (columns 0 .. 15), the upper one q = 2, 3
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        const auto r = __builtin_amdgcn_permlane32_swap(w[p], w[p + 4], false, false);
-        w[p] = r[0];
-        w[p + 4] = r[1];
+    __device__ __forceinline__ void rest(const Mx4LinearArgs& a, int64_t m0) {
+        if (end) flush(a, m0, a.y_dtype == NERFX_TYPE_MX4 ? mx4_blocks(a.n) * 16 : a.n * (a.y_dtype == NERFX_TYPE_F32 ? 4 : 2));
     }
-    if (m >= a.m) return;
-    uint16_t* y = (uint16_t*)a.y + m * a.n;
-    const int n = n0 + 16 * h;
-    if (n < a.n) *(u32x4_t*)(y + n) = {w[0], w[1], w[4], w[5]};
-    if (n + 8 < a.n) *(u32x4_t*)(y + n + 8) = {w[2], w[3], w[6], w[7]};
-}
+};
 
 // A (32 FP WP) x (32 FQ WQ) tile of W x^T per workgroup of WP x WQ waves.  A stage is eight blocks (256 values) of every
 // row of both operands, 128 bytes a row, brought by LDS-DMA while the stage before is worked on; block c of row r lies
@@ -383,9 +413,11 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
             multiply(f1, S3{});
         }
     }
-    // row by row of y: the runs of one row that neighbouring tiles write follow each other
+    __syncthreads();                                           // the stages have been read: their place is the waves' own now
+    Mx4Lines lines{lds + wave * Mx4Lines::BYTES};
+    static_assert(T::WAVES * Mx4Lines::BYTES <= T::SCALES_AT, "the bias is still needed");
 #pragma unroll
-    for (int j = 0; j < FQ; ++j)
+    for (int j = 0; j < FQ; ++j) {
 #pragma unroll
         for (int i = 0; i < FP; ++i) {
             const int n = n0 + wp + 32 * i;
@@ -396,8 +428,10 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += b[e];
             }
-            mx4_store(a, acc[i][j], m0 + wq + 32 * j, n);
+            lines.add(a, acc[i][j], m0 + wq + 32 * j, n);
         }
+        lines.rest(a, m0 + wq + 32 * j);
+    }
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------
@@ -540,7 +574,7 @@ constexpr int STREAM_WAVES = 8, STREAM_ROWS = 32 * STREAM_WAVES;
 __host__ __device__ inline int stream_row_bytes(int ks) { return (2 * ks + 1) * 16; }
 __host__ __device__ inline int stream_scale_bytes(int ks) { return ks > 4 ? 16 : 8; }      // both halves of a row
 __host__ __device__ inline int stream_lds(int ks, int columns) {
-    return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4);
+    return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4) + STREAM_WAVES * Mx4Lines::BYTES;
 }
 
 template <int DT, int KS>
@@ -551,6 +585,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
     const int nb = mx4_blocks(a.k), c0 = blockIdx.y * columns;
     char* scale_lds = lds + columns * stream_row_bytes(KS);
     float* bias_lds = (float*)(scale_lds + columns * stream_scale_bytes(KS));
+    char* line_lds = (char*)(bias_lds + columns) + wave * Mx4Lines::BYTES;
     for (int c = threadIdx.x; c < columns; c += 64 * STREAM_WAVES) bias_lds[c] = a.bias && c0 + c < a.n ? a.bias[c0 + c] : 0.f;
     for (int c = threadIdx.x; c < columns * 2 * KS; c += 64 * STREAM_WAVES) {
         const int r = c / (2 * KS), b = c - r * 2 * KS;
@@ -600,7 +635,8 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
                 if (KS > AT_ONCE) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        for (int n = 0; n < columns; n += 32) {
+        Mx4Lines lines{line_lds};
+        for (int n = 0; n < columns && c0 + n < a.n; n += 32) {
             const int r = n + (lane & 31);
             const char* wr = lds + r * stream_row_bytes(KS) + h * 16;
             uint32_t ws[SB / 4];
@@ -618,8 +654,9 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
                                                                       4, 4, s & 3, (int)ws[s / 4 < SB / 4 ? s / 4 : 0], s & 3, (int)xs[s / 4 < (KS + 3) / 4 ? s / 4 : 0]);
             NERFX_STEP(0) NERFX_STEP(1) NERFX_STEP(2) NERFX_STEP(3) NERFX_STEP(4) NERFX_STEP(5) NERFX_STEP(6) NERFX_STEP(7)
 #undef NERFX_STEP
-            mx4_store(a, acc, m0, c0 + n);
+            lines.add(a, acc, m0, c0 + n);
         }
+        lines.rest(a, m0);
     }
 }
 
