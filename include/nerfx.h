@@ -371,7 +371,9 @@ typedef struct {
  * `dtype` (NERFX_TYPE_*) of grad and out.  A zero matrix gives zeros; a matrix with an infinity or
  * a NaN gives NaN.  `mats` is a host array; all matrices share the launches.  Coefficients
  * that would let a singular value grow beyond 64 are refused.  `workspace`:
- * nerfx_orthogonalize_workspace_bytes(mats, count) bytes, aligned to 16; it holds nothing between calls. */
+ * nerfx_orthogonalize_workspace_bytes(mats, count) bytes (0 for groups of matrices of up to 64 x 256), aligned to 16;
+ * it holds nothing between calls.  The first call on a device opts kernels into their LDS sizes: make it outside of
+ * graph capture. */
 int64_t nerfx_orthogonalize_workspace_bytes(const nerfx_matrix_t* mats /* host */, int count);
 int nerfx_orthogonalize(const nerfx_matrix_t* mats /* host */, int count, int dtype,
                         const float* coefficients /* host */, int steps, float eps,
@@ -398,7 +400,7 @@ int nerfx_mx4_quantize(const void* x, int dtype, int64_t rows, int k, uint8_t* c
 int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k, int dtype, void* out,
                          void* stream);
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
- * x_scales its scales; NULL otherwise), W (n, k) as codes and scales, bias (n) fp32 or NULL, sums in fp32,
+ * x_scales its scales; NULL otherwise), W (n, k) as codes and scales (n <= 2^24), bias (n) fp32 or NULL, sums in fp32,
  * activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as above along n, y its codes and
  * y_scales its scales; NULL otherwise).  x, the weight's codes and y's codes aligned to 16 bytes.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */

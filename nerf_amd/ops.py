@@ -855,6 +855,9 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     spans.sort()
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise RuntimeError("muon_step: two of `params` and `momenta` share memory")
+    held = {m.data_ptr() for m in momenta if m.numel()}
+    if any(g.data_ptr() in held for g in grads):
+        raise RuntimeError("muon_step: a gradient is one of the `momenta`, which are written first")
     for name, t in (("grad_scale", grad_scale), ("found_inf", found_inf)):
         if t is not None and not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.numel() == 1):
             raise RuntimeError(f"muon_step: `{name}` must be one fp32 element on {dev}")

@@ -202,7 +202,7 @@ def test_muon_step(ops, nesterov, decay, rule):
 def test_muon_step_refuses(ops):
     w, g, m = (matrix((8, 6), i) for i in range(3))
     big = matrix((16, 6), 3)
-    for args in (([w], [g], [w]), ([w], [g], [m.half()]), ([w], [g.t()], [m]), ([w], [g[0]], [m]), ([w.t()], [g.t()], [m.t().contiguous()]),
+    for args in (([w], [g], [w]), ([w], [m], [m]), ([w], [g], [m.half()]), ([w], [g.t()], [m]), ([w], [g[0]], [m]), ([w.t()], [g.t()], [m.t().contiguous()]),
                  ([w, w], [g, g], [m, m.clone()]), ([big[:8], big[4:12]], [g, g], [m, m.clone()]), ([w.cpu()], [g], [m])):
         before = [t.clone() for t in (w, m, big)]
         with pytest.raises(RuntimeError):

@@ -46,7 +46,8 @@ def test_c_refusals():
         return lib.nerfx_mx4_linear(x, xt, xs, m, k, w, ws, n, None, act, y, yt, ys, work, size, None)
 
     refused(linear(m=-1), b"rows")
-    refused(linear(n=-1), b"rows")
+    refused(linear(n=-1), b"n -1")
+    refused(linear(n=(1 << 24) + 1), b"n 16777217")
     refused(linear(k=0), b"k 0")
     refused(linear(xt=4), b"of x")
     refused(linear(yt=4), b"of y")
