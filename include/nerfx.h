@@ -402,7 +402,7 @@ int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
  * x_scales its scales; NULL otherwise), W (n, k) as codes and scales (n <= 2^24), bias (n) fp32 or NULL, sums in fp32,
  * activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as above along n, y its codes and
- * y_scales its scales; NULL otherwise).  x, the weight's codes and y's codes aligned to 16 bytes.
+ * y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
 int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,

@@ -10,47 +10,68 @@
 namespace nerfx {
 
 // ---- to and from -----------------------------------------------------------------------------------------------------
-// Four lanes make a block, eight values each: every load and store of a wave is one run of memory.  Bound by memory (524,288 x
-// 256 bf16: 5.4 TB/s to, 5.4 TB/s from), as long as nothing but the conversion instructions touches the values: where rows are
-// whole blocks the matrix is one run (MX4_FULL), and no division finds the row.
-enum { MX4_VALUES, MX4_PIECES, MX4_FULL };     // rows value by value; whole 16-byte pieces, aligned; whole blocks as well
+// Four lanes make a block, eight values each: every load and store of a wave is one run of memory, 16 bytes a lane wherever the
+// row begins (the memory pipes take any address; value by value an odd row length cost eight times the time).  Bound by memory
+// (524,288 x 256 bf16: 5.4 TB/s to, 5.4 TB/s from), as long as nothing but the conversion instructions touches the values: where
+// rows are whole blocks the matrix is one run, and no division finds the row.
 
-// Value eight of part `q` begins at `at` of `row`; its place in memory is row * k + at.
-__device__ __forceinline__ int64_t mx4_place(uint64_t q, int k, int how, int& at) {
-    if (how == MX4_FULL) { at = 0; return (int64_t)q * 8; }    // at: only compared with k, and every part is whole
+// Part `q`, eight values, begins at `at` of its row; -> its place in memory, row * k + at.  RUN: k is a multiple of 32, every part
+// is whole and the row is of no interest.
+template <bool RUN>
+__device__ __forceinline__ int64_t mx4_place(uint64_t q, int k, int& at) {
+    at = 0;
+    if constexpr (RUN) return (int64_t)q * 8;
     const uint32_t nb = mx4_blocks(k);
     const uint64_t block = q >> 2, row = block >> 32 ? block / nb : (uint32_t)block / nb;
     at = (int)(block - row * nb) * MX4_BLOCK + (int)(q & 3) * 8;
     return (int64_t)row * k + at;
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t parts, int k, int how,
+// N values (a multiple of 8, at most 32) from `row + at` on: all there, or zeros behind k.
+template <int DT, int N>
+__device__ __forceinline__ Mx4Raw<DT, N> mx4_load_whole(const char* row, int at) {
+    Mx4Raw<DT, N> v;
+#pragma unroll
+    for (int i = 0; i < Mx4Raw<DT, N>::WORDS / 4; ++i) {
+        const u32x4_t w = *(const u32x4_any_t*)(row + (int64_t)at * (DT == NERFX_TYPE_F32 ? 4 : 2) + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.w[4 * i + j] = w[j];
+    }
+    return v;
+}
+
+template <int DT, int N>
+__device__ __forceinline__ Mx4Raw<DT, N> mx4_load(const char* row, int at, int k) {
+    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
+    Mx4Raw<DT, N> v;
+    if (at + N <= k) {
+        v = mx4_load_whole<DT, N>(row, at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Mx4Raw<DT, N>::WORDS; ++i) {
+            if constexpr (SIZE == 4) {
+                v.w[i] = at + i < k ? *(const uint32_t*)(row + (int64_t)(at + i) * 4) : 0u;
+            } else {
+                const uint32_t lo = at + 2 * i < k ? *(const uint16_t*)(row + (int64_t)(at + 2 * i) * 2) : 0u;
+                const uint32_t hi = at + 2 * i + 1 < k ? *(const uint16_t*)(row + (int64_t)(at + 2 * i + 1) * 2) : 0u;
+                v.w[i] = lo | hi << 16;
+            }
+        }
+    }
+    return v;
+}
+
+template <int DT, bool RUN>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t parts, int k,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     using Raw = Mx4Raw<DT, 8>;
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
         int at;
-        const char* src = (const char*)x + mx4_place(q, k, how, at) * SIZE;
+        const int64_t place = mx4_place<RUN>(q, k, at);
         Raw v;
-        if (how != MX4_VALUES && at + 8 <= k) {
-#pragma unroll
-            for (int i = 0; i < Raw::WORDS / 4; ++i) {
-                const u32x4_t p = *(const u32x4_t*)(src + 16 * i);
-                v.w[4 * i] = p[0]; v.w[4 * i + 1] = p[1]; v.w[4 * i + 2] = p[2]; v.w[4 * i + 3] = p[3];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < Raw::WORDS; ++i) {
-                if constexpr (DT == NERFX_TYPE_F32) {
-                    v.w[i] = at + i < k ? *(const uint32_t*)(src + 4 * i) : 0u;
-                } else {
-                    const uint32_t lo = at + 2 * i < k ? *(const uint16_t*)(src + 4 * i) : 0u;
-                    const uint32_t hi = at + 2 * i + 1 < k ? *(const uint16_t*)(src + 4 * i + 2) : 0u;
-                    v.w[i] = lo | hi << 16;
-                }
-            }
-        }
+        if constexpr (RUN) v = mx4_load_whole<DT, 8>((const char*)x + place * SIZE, 0);
+        else v = mx4_load<DT, 8>((const char*)x + (place - at) * SIZE, at, k);
         uint32_t top = v.top_bits();
         top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
         top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
@@ -60,14 +81,14 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restric
     }
 }
 
-template <int DT>
+template <int DT, bool RUN>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                             int64_t parts, int k, int how, void* __restrict__ out) {
+                                                             int64_t parts, int k, void* __restrict__ out) {
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
         int at;
-        char* dst = (char*)out + mx4_place(q, k, how, at) * SIZE;
-        if (at >= k) continue;
+        char* dst = (char*)out + mx4_place<RUN>(q, k, at) * SIZE;
+        if (!RUN && at >= k) continue;
         const uint32_t c = codes[q], byte = scales[q >> 2];
         const float scale = Mx4Raw<DT, 8>::scale_value(byte);
         uint32_t w[8 * SIZE / 4];
@@ -87,10 +108,13 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
 #pragma unroll
             for (int i = 0; i < 2 * SIZE; ++i) w[i] = DT == NERFX_TYPE_F32 ? 0x7fc00000u : DT == NERFX_TYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
         }
-        if (how != MX4_VALUES && at + 8 <= k) {
+        if (RUN || at + 8 <= k) {
 #pragma unroll
-            for (int i = 0; i < SIZE / 2; ++i)
-                __builtin_nontemporal_store((u32x4_t){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]}, (u32x4_t*)(dst + 16 * i));
+            for (int i = 0; i < SIZE / 2; ++i) {
+                const u32x4_any_t piece = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+                if constexpr (RUN) __builtin_nontemporal_store(piece, (u32x4_any_t*)(dst + 16 * i));
+                else *(u32x4_any_t*)(dst + 16 * i) = piece;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -109,7 +133,7 @@ struct Mx4LinearArgs {
     void* y;
     uint8_t* y_scales;
     int64_t m;
-    int32_t n, k, activ, y_dtype, y_whole;     // y_whole: 16-byte stores are possible
+    int32_t n, k, activ, y_dtype;
 };
 
 __device__ __forceinline__ float mx4_activate(float v, int activ) {
@@ -138,7 +162,7 @@ __device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
 // m0 + lane % 32 and, with h = lane / 32, columns n0 + 8 q + 4 h + i of it in element 4 q + i: written from there, a store would
 // touch 32 rows with 32 bytes each.  So a wave collects 128 bytes of each of its rows in LDS (one tile of fp32, two of 16 bits,
 // eight of blocks) and writes them as lines (524,288 x 256 by 256 x 256, bf16: 138 -> 114 us).  Rows lie 144 bytes apart there: a phase's
-// sixteen on different banks.  Where y's rows are not whole 16-byte pieces every value is stored by itself.
+// sixteen on different banks.
 struct Mx4Lines {
     static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
     char* lds;
@@ -171,15 +195,6 @@ struct Mx4Lines {
             *(u32x2_t*)(row + n0 / 2 - begin + 8 * h) = w;
             close(a, m0, n0 / 2 + 16, mx4_blocks(a.n) * 16);
         } else if (a.y_dtype == NERFX_TYPE_F32) {
-            if (!a.y_whole) {
-                float* y = (float*)a.y + m * a.n;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    if (m < a.m && n < a.n) y[n] = v[e];
-                }
-                return;
-            }
             open(4 * n0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) *(f32x4_t*)(row + 32 * q + 16 * h) = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
@@ -192,15 +207,6 @@ struct Mx4Lines {
             if (a.y_dtype == NERFX_TYPE_F16) {
 #pragma unroll
                 for (int p = 0; p < 8; ++p) w[p] = __builtin_bit_cast(uint32_t, (f16x2_t){(_Float16)v[2 * p], (_Float16)v[2 * p + 1]});
-            }
-            if (!a.y_whole) {
-                uint16_t* y = (uint16_t*)a.y + m * a.n;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    if (m < a.m && n < a.n) y[n] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                }
-                return;
             }
             // exchange halves between lanes l and l + 32, so that one lane has 16 columns in a row: the lower lane
             // q = 0, 1 (columns 0 .. 15), the upper one q = 2, 3
@@ -229,11 +235,15 @@ public:
     // Also needed behind the last tile of some columns, where they end in the middle of a row's line.
     __device__ __forceinline__ void flush(const Mx4LinearArgs& a, int64_t m0, int row_bytes) {
         const int lane = threadIdx.x & 63, at = begin + 16 * (lane & 7);
+        const int there = min(end, row_bytes) - at;            // bytes of this lane's piece
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = 8 * i + (lane >> 3);
-            const u32x4_t v = *(const u32x4_t*)(lds + r * PITCH + 16 * (lane & 7));
-            if (m0 + r < a.m && at < min(end, row_bytes)) *(u32x4_t*)((char*)a.y + (m0 + r) * row_bytes + at) = v;
+            const char* piece = lds + r * PITCH + 16 * (lane & 7);
+            char* y = (char*)a.y + (m0 + r) * row_bytes + at;
+            if (m0 + r >= a.m) continue;
+            if (there >= 16) *(u32x4_any_t*)y = *(const u32x4_t*)piece;
+            else for (int c = 0; c < there; c += 2) *(uint16_t*)(y + c) = *(const uint16_t*)(piece + c);
         }
         end = 0;
     }
@@ -441,39 +451,6 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 // loads of W are on their way.
 constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024;
 
-// One block of x, 32 values: whole blocks from aligned memory (MX4_FULL), whole pieces of 16 bytes from aligned memory
-// (MX4_PIECES), or value by value; zeros behind k.
-template <int DT>
-__device__ __forceinline__ Mx4Raw<DT, 32> mx4_load_block(const char* row, int at, int k, int how) {
-    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, PIECE = 16 / SIZE;
-    Mx4Raw<DT, 32> v;
-    if (how == MX4_FULL) {
-#pragma unroll
-        for (int i = 0; i < 32 / PIECE; ++i) {
-            const u32x4_t p = *(const u32x4_t*)(row + (at + i * PIECE) * SIZE);
-            v.w[4 * i] = p[0]; v.w[4 * i + 1] = p[1]; v.w[4 * i + 2] = p[2]; v.w[4 * i + 3] = p[3];
-        }
-    } else if (how == MX4_PIECES) {
-#pragma unroll
-        for (int i = 0; i < 32 / PIECE; ++i) {
-            u32x4_t p = {0, 0, 0, 0};
-            if (at + i * PIECE < k) p = *(const u32x4_t*)(row + (at + i * PIECE) * SIZE);
-            v.w[4 * i] = p[0]; v.w[4 * i + 1] = p[1]; v.w[4 * i + 2] = p[2]; v.w[4 * i + 3] = p[3];
-        }
-    } else if constexpr (SIZE == 4) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v.w[i] = at + i < k ? *(const uint32_t*)(row + (at + i) * 4) : 0u;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t lo = at + 2 * i < k ? *(const uint16_t*)(row + (at + 2 * i) * 2) : 0u;
-            const uint32_t hi = at + 2 * i + 1 < k ? *(const uint16_t*)(row + (at + 2 * i + 1) * 2) : 0u;
-            v.w[i] = lo | hi << 16;
-        }
-    }
-    return v;
-}
-
 __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
     const float v = mx4_activate(acc + (a.bias ? a.bias[n] : 0.f), a.activ);
     const int64_t at = m * a.n + n;
@@ -483,7 +460,7 @@ __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m,
 }
 
 template <int DT, int MT>
-__global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4LinearArgs a, int how) {
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4LinearArgs a) {
     extern __shared__ __align__(16) char lds[];
     constexpr bool FLOAT = DT != NERFX_TYPE_MX4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
@@ -507,7 +484,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4
         using Raw = Mx4Raw<DT, 32>;
         for (int q = threadIdx.x; q < m * nb; q += 64 * SKINNY_WAVES) {
             const int r = q / nb, b = q - r * nb;
-            const Raw v = mx4_load_block<DT>((const char*)a.x + (int64_t)r * a.k * (DT == NERFX_TYPE_F32 ? 4 : 2), b * 32, a.k, how);
+            const Raw v = mx4_load<DT, 32>((const char*)a.x + (int64_t)r * a.k * (DT == NERFX_TYPE_F32 ? 4 : 2), b * 32, a.k);
             const uint32_t byte = Raw::scale_byte(v.top_bits());
             const float scale = Raw::scale_value(byte);
             *(u32x4_t*)(lds + q * 16) = {v.codes(0, scale), v.codes(1, scale), v.codes(2, scale), v.codes(3, scale)};
@@ -617,22 +594,41 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
         } else {
             using Raw = Mx4Raw<DT, 32>;
             constexpr int AT_ONCE = DT == NERFX_TYPE_F32 ? 2 : 4;          // as many loads in flight as registers allow
+            const char* row = (const char*)a.x + m * a.k * SIZE;
+            const int whole = a.k / MX4_BLOCK;                             // blocks
+            auto take = [&](const Raw& raw, int s) {
+                const uint32_t byte = Raw::scale_byte(raw.top_bits());
+                const float scale = Raw::scale_value(byte);
+                xc[s] = {raw.codes(0, scale), raw.codes(1, scale), raw.codes(2, scale), raw.codes(3, scale)};
+                xs[s / 4] |= byte << (8 * (s & 3));
+            };
+            if (whole > 0) {
 #pragma unroll
-            for (int s0 = 0; s0 < KS; s0 += AT_ONCE) {
-                Raw raw[AT_ONCE];
+                for (int s0 = 0; s0 < KS; s0 += AT_ONCE) {
+                    Raw raw[AT_ONCE];
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u)
-                    if (s0 + u < KS) raw[u] = mx4_load_block<DT>((const char*)a.x + m * a.k * SIZE, (2 * (s0 + u) + h) * 32, a.k, MX4_FULL);
+                    for (int u = 0; u < AT_ONCE; ++u)                      // behind the row's last whole block: that one again
+                        if (s0 + u < KS) raw[u] = mx4_load_whole<DT, 32>(row, min(2 * (s0 + u) + h, whole - 1) * MX4_BLOCK);
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u) {
-                    if (s0 + u >= KS) break;
-                    const int s = s0 + u;
-                    const uint32_t byte = Raw::scale_byte(raw[u].top_bits());
-                    const float scale = Raw::scale_value(byte);
-                    xc[s] = {raw[u].codes(0, scale), raw[u].codes(1, scale), raw[u].codes(2, scale), raw[u].codes(3, scale)};
-                    xs[s / 4] |= byte << (8 * (s & 3));
+                    for (int u = 0; u < AT_ONCE; ++u) {
+                        if (s0 + u < KS) take(raw[u], s0 + u);
+                    }
+                    if (KS > AT_ONCE) __builtin_amdgcn_sched_barrier(0);
                 }
-                if (KS > AT_ONCE) __builtin_amdgcn_sched_barrier(0);
+            }
+            if (nb != 2 * KS || whole != nb) {                             // rows that end earlier: a part of a block, and zeros
+                Raw tail = mx4_load<DT, 32>(row, whole * MX4_BLOCK, a.k);
+                const uint32_t byte = Raw::scale_byte(tail.top_bits());
+                const float scale = Raw::scale_value(byte);
+                const u32x4_t codes = {tail.codes(0, scale), tail.codes(1, scale), tail.codes(2, scale), tail.codes(3, scale)};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int b = 2 * s + h;
+                    if (b < whole) continue;
+                    const bool part = b == whole && whole < nb;
+                    xc[s] = part ? codes : (u32x4_t){0, 0, 0, 0};
+                    xs[s / 4] = (xs[s / 4] & ~(255u << (8 * (s & 3)))) | (part ? byte : 127u) << (8 * (s & 3));
+                }
             }
         }
         Mx4Lines lines{line_lds};
@@ -663,22 +659,20 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
 // ---- host side -------------------------------------------------------------------------------------------------------
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// How the rows of a matrix in a float type can be read or written: see the kernels.
-static int mx4_rows(const void* p, int k, int dtype) {
-    if (!aligned16(p) || k % (dtype == NERFX_TYPE_F32 ? 4 : 8) != 0) return MX4_VALUES;
-    return k % MX4_BLOCK == 0 ? MX4_FULL : MX4_PIECES;
-}
 static dim3 mx4_grid(int64_t parts) { return dim3((unsigned)std::min<int64_t>((parts + 255) / 256, 256 * 32)); }
 
 static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_t* codes, uint8_t* scales, hipStream_t stream) {
     const int64_t parts = rows * mx4_blocks(k) * 4;
-    const int how = mx4_rows(x, k, dtype);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, stream, x, parts, k, how, (uint32_t*)codes, scales);
+        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, stream, x, parts, k, (uint32_t*)codes, scales);
         return launch_status("mx4_quantize_kernel");
     };
-    return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32>)
-         : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16>) : go(mx4_quantize_kernel<NERFX_TYPE_F16>);
+    if (k % MX4_BLOCK == 0) {
+        return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32, true>)
+             : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, true>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, true>);
+    }
+    return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32, false>)
+         : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, false>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, false>);
 }
 
 template <int FP, int WP, int FQ, int WQ>
@@ -695,8 +689,7 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes (else by way of the workspace): W is read once, by
 //          as many workgroups as it has 16 rows (one row by 4096 x 4096: 62 us with tiles).  Not for a result in blocks, which
 //          are of 32 columns;
-//  stream  otherwise up to 256 columns and 512 values a row: float rows of 64, 128, 192, 256, 320 or 512 values are quantised in
-//          registers, others into the workspace first;
+//  stream  otherwise up to 256 columns and 512 values a row: float rows are quantised in registers;
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.
 enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
 // Steps of 64 values that a row is worked on in: what the stream kernel is made for.
@@ -708,10 +701,7 @@ static int mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype, bool& sta
     const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
     stage = false;
     if (!blocks_out && m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
-    if (n <= 256 && k <= 512 && (blocks_out || m > SKINNY_ROWS)) {
-        stage = is_float && k != 64 * stream_steps(k);
-        return MX4_STREAM;
-    }
+    if (n <= 256 && k <= 512 && (blocks_out || m > SKINNY_ROWS)) return MX4_STREAM;
     stage = is_float;
     return !blocks_out && m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
 }
@@ -721,11 +711,10 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     const int mt = (int)(a.m + 15) / 16, nb = mx4_blocks(a.k);
     const size_t codes = DT == NERFX_TYPE_MX4 ? 0 : (size_t)a.m * nb * 17, sums = (size_t)SKINNY_WAVES * mt * 1024;
     const size_t lds = std::max(codes, sums);
-    const int how = mx4_rows(a.x, a.k, DT);
     const dim3 grid((unsigned)((a.n + 15) / 16)), block(64 * SKINNY_WAVES);
     auto go = [&](auto kernel) {
         NERFX_OPT_IN_LDS(kernel, lds);
-        hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, how);
+        hipLaunchKernelGGL(kernel, grid, block, lds, stream, a);
         return launch_status("mx4_skinny_kernel");
     };
     switch (mt) {
@@ -787,13 +776,16 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
     NERFX_REQUIRE(codes && scales && out, "codes / scales / out is NULL");
     NERFX_REQUIRE(((uintptr_t)codes & 3) == 0, "codes are not aligned to 4 bytes");
     const int64_t parts = rows * mx4_blocks(k) * 4;
-    const int how = mx4_rows(out, k, dtype);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)codes, scales, parts, k, how, out);
+        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)codes, scales, parts, k, out);
         return launch_status("mx4_dequantize_kernel");
     };
-    return dtype == NERFX_TYPE_F32 ? go(mx4_dequantize_kernel<NERFX_TYPE_F32>)
-         : dtype == NERFX_TYPE_BF16 ? go(mx4_dequantize_kernel<NERFX_TYPE_BF16>) : go(mx4_dequantize_kernel<NERFX_TYPE_F16>);
+    if (k % MX4_BLOCK == 0) {
+        return dtype == NERFX_TYPE_F32 ? go(mx4_dequantize_kernel<NERFX_TYPE_F32, true>)
+             : dtype == NERFX_TYPE_BF16 ? go(mx4_dequantize_kernel<NERFX_TYPE_BF16, true>) : go(mx4_dequantize_kernel<NERFX_TYPE_F16, true>);
+    }
+    return dtype == NERFX_TYPE_F32 ? go(mx4_dequantize_kernel<NERFX_TYPE_F32, false>)
+         : dtype == NERFX_TYPE_BF16 ? go(mx4_dequantize_kernel<NERFX_TYPE_BF16, false>) : go(mx4_dequantize_kernel<NERFX_TYPE_F16, false>);
 }
 
 static bool mx4_type(int dtype) { return float_type(dtype) || dtype == NERFX_TYPE_MX4; }
@@ -818,14 +810,13 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
     NERFX_REQUIRE(x && w_codes && w_scales && y && (x_dtype != NERFX_TYPE_MX4 || x_scales) && (y_dtype != NERFX_TYPE_MX4 || y_scales),
                   "a required pointer is NULL");
     NERFX_REQUIRE(y_dtype != NERFX_TYPE_MX4 || aligned16(y), "y's codes are not aligned to 16 bytes");
-    NERFX_REQUIRE(aligned16(w_codes) && aligned16(x), "x or the weight's codes are not aligned to 16 bytes");
+    NERFX_REQUIRE(aligned16(w_codes) && (x_dtype != NERFX_TYPE_MX4 || aligned16(x)), "codes are not aligned to 16 bytes");
     const int64_t need = nerfx_mx4_linear_workspace_bytes(m, n, k, x_dtype, y_dtype);
     NERFX_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
                   "workspace NULL, not aligned to 16 bytes, or of %lld bytes with %lld needed", (long long)workspace_bytes, (long long)need);
     Mx4LinearArgs a{};
     a.w = w_codes; a.w_scales = w_scales; a.bias = bias; a.y = y; a.y_scales = y_scales;
     a.m = m; a.n = n; a.k = k; a.activ = activ; a.y_dtype = y_dtype;
-    a.y_whole = aligned16(y) && n % (y_dtype == NERFX_TYPE_F32 ? 4 : 8) == 0;
     a.x = (const uint8_t*)x; a.x_scales = x_scales;
     const hipStream_t st = (hipStream_t)stream;
     bool stage;

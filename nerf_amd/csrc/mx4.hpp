@@ -24,6 +24,9 @@ typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
+// Sixteen bytes of a row of floats, which begins wherever it begins.
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
 // N consecutive values of one block in one lane, as they are in memory (16-bit types two to a word).
 template <int DT, int N>
 struct Mx4Raw {

@@ -984,8 +984,6 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
         width, default = x.k, torch.float32
     else:
         src = _mx4_input(x, "x")
-        if src.data_ptr() % 16:
-            src = src.clone()
         lead, dt, scales, dev, width, default = src.shape[:-1], _TYPES[src.dtype], None, src.device, src.shape[-1], src.dtype
     if width != k:
         raise ValueError(f"x has {width} columns, weight {k}")

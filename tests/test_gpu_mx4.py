@@ -256,6 +256,32 @@ def test_linear_writes_nothing_beside_its_result(ops):
         assert torch.equal(y.view(m, n), ops.mx4_linear(x, qw, bias, "relu"))
 
 
+@pytest.mark.parametrize("m,n,k", [(7, 37, 43), (90, 37, 43), (90, 3, 31), (200, 301, 333), (90, 65, 96)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_from_and_to_any_place(ops, dtype, m, n, k):
+    """x amid NaNs and y amid other numbers, each from any value of a buffer on: nothing from beside x counts, nothing beside y changes."""
+    import ctypes as C
+    from nerf_amd import _lib
+    x, w, bias = pair(m, n, k, dtype, 7)
+    qw = ops.mx4_quantize(w)
+    code = TYPES.index(dtype)
+    p = lambda t: C.c_void_p(t.data_ptr())
+    need = _lib.lib.nerfx_mx4_linear_workspace_bytes(m, n, k, code, code)
+    ws = torch.empty(max(need, 16), device="cuda", dtype=torch.uint8)
+    want = check_linear(ops, x, w, bias, None)
+    for at in range(9):
+        src = torch.full((m * k + 64,), float("nan"), device="cuda", dtype=dtype)
+        buf = torch.full((m * n + 64,), 3.0, device="cuda", dtype=dtype)
+        src[at:at + m * k] = x.flatten()
+        y = buf[8 - at:8 - at + m * n]
+        _lib.check(_lib.lib.nerfx_mx4_linear(p(src[at:]), code, None, m, k, p(qw.codes), p(qw.scales), n, p(bias), -1, p(y), code, None, p(ws),
+                                             need, C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        assert torch.equal(y.view(m, n), want), at
+        assert bool((buf[:8 - at] == 3).all()) and bool((buf[8 - at + m * n:] == 3).all()), at
+        q = ops.mx4_quantize(src[at:at + m * k].view(m, k))
+        assert torch.equal(q.scales, ops.mx4_quantize(x).scales) and torch.equal(q.codes, ops.mx4_quantize(x).codes), at
+
+
 def test_linear_refuses(ops):
     x, w, bias = pair(4, 8, 64, torch.float32, 6)
     qw = ops.mx4_quantize(w)

@@ -20,7 +20,7 @@ def test_workspace_bytes():
     assert size(-1, 4, 4, 0, 0) == size(4, -1, 4, 0, 0) == size(4, 4, 0, 0, 0) == size(4, 4, (1 << 20) + 1, 0, 0) == -1
     assert size(4, 4, 4, 9, 0) == size(4, 4, 4, 0, 9) == size(1 << 31, 4, 4, 0, 0) == -1
     assert size(524288, 256, 256, _lib.TYPE_BF16, _lib.TYPE_BF16) == 0          # quantised in registers
-    assert size(524288, 256, 295, _lib.TYPE_BF16, _lib.TYPE_MX4) >= 524288 * 10 * 17
+    assert size(524288, 300, 295, _lib.TYPE_BF16, _lib.TYPE_MX4) >= 524288 * 10 * 17
 
 
 def test_c_refusals():
@@ -53,8 +53,9 @@ def test_c_refusals():
     refused(linear(yt=4), b"of y")
     refused(linear(yt=3), b"NULL")                                     # codes without scales
     refused(linear(yt=3, ys=p, y=p + 8), b"aligned")
-    refused(linear(m=100, k=65, size=0), b"workspace")
-    refused(linear(m=100, k=65, work=None), b"workspace")
+    refused(linear(m=100, n=300, size=0), b"workspace")
+    refused(linear(m=100, n=300, work=None), b"workspace")
+    refused(linear(m=100, n=300, work=p + 8), b"workspace")
     refused(linear(act=3), b"activation")
     refused(linear(act=-2), b"activation")
     for name in ("x", "w", "ws", "y"):
