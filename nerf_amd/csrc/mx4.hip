@@ -253,22 +253,28 @@ public:
 };
 
 // A (32 FP WP) x (32 FQ WQ) tile of W x^T per workgroup of WP x WQ waves.  A stage is eight blocks (256 values) of every
-// row of both operands, 128 bytes a row, brought by LDS-DMA while the stage before is worked on; block c of row r lies
+// row of both operands, 128 bytes a row, brought by LDS-DMA while the S - 1 stages before are worked on; block c of row r lies
 // at place c ^ (r / 2 % 8), so that the sixteen rows of a read phase touch different banks.  The scales, a byte a block, come
-// sixteen a row, two stages' worth, by way of registers: read in smaller pieces they would be most of the requests;
-// fragments are read one step (64 values) ahead of their use.  Rows behind
-// the last one and blocks behind a row's end are read from the last ones: the results of the former are not stored, the codes of
-// the latter are cleared on one side.
-template <int FP, int WP, int FQ, int WQ>
+// sixteen a row, two stages' worth, by way of registers: read in smaller pieces they would be most of the requests.  With more
+// than two stages (DEEP) they are all in LDS before the first product, since the wait for a register is one for every load sent
+// out before it.  Fragments are read one step (64 values) ahead of their use.  Rows behind the last one and blocks behind a row's
+// end are read from the last ones: the results of the former are not stored, the codes of the latter are cleared on one side.
+// Bound by LDS: a stage of a 64 x 64 tile writes 16 KB and reads 32, at some 64 bytes a clock, and takes 0.37 us; more stages, or
+// reads of a whole stage ahead, change nothing.
+template <int FP, int WP, int FQ, int WQ, int S>
 struct Mx4Tile {
-    static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ, STAGES = 2;
+    static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ, STAGES = S;
+    static constexpr bool DEEP = S > 2;
     static constexpr int STAGE_BLOCKS = 8, ROW_BYTES = STAGE_BLOCKS * MX4_BLOCK_BYTES;
     static constexpr int STAGE_BYTES = (TP + TQ) * ROW_BYTES;
-    // behind the stages: two chunks of scales, 16 bytes a row each, and the bias
-    static constexpr int SCALES_AT = STAGES * STAGE_BYTES, CHUNK_BYTES = (TP + TQ) * 16, BIAS_AT = SCALES_AT + 2 * CHUNK_BYTES;
-    static constexpr int LDS_BYTES = BIAS_AT + 4 * TP, CHUNK_ROWS = (TP + TQ) / (64 * WAVES);
+    // behind the stages: the bias, and the scales, two chunks of 16 bytes a row or (DEEP) whole rows
+    static constexpr int BIAS_AT = STAGES * STAGE_BYTES, SCALES_AT = BIAS_AT + 4 * TP, CHUNK_BYTES = (TP + TQ) * 16;
+    static constexpr int CHUNK_ROWS = DEEP ? 1 : (TP + TQ) / (64 * WAVES);
     static constexpr int LOADS_P = TP / (8 * WAVES), LOADS_Q = TQ / (8 * WAVES);
-    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && WAVES % 2 == 0 && (TP + TQ) % (64 * WAVES) == 0 && LDS_BYTES <= 160 * 1024, "whole loads per wave");
+    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && WAVES % 2 == 0 && (DEEP || (TP + TQ) % (64 * WAVES) == 0), "whole loads per wave");
+    // Whole rows of scales lie an odd number of 8 bytes apart: a phase's reads on different banks.
+    static __host__ __device__ int scale_pitch(int nb) { return 8 * ((nb + 7) / 8 | 1); }
+    static __host__ __device__ int lds_bytes(int nb) { return SCALES_AT + (DEEP ? (TP + TQ) * scale_pitch(nb) : 2 * CHUNK_BYTES); }
 
     struct Frags { u32x4_t p[FP], q[FQ]; };
     // step s of the stage in `buf`
@@ -292,15 +298,15 @@ struct Mx4Tile {
         return v;
     }
     // From a chunk in LDS: those of blocks 2 s + h of stage st, one a byte.
-    static __device__ __forceinline__ uint32_t scales(const char* chunks, int row, int st, int h) {
-        const u32x2_t v = *(const u32x2_t*)(chunks + (st >> 1 & 1) * CHUNK_BYTES + row * 16 + (st & 1) * 8);
+    static __device__ __forceinline__ uint32_t scales(const char* chunks, int row, int st, int h, int pitch) {
+        const u32x2_t v = *(const u32x2_t*)(chunks + (DEEP ? row * pitch + st * 8 : (st >> 1 & 1) * CHUNK_BYTES + row * 16 + (st & 1) * 8));
         return __builtin_amdgcn_perm(v[1], v[0], h ? 0x07050301u : 0x06040200u);
     }
 };
 
-template <int FP, int WP, int FQ, int WQ>
+template <int FP, int WP, int FQ, int WQ, int S>
 __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearArgs a) {
-    using T = Mx4Tile<FP, WP, FQ, WQ>;
+    using T = Mx4Tile<FP, WP, FQ, WQ, S>;
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int nb = mx4_blocks(a.k), stages = (nb + 7) / 8;
@@ -327,13 +333,14 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
         for (int i = 0; i < T::LOADS_Q; ++i) dma16(to + T::TP * T::ROW_BYTES + i * T::WAVES * 1024, Q, q_at[i] + block);
     };
     // this thread's rows of a chunk of scales
+    const int scale_pitch = T::scale_pitch(nb);
     const uint8_t* scale_row[T::CHUNK_ROWS];
     u32x4_t chunk[T::CHUNK_ROWS];
+    auto scales_of = [&](int r) {
+        return r < T::TP ? a.w_scales + (int64_t)(n0 + min(r, p_last)) * nb : a.x_scales + (m0 + min(r - T::TP, q_last)) * nb;
+    };
 #pragma unroll
-    for (int i = 0; i < T::CHUNK_ROWS; ++i) {
-        const int r = threadIdx.x + 64 * T::WAVES * i;
-        scale_row[i] = r < T::TP ? a.w_scales + (int64_t)(n0 + min(r, p_last)) * nb : a.x_scales + (m0 + min(r - T::TP, q_last)) * nb;
-    }
+    for (int i = 0; i < T::CHUNK_ROWS; ++i) scale_row[i] = scales_of(threadIdx.x + 64 * T::WAVES * i);
     auto fetch_chunk = [&](int c) {
 #pragma unroll
         for (int i = 0; i < T::CHUNK_ROWS; ++i) chunk[i] = T::chunk(scale_row[i], c, nb);
@@ -347,9 +354,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     uint32_t sp[FP], sq[FQ];
     auto take_scales = [&](int st) {
 #pragma unroll
-        for (int i = 0; i < FP; ++i) sp[i] = T::scales(lds + T::SCALES_AT, p_row + 32 * i, st, h);
+        for (int i = 0; i < FP; ++i) sp[i] = T::scales(lds + T::SCALES_AT, p_row + 32 * i, st, h, scale_pitch);
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) sq[j] = T::scales(lds + T::SCALES_AT, q_row + 32 * j, st, h);
+        for (int j = 0; j < FQ; ++j) sq[j] = T::scales(lds + T::SCALES_AT, q_row + 32 * j, st, h, scale_pitch);
     };
     float16_t_ acc[FP][FQ];
 #pragma unroll
@@ -372,16 +379,29 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     typename T::Frags f0, f1;
     float* bias_lds = (float*)(lds + T::BIAS_AT);
     for (int c = threadIdx.x; c < T::TP; c += 64 * T::WAVES) bias_lds[c] = a.bias && c <= p_last ? a.bias[n0 + c] : 0.f;
-    fetch_chunk(0);
-    store_chunk(0);
-    fetch(0);
-    landed<0>();
-    if (stages > 1) fetch(1);
+    if constexpr (T::DEEP) {
+        for (int st = 0; st < min(S, stages); ++st) fetch(st);
+        const int pieces = (nb + 15) / 16;
+        for (int c = threadIdx.x; c < (T::TP + T::TQ) * pieces; c += 64 * T::WAVES) {
+            const int r = c / pieces, at = c - r * pieces;
+            const u32x4_t v = T::chunk(scales_of(r), at, nb);
+            u32x2_t* to = (u32x2_t*)(lds + T::SCALES_AT + r * scale_pitch + 16 * at);
+            to[0] = (u32x2_t){v[0], v[1]};
+            if (16 * at + 8 < scale_pitch) to[1] = (u32x2_t){v[2], v[3]};
+        }
+        landed<0>();
+    } else {
+        fetch_chunk(0);
+        store_chunk(0);
+        fetch(0);
+        landed<0>();
+        if (stages > 1) fetch(1);
+    }
     take_scales(0);
     T::read(f0, lds, 0, p_row, q_row, h);
     for (int st = 0; st < stages - 1; ++st) {
         const char* buf = lds + (st % T::STAGES) * T::STAGE_BYTES;
-        const bool new_chunk = (st & 1) && st + 1 < stages;    // the next stage begins a chunk
+        const bool new_chunk = !T::DEEP && (st & 1) && st + 1 < stages; // the next stage begins a chunk
         if (new_chunk) fetch_chunk((st + 1) >> 1);
         __builtin_amdgcn_sched_barrier(0);                     // on its way for the whole stage
         T::read(f1, buf, 1, p_row, q_row, h);
@@ -393,8 +413,10 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
         // The compiler does not know of the loads into LDS and waits for its own as if they were the only ones: the chunk has
         // to be put away before the next of those are sent out, or it would wait for them all.
         if (new_chunk) store_chunk((st + 1) >> 1);
-        landed<0>();                                           // the next stage is there, and every wave has read all of this one
-        if (st + 2 < stages) fetch(st + 2);
+        // the next stage is there, and every wave has read all of this one
+        if (T::DEEP && st + S <= stages) landed<(S - 2) * (T::LOADS_P + T::LOADS_Q)>();
+        else landed<0>();
+        if (st + S < stages) fetch(st + S);
         T::read(f0, lds + ((st + 1) % T::STAGES) * T::STAGE_BYTES, 0, p_row, q_row, h);
         multiply(f1, S3{});
         take_scales(st + 1);
@@ -425,7 +447,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     }
     __syncthreads();                                           // the stages have been read: their place is the waves' own now
     Mx4Lines lines{lds + wave * Mx4Lines::BYTES};
-    static_assert(T::WAVES * Mx4Lines::BYTES <= T::SCALES_AT, "the bias is still needed");
+    static_assert(T::WAVES * Mx4Lines::BYTES <= T::BIAS_AT, "the bias is still needed");
 #pragma unroll
     for (int j = 0; j < FQ; ++j) {
 #pragma unroll
@@ -675,13 +697,14 @@ static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_
          : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, false>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, false>);
 }
 
-template <int FP, int WP, int FQ, int WQ>
+template <int FP, int WP, int FQ, int WQ, int S>
 static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
-    using T = Mx4Tile<FP, WP, FQ, WQ>;
+    using T = Mx4Tile<FP, WP, FQ, WQ, S>;
     const int64_t tiles = ((a.n + T::TP - 1) / T::TP) * ((a.m + T::TQ - 1) / T::TQ);
     NERFX_REQUIRE(tiles <= 1 << 22, "%lld x %d results are too many for one launch", (long long)a.m, a.n);
-    NERFX_OPT_IN_LDS((mx4_tile_kernel<FP, WP, FQ, WQ>), T::LDS_BYTES);
-    hipLaunchKernelGGL((mx4_tile_kernel<FP, WP, FQ, WQ>), dim3((unsigned)tiles), dim3(64 * T::WAVES), T::LDS_BYTES, stream, a);
+    const int lds = T::lds_bytes(mx4_blocks(a.k));
+    NERFX_OPT_IN_LDS((mx4_tile_kernel<FP, WP, FQ, WQ, S>), lds);
+    hipLaunchKernelGGL((mx4_tile_kernel<FP, WP, FQ, WQ, S>), dim3((unsigned)tiles), dim3(64 * T::WAVES), lds, stream, a);
     return launch_status("mx4_tile_kernel");
 }
 
@@ -689,8 +712,12 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes (else by way of the workspace): W is read once, by
 //          as many workgroups as it has 16 rows (one row by 4096 x 4096: 62 us with tiles).  Not for a result in blocks, which
 //          are of 32 columns;
-//  stream  otherwise up to 256 columns and 512 values a row: float rows are quantised in registers;
-//  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.
+//  stream  otherwise up to 256 values a row, or 512 and up to 256 columns: float rows are quantised in registers, once for every
+//          256 columns (16,384 x 4096 by 128: 40 us, 54 with tiles; by 512: 82, and 69 with tiles);
+//  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
+//          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit) and a row's scales fit: a
+//          small product lasts as long as one tile does (256 x 4096 by 4096: 12 us, 21 with 128 x 128; 1024 x 4096 by 4096, 1024
+//          tiles: 28 and 27); else 128 x 128.
 enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
 // Steps of 64 values that a row is worked on in: what the stream kernel is made for.
 static int stream_steps(int k) {
@@ -701,7 +728,7 @@ static int mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype, bool& sta
     const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
     stage = false;
     if (!blocks_out && m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
-    if (n <= 256 && k <= 512 && (blocks_out || m > SKINNY_ROWS)) return MX4_STREAM;
+    if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20 && (blocks_out || m > SKINNY_ROWS)) return MX4_STREAM;
     stage = is_float;
     return !blocks_out && m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
 }
@@ -728,9 +755,10 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 template <int DT>
 static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     const int64_t row_tiles = (a.m + STREAM_ROWS - 1) / STREAM_ROWS;
-    // few rows: the columns are spread over workgroups until the device is full
+    // up to 256 columns in LDS at a time; few rows: the columns are spread over workgroups until the device is full
     const int tiles = (a.n + 31) / 32;
-    const int per = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, row_tiles * tiles / 256));
+    const int groups = (int)std::min<int64_t>(tiles, std::max<int64_t>((tiles + 7) / 8, 256 / row_tiles));
+    const int per = (tiles + groups - 1) / groups;
     const int columns = 32 * per;
     const dim3 grid((unsigned)std::min<int64_t>(row_tiles, 512), (unsigned)((tiles + per - 1) / per)), block(64 * STREAM_WAVES);
     auto go = [&](auto kernel, int ks) {
@@ -829,8 +857,9 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
         x_dtype = NERFX_TYPE_MX4;
     }
     if (plan == MX4_TILE) {
-        const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-        return big >= 192 ? tile_launch<4, 2, 2, 4>(a, st) : tile_launch<2, 2, 2, 2>(a, st);
+        const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256), small = ((a.m + 63) / 64) * ((a.n + 63) / 64);
+        if (small <= 512 && Mx4Tile<1, 2, 1, 2, 3>::lds_bytes(mx4_blocks(k)) <= 160 * 1024) return tile_launch<1, 2, 1, 2, 3>(a, st);
+        return big >= 192 ? tile_launch<4, 2, 2, 4, 2>(a, st) : tile_launch<2, 2, 2, 2, 2>(a, st);
     }
     auto by_type = [&](auto skinny, auto str) { return plan == MX4_SKINNY ? skinny(a, st) : str(a, st); };
     switch (x_dtype) {

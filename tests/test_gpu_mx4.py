@@ -162,6 +162,15 @@ def test_linear(ops, dtype, m, n, k):
         check_linear(ops, x, w, bias, act, what=f"{m} x {n} x {k} {act}")
 
 
+# Columns in several groups; tiles of each size, with rows of one stage and more, and too long for their scales to be in LDS.
+@pytest.mark.parametrize("m,n,k", [(70, 300, 200), (300, 1000, 256), (5000, 520, 33), (600, 2100, 64), (20000, 257, 256), (70, 100, 30000),
+                                   (100, 70, 8200), (65, 65, 513), (2100, 1600, 300), (1700, 2500, 1100), (2100, 1600, 520), (6200, 2050, 290),
+                                   (5000, 3000, 700), (12300, 1030, 545)])
+def test_linear_many_columns_and_tiles(ops, m, n, k):
+    x, w, bias = pair(m, n, k, torch.bfloat16, 8)
+    check_linear(ops, x, w, bias, "relu", what=f"{m} x {n} by {k}")
+
+
 @pytest.mark.parametrize("act", [None, "relu", "leaky_relu", "silu"])
 @pytest.mark.parametrize("m,n,k", [(5, 96, 64), (300, 256, 256), (700, 640, 416)])
 def test_linear_activations_and_types(ops, m, n, k, act):
@@ -183,7 +192,7 @@ def test_linear_of_a_quantized_input(ops, m, n, k):
 
 @pytest.mark.parametrize("act", [None, "relu", "silu"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (3, 40, 39), (64, 256, 256), (129, 256, 295), (300, 31, 96), (300, 256, 256), (500, 300, 64),
-                                   (515, 700, 1032), (200, 64, 600)])
+                                   (33, 600, 200), (2100, 1600, 300), (515, 700, 1032), (200, 64, 600)])
 def test_linear_into_blocks(ops, m, n, k, act):
     """A result quantised on its way out is the fp32 result, which the same product gives, quantised."""
     for dtype in TYPES:

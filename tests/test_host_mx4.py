@@ -53,9 +53,9 @@ def test_c_refusals():
     refused(linear(yt=4), b"of y")
     refused(linear(yt=3), b"NULL")                                     # codes without scales
     refused(linear(yt=3, ys=p, y=p + 8), b"aligned")
-    refused(linear(m=100, n=300, size=0), b"workspace")
-    refused(linear(m=100, n=300, work=None), b"workspace")
-    refused(linear(m=100, n=300, work=p + 8), b"workspace")
+    refused(linear(m=100, n=300, k=600, size=0), b"workspace")
+    refused(linear(m=100, n=300, k=600, work=None), b"workspace")
+    refused(linear(m=100, n=300, k=600, work=p + 8), b"workspace")
     refused(linear(act=3), b"activation")
     refused(linear(act=-2), b"activation")
     for name in ("x", "w", "ws", "y"):
