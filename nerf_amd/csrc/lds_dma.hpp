@@ -13,6 +13,10 @@ __device__ __forceinline__ uint32_t lds_address(const char* lds) {
 __device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t offset) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
+// The same from an address of each lane's own.
+__device__ __forceinline__ void dma16(uint32_t lds, const char* from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
 // All but the newest N of this wave's loads are done, and so are its LDS reads: then, behind the barrier, so are every wave's.
 template <int N>
 __device__ __forceinline__ void landed() {

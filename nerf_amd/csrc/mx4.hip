@@ -61,24 +61,29 @@ __device__ __forceinline__ Mx4Raw<DT, N> mx4_load(const char* row, int at, int k
     return v;
 }
 
+// Part q's codes are stored, `scale(byte)` stores its block's scale.
+template <int DT, bool RUN, class Scale>
+__device__ __forceinline__ void mx4_quantize_part(const void* x, int64_t q, int k, uint32_t* codes, Scale scale) {
+    using Raw = Mx4Raw<DT, 8>;
+    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
+    int at;
+    const int64_t place = mx4_place<RUN>(q, k, at);
+    Raw v;
+    if constexpr (RUN) v = mx4_load_whole<DT, 8>((const char*)x + place * SIZE, 0);
+    else v = mx4_load<DT, 8>((const char*)x + (place - at) * SIZE, at, k);
+    uint32_t top = v.top_bits();
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+    const uint32_t byte = Raw::scale_byte(top);
+    codes[q] = byte == 255u ? 0u : v.codes(0, Raw::scale_value(byte));
+    if ((q & 3) == 0) scale((uint8_t)byte);
+}
+
 template <int DT, bool RUN>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t parts, int k,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    using Raw = Mx4Raw<DT, 8>;
-    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
-        int at;
-        const int64_t place = mx4_place<RUN>(q, k, at);
-        Raw v;
-        if constexpr (RUN) v = mx4_load_whole<DT, 8>((const char*)x + place * SIZE, 0);
-        else v = mx4_load<DT, 8>((const char*)x + (place - at) * SIZE, at, k);
-        uint32_t top = v.top_bits();
-        top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
-        const uint32_t byte = Raw::scale_byte(top);
-        codes[q] = byte == 255u ? 0u : v.codes(0, Raw::scale_value(byte));
-        if ((q & 3) == 0) scales[q >> 2] = (uint8_t)byte;
-    }
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256)
+        mx4_quantize_part<DT, RUN>(x, q, k, codes, [&](uint8_t byte) { scales[q >> 2] = byte; });
 }
 
 template <int DT, bool RUN>
@@ -252,29 +257,80 @@ public:
     }
 };
 
+// Scales in the order in which tiles need them: of eight blocks at a time, all rows.  Behind a row's end 127, a number.
+constexpr int MX4_STAGE = 8;                                   // blocks
+__host__ __device__ inline int mx4_stages(int nb) { return (nb + MX4_STAGE - 1) / MX4_STAGE; }
+__host__ __device__ inline int64_t mx4_ordered_bytes(int64_t rows) { return (rows + 1) / 2 * 2 * MX4_STAGE; }    // of one stage
+
+__device__ __forceinline__ void mx4_order_scales(const uint8_t* __restrict__ from, int64_t rows, int nb, uint8_t* __restrict__ to,
+                                                 int64_t first, int64_t step) {
+    const int stages = mx4_stages(nb);
+    for (int64_t i = first; i < rows * stages; i += step) {
+        const int64_t row = i / stages;
+        const int st = (int)(i - row * stages), there = nb - st * MX4_STAGE;
+        const uint8_t* src = from + row * nb + st * MX4_STAGE;
+        u32x2_t v = {0x7f7f7f7fu, 0x7f7f7f7fu};
+        if (there >= MX4_STAGE) {
+            __builtin_memcpy(&v, src, 8);
+        } else {
+#pragma unroll
+            for (int b = 0; b < MX4_STAGE; ++b)
+                if (b < there) v[b / 4] = (v[b / 4] & ~(255u << (8 * (b % 4)))) | (uint32_t)src[b] << (8 * (b % 4));
+        }
+        *(u32x2_t*)(to + st * mx4_ordered_bytes(rows) + row * MX4_STAGE) = v;
+    }
+}
+
+// What a product in tiles needs beforehand, in one launch: the first `w_groups` workgroups order W's scales, the others quantise x
+// with its scales in order (or, if x is quantised, order those).
+struct Mx4PrepareArgs {
+    const void* x;
+    const uint8_t *x_scales, *w_scales;
+    uint32_t* codes;
+    uint8_t *x_ordered, *w_ordered;
+    int64_t m;
+    int32_t n, k, w_groups;
+};
+template <int DT, bool RUN>
+__global__ __launch_bounds__(256) void mx4_prepare_kernel(const Mx4PrepareArgs a) {
+    const int nb = mx4_blocks(a.k);
+    if ((int)blockIdx.x < a.w_groups) {
+        mx4_order_scales(a.w_scales, a.n, nb, a.w_ordered, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)a.w_groups * 256);
+        return;
+    }
+    const int64_t first = (int64_t)(blockIdx.x - a.w_groups) * 256 + threadIdx.x, step = (int64_t)(gridDim.x - a.w_groups) * 256;
+    if constexpr (DT == NERFX_TYPE_MX4) {
+        mx4_order_scales(a.x_scales, a.m, nb, a.x_ordered, first, step);
+    } else {
+        const int64_t parts = a.m * nb * 4, stage_bytes = mx4_ordered_bytes(a.m);
+        for (int64_t q = first; q < parts; q += step)
+            mx4_quantize_part<DT, RUN>(a.x, q, a.k, a.codes, [&](uint8_t byte) {
+                const uint64_t block = (uint64_t)q >> 2, row = block >> 32 ? block / nb : (uint32_t)block / nb;
+                const int b = (int)(block - row * nb);
+                uint8_t* to = a.x_ordered + b / MX4_STAGE * stage_bytes + row * MX4_STAGE;
+                to[b % MX4_STAGE] = byte;
+                if (b == nb - 1)
+                    for (int i = b % MX4_STAGE + 1; i < MX4_STAGE; ++i) to[i] = 127;
+            });
+    }
+}
+
 // A (32 FP WP) x (32 FQ WQ) tile of W x^T per workgroup of WP x WQ waves.  A stage is eight blocks (256 values) of every
 // row of both operands, 128 bytes a row, brought by LDS-DMA while the S - 1 stages before are worked on; block c of row r lies
-// at place c ^ (r / 2 % 8), so that the sixteen rows of a read phase touch different banks.  The scales, a byte a block, come
-// sixteen a row, two stages' worth, by way of registers: read in smaller pieces they would be most of the requests.  With more
-// than two stages (DEEP) they are all in LDS before the first product, since the wait for a register is one for every load sent
-// out before it.  Fragments are read one step (64 values) ahead of their use.  Rows behind the last one and blocks behind a row's
-// end are read from the last ones: the results of the former are not stored, the codes of the latter are cleared on one side.
-// Bound by LDS: a stage of a 64 x 64 tile writes 16 KB and reads 32, at some 64 bytes a clock, and takes 0.37 us; more stages, or
-// reads of a whole stage ahead, change nothing.
+// at place c ^ (r / 2 % 8), so that the sixteen rows of a read phase touch different banks.  The stage's scales, eight bytes a row,
+// come the same way, from scales put in order beforehand: as they are given every row's few bytes are a request of their own
+// (4096 x 4096 by 8192, x in blocks: 93 us by way of registers, 85 so, 3 of them for the order).  Fragments are read one step (64
+// values) ahead of their use.  Rows behind the last one and blocks behind a row's end are read from the last ones: the results of
+// the former are not stored, the codes of the latter are cleared on one side.
 template <int FP, int WP, int FQ, int WQ, int S>
 struct Mx4Tile {
     static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ, STAGES = S;
-    static constexpr bool DEEP = S > 2;
-    static constexpr int STAGE_BLOCKS = 8, ROW_BYTES = STAGE_BLOCKS * MX4_BLOCK_BYTES;
-    static constexpr int STAGE_BYTES = (TP + TQ) * ROW_BYTES;
-    // behind the stages: the bias, and the scales, two chunks of 16 bytes a row or (DEEP) whole rows
-    static constexpr int BIAS_AT = STAGES * STAGE_BYTES, SCALES_AT = BIAS_AT + 4 * TP, CHUNK_BYTES = (TP + TQ) * 16;
-    static constexpr int CHUNK_ROWS = DEEP ? 1 : (TP + TQ) / (64 * WAVES);
-    static constexpr int LOADS_P = TP / (8 * WAVES), LOADS_Q = TQ / (8 * WAVES);
-    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && WAVES % 2 == 0 && (DEEP || (TP + TQ) % (64 * WAVES) == 0), "whole loads per wave");
-    // Whole rows of scales lie an odd number of 8 bytes apart: a phase's reads on different banks.
-    static __host__ __device__ int scale_pitch(int nb) { return 8 * ((nb + 7) / 8 | 1); }
-    static __host__ __device__ int lds_bytes(int nb) { return SCALES_AT + (DEEP ? (TP + TQ) * scale_pitch(nb) : 2 * CHUNK_BYTES); }
+    static constexpr int ROW_BYTES = MX4_STAGE * MX4_BLOCK_BYTES, STAGE_BYTES = (TP + TQ) * ROW_BYTES, SCALE_BYTES = (TP + TQ) * MX4_STAGE;
+    static constexpr int SCALES_AT = STAGES * STAGE_BYTES, BIAS_AT = SCALES_AT + STAGES * SCALE_BYTES, LDS_BYTES = BIAS_AT + 4 * TP;
+    static constexpr int LOADS_P = TP / (8 * WAVES), LOADS_Q = TQ / (8 * WAVES), LOADS = LOADS_P + LOADS_Q;    // of a wave and stage
+    static constexpr int SCALE_WAVES = SCALE_BYTES / 1024;     // waves that have one more, for scales
+    static_assert(TP % (8 * WAVES) == 0 && TQ % (8 * WAVES) == 0 && WAVES % 2 == 0 && SCALE_BYTES % 1024 == 0 && SCALE_WAVES <= WAVES &&
+                  LDS_BYTES <= 160 * 1024, "whole loads per wave");
 
     struct Frags { u32x4_t p[FP], q[FQ]; };
     // step s of the stage in `buf`
@@ -286,20 +342,9 @@ struct Mx4Tile {
         for (int j = 0; j < FQ; ++j) f.q[j] = frag(q_row + 32 * j);
         __builtin_amdgcn_sched_barrier(0);                     // in front of the products of the step before, not behind them
     }
-    // Scales of a row's blocks 16 chunk .. + 15; behind the row's end the last one again.
-    static __device__ __forceinline__ u32x4_t chunk(const uint8_t* row, int chunk, int nb) {
-        u32x4_t v = {0, 0, 0, 0};
-        if (16 * chunk + 16 <= nb) {
-            __builtin_memcpy(&v, row + 16 * chunk, 16);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i / 4] |= (uint32_t)row[min(16 * chunk + i, nb - 1)] << (8 * (i % 4));
-        }
-        return v;
-    }
-    // From a chunk in LDS: those of blocks 2 s + h of stage st, one a byte.
-    static __device__ __forceinline__ uint32_t scales(const char* chunks, int row, int st, int h, int pitch) {
-        const u32x2_t v = *(const u32x2_t*)(chunks + (DEEP ? row * pitch + st * 8 : (st >> 1 & 1) * CHUNK_BYTES + row * 16 + (st & 1) * 8));
+    // Of a row in a stage: those of blocks 2 s + h, one a byte.
+    static __device__ __forceinline__ uint32_t scales(const char* stage, int row, int h) {
+        const u32x2_t v = *(const u32x2_t*)(stage + row * MX4_STAGE);
         return __builtin_amdgcn_perm(v[1], v[0], h ? 0x07050301u : 0x06040200u);
     }
 };
@@ -309,7 +354,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     using T = Mx4Tile<FP, WP, FQ, WQ, S>;
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-    const int nb = mx4_blocks(a.k), stages = (nb + 7) / 8;
+    const int nb = mx4_blocks(a.k), stages = mx4_stages(nb);
     const int n_tiles = (a.n + T::TP - 1) / T::TP;
     const int n0 = (int)(blockIdx.x % n_tiles) * T::TP;
     const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * T::TQ;
@@ -324,7 +369,14 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     for (int i = 0; i < T::LOADS_P; ++i) p_at[i] = (uint32_t)min(my_row + 8 * T::WAVES * i, p_last) * pitch;
 #pragma unroll
     for (int i = 0; i < T::LOADS_Q; ++i) q_at[i] = (uint32_t)min(my_row + 8 * T::WAVES * i, q_last) * pitch;
+    // and two rows' scales, of the stage that is fetched next
+    const int scale_row = 128 * wave + 2 * lane;
+    const int64_t scale_step = mx4_ordered_bytes(scale_row < T::TP ? a.n : a.m);
+    const char* scale_from = scale_row < T::TP ? (const char*)a.w_scales + (int64_t)(n0 + min(scale_row, p_last & ~1)) * MX4_STAGE
+                                               : (const char*)a.x_scales + (m0 + min(scale_row - T::TP, q_last & ~1)) * MX4_STAGE;
     auto fetch = [&](int st) {
+        if (wave < T::SCALE_WAVES) dma16(lds0 + T::SCALES_AT + (uint32_t)(st % T::STAGES) * T::SCALE_BYTES + wave * 1024, scale_from);
+        scale_from += scale_step;
         const uint32_t to = lds0 + (uint32_t)(st % T::STAGES) * T::STAGE_BYTES + wave * 1024;
         const uint32_t block = (uint32_t)min(st * 8 + my_block, nb - 1) * MX4_BLOCK_BYTES;
 #pragma unroll
@@ -332,31 +384,14 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 #pragma unroll
         for (int i = 0; i < T::LOADS_Q; ++i) dma16(to + T::TP * T::ROW_BYTES + i * T::WAVES * 1024, Q, q_at[i] + block);
     };
-    // this thread's rows of a chunk of scales
-    const int scale_pitch = T::scale_pitch(nb);
-    const uint8_t* scale_row[T::CHUNK_ROWS];
-    u32x4_t chunk[T::CHUNK_ROWS];
-    auto scales_of = [&](int r) {
-        return r < T::TP ? a.w_scales + (int64_t)(n0 + min(r, p_last)) * nb : a.x_scales + (m0 + min(r - T::TP, q_last)) * nb;
-    };
-#pragma unroll
-    for (int i = 0; i < T::CHUNK_ROWS; ++i) scale_row[i] = scales_of(threadIdx.x + 64 * T::WAVES * i);
-    auto fetch_chunk = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < T::CHUNK_ROWS; ++i) chunk[i] = T::chunk(scale_row[i], c, nb);
-    };
-    auto store_chunk = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < T::CHUNK_ROWS; ++i)
-            *(u32x4_t*)(lds + T::SCALES_AT + (c & 1) * T::CHUNK_BYTES + (threadIdx.x + 64 * T::WAVES * i) * 16) = chunk[i];
-    };
     const int p_row = wp + (lane & 31), q_row = T::TP + wq + (lane & 31);
     uint32_t sp[FP], sq[FQ];
     auto take_scales = [&](int st) {
+        const char* stage = lds + T::SCALES_AT + st % T::STAGES * T::SCALE_BYTES;
 #pragma unroll
-        for (int i = 0; i < FP; ++i) sp[i] = T::scales(lds + T::SCALES_AT, p_row + 32 * i, st, h, scale_pitch);
+        for (int i = 0; i < FP; ++i) sp[i] = T::scales(stage, p_row + 32 * i, h);
 #pragma unroll
-        for (int j = 0; j < FQ; ++j) sq[j] = T::scales(lds + T::SCALES_AT, q_row + 32 * j, st, h, scale_pitch);
+        for (int j = 0; j < FQ; ++j) sq[j] = T::scales(stage, q_row + 32 * j, h);
     };
     float16_t_ acc[FP][FQ];
 #pragma unroll
@@ -379,43 +414,22 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     typename T::Frags f0, f1;
     float* bias_lds = (float*)(lds + T::BIAS_AT);
     for (int c = threadIdx.x; c < T::TP; c += 64 * T::WAVES) bias_lds[c] = a.bias && c <= p_last ? a.bias[n0 + c] : 0.f;
-    if constexpr (T::DEEP) {
-        for (int st = 0; st < min(S, stages); ++st) fetch(st);
-        const int pieces = (nb + 15) / 16;
-        for (int c = threadIdx.x; c < (T::TP + T::TQ) * pieces; c += 64 * T::WAVES) {
-            const int r = c / pieces, at = c - r * pieces;
-            const u32x4_t v = T::chunk(scales_of(r), at, nb);
-            u32x2_t* to = (u32x2_t*)(lds + T::SCALES_AT + r * scale_pitch + 16 * at);
-            to[0] = (u32x2_t){v[0], v[1]};
-            if (16 * at + 8 < scale_pitch) to[1] = (u32x2_t){v[2], v[3]};
-        }
-        landed<0>();
-    } else {
-        fetch_chunk(0);
-        store_chunk(0);
-        fetch(0);
-        landed<0>();
-        if (stages > 1) fetch(1);
-    }
+    for (int st = 0; st < min(S, stages); ++st) fetch(st);
+    landed<0>();
     take_scales(0);
     T::read(f0, lds, 0, p_row, q_row, h);
     for (int st = 0; st < stages - 1; ++st) {
         const char* buf = lds + (st % T::STAGES) * T::STAGE_BYTES;
-        const bool new_chunk = !T::DEEP && (st & 1) && st + 1 < stages; // the next stage begins a chunk
-        if (new_chunk) fetch_chunk((st + 1) >> 1);
-        __builtin_amdgcn_sched_barrier(0);                     // on its way for the whole stage
         T::read(f1, buf, 1, p_row, q_row, h);
         multiply(f0, S0{});
         T::read(f0, buf, 2, p_row, q_row, h);
         multiply(f1, S1{});
         T::read(f1, buf, 3, p_row, q_row, h);
         multiply(f0, S2{});
-        // The compiler does not know of the loads into LDS and waits for its own as if they were the only ones: the chunk has
-        // to be put away before the next of those are sent out, or it would wait for them all.
-        if (new_chunk) store_chunk((st + 1) >> 1);
         // the next stage is there, and every wave has read all of this one
-        if (T::DEEP && st + S <= stages) landed<(S - 2) * (T::LOADS_P + T::LOADS_Q)>();
-        else landed<0>();
+        if (S == 2 || st + S > stages) landed<0>();
+        else if (wave < T::SCALE_WAVES) landed<(S - 2) * (T::LOADS + 1)>();
+        else landed<(S - 2) * T::LOADS>();
         if (st + S < stages) fetch(st + S);
         T::read(f0, lds + ((st + 1) % T::STAGES) * T::STAGE_BYTES, 0, p_row, q_row, h);
         multiply(f1, S3{});
@@ -697,14 +711,29 @@ static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_
          : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, false>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, false>);
 }
 
+static int prepare_launch(Mx4PrepareArgs& a, int dtype, hipStream_t stream) {
+    const int64_t nb = mx4_blocks(a.k), parts = dtype == NERFX_TYPE_MX4 ? a.m * mx4_stages(nb) : a.m * nb * 4;
+    a.w_groups = (int)std::min<int64_t>(((int64_t)a.n * mx4_stages(nb) + 255) / 256, 256);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.w_groups + mx4_grid(parts).x), dim3(256), 0, stream, a);
+        return launch_status("mx4_prepare_kernel");
+    };
+    const bool run = a.k % MX4_BLOCK == 0;
+    switch (dtype) {
+        case NERFX_TYPE_F32: return run ? go(mx4_prepare_kernel<NERFX_TYPE_F32, true>) : go(mx4_prepare_kernel<NERFX_TYPE_F32, false>);
+        case NERFX_TYPE_BF16: return run ? go(mx4_prepare_kernel<NERFX_TYPE_BF16, true>) : go(mx4_prepare_kernel<NERFX_TYPE_BF16, false>);
+        case NERFX_TYPE_F16: return run ? go(mx4_prepare_kernel<NERFX_TYPE_F16, true>) : go(mx4_prepare_kernel<NERFX_TYPE_F16, false>);
+        default: return go(mx4_prepare_kernel<NERFX_TYPE_MX4, true>);
+    }
+}
+
 template <int FP, int WP, int FQ, int WQ, int S>
 static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     using T = Mx4Tile<FP, WP, FQ, WQ, S>;
     const int64_t tiles = ((a.n + T::TP - 1) / T::TP) * ((a.m + T::TQ - 1) / T::TQ);
     NERFX_REQUIRE(tiles <= 1 << 22, "%lld x %d results are too many for one launch", (long long)a.m, a.n);
-    const int lds = T::lds_bytes(mx4_blocks(a.k));
-    NERFX_OPT_IN_LDS((mx4_tile_kernel<FP, WP, FQ, WQ, S>), lds);
-    hipLaunchKernelGGL((mx4_tile_kernel<FP, WP, FQ, WQ, S>), dim3((unsigned)tiles), dim3(64 * T::WAVES), lds, stream, a);
+    NERFX_OPT_IN_LDS((mx4_tile_kernel<FP, WP, FQ, WQ, S>), T::LDS_BYTES);
+    hipLaunchKernelGGL((mx4_tile_kernel<FP, WP, FQ, WQ, S>), dim3((unsigned)tiles), dim3(64 * T::WAVES), T::LDS_BYTES, stream, a);
     return launch_status("mx4_tile_kernel");
 }
 
@@ -715,22 +744,36 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //  stream  otherwise up to 256 values a row, or 512 and up to 256 columns: float rows are quantised in registers, once for every
 //          256 columns (16,384 x 4096 by 128: 40 us, 54 with tiles; by 512: 82, and 69 with tiles);
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
-//          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit) and a row's scales fit: a
-//          small product lasts as long as one tile does (256 x 4096 by 4096: 12 us, 21 with 128 x 128; 1024 x 4096 by 4096, 1024
-//          tiles: 28 and 27); else 128 x 128.
+//          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit): a small product lasts as
+//          long as one tile does (256 x 4096 by 4096: 13 us, 21 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 28 and 27);
+//          else 128 x 128.
 enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
 // Steps of 64 values that a row is worked on in: what the stream kernel is made for.
 static int stream_steps(int k) {
     const int ks = (k + 63) / 64;
     return ks <= 5 ? ks : 8;
 }
-static int mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype, bool& stage) {
+struct Mx4Plan {
+    int kind;
+    int64_t w_ordered, x_ordered, codes;                       // bytes of the workspace, in this order; all multiples of 16
+    int64_t scales;                                            // or, without tiles: scales in rows, behind the codes
+};
+static Mx4Plan mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype) {
     const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
-    stage = false;
-    if (!blocks_out && m <= SKINNY_ROWS && (!is_float || m * mx4_blocks(k) * 17 <= SKINNY_LDS)) return MX4_SKINNY;
-    if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20 && (blocks_out || m > SKINNY_ROWS)) return MX4_STREAM;
-    stage = is_float;
-    return !blocks_out && m <= SKINNY_ROWS ? MX4_SKINNY : MX4_TILE;
+    const int64_t nb = mx4_blocks(k);
+    Mx4Plan plan{};
+    if (!blocks_out && m <= SKINNY_ROWS) {
+        plan.kind = MX4_SKINNY;
+        if (is_float && m * nb * 17 > SKINNY_LDS) { plan.codes = m * nb * 16; plan.scales = (m * nb + 15) / 16 * 16; }
+    } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20) {
+        plan.kind = MX4_STREAM;
+    } else {
+        plan.kind = MX4_TILE;
+        plan.w_ordered = mx4_stages(nb) * mx4_ordered_bytes(n);
+        plan.x_ordered = mx4_stages(nb) * mx4_ordered_bytes(m);
+        if (is_float) plan.codes = m * nb * 16;
+    }
+    return plan;
 }
 
 template <int DT>
@@ -820,10 +863,8 @@ static bool mx4_type(int dtype) { return float_type(dtype) || dtype == NERFX_TYP
 
 extern "C" int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype) {
     if (check_mx4(m, k) || n < 0 || n > 1 << 24 || !mx4_type(x_dtype) || !mx4_type(y_dtype)) return -1;
-    bool stage;
-    mx4_plan(m, n, k, x_dtype, y_dtype, stage);
-    if (!stage) return 0;
-    return (m * mx4_blocks(k) * 17 + 15) / 16 * 16;
+    const Mx4Plan plan = mx4_plan(m, n, k, x_dtype, y_dtype);
+    return plan.w_ordered + plan.x_ordered + plan.codes + plan.scales;
 }
 
 extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k, const uint8_t* w_codes,
@@ -847,21 +888,27 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
     a.m = m; a.n = n; a.k = k; a.activ = activ; a.y_dtype = y_dtype;
     a.x = (const uint8_t*)x; a.x_scales = x_scales;
     const hipStream_t st = (hipStream_t)stream;
-    bool stage;
-    const int plan = mx4_plan(m, n, k, x_dtype, y_dtype, stage);
-    if (stage) {
-        uint8_t* codes = (uint8_t*)workspace;
-        uint8_t* scales = codes + m * mx4_blocks(k) * 16;
+    const Mx4Plan plan = mx4_plan(m, n, k, x_dtype, y_dtype);
+    if (plan.kind == MX4_TILE) {
+        Mx4PrepareArgs p{};
+        p.x = x; p.x_scales = x_scales; p.w_scales = w_scales; p.m = m; p.n = n; p.k = k;
+        p.w_ordered = (uint8_t*)workspace;
+        p.x_ordered = p.w_ordered + plan.w_ordered;
+        p.codes = (uint32_t*)(p.x_ordered + plan.x_ordered);
+        if (int rc = prepare_launch(p, x_dtype, st)) return rc;
+        a.w_scales = p.w_ordered; a.x_scales = p.x_ordered;
+        if (x_dtype != NERFX_TYPE_MX4) a.x = (const uint8_t*)p.codes;
+        const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256), small = ((a.m + 63) / 64) * ((a.n + 63) / 64);
+        if (small <= 512) return tile_launch<1, 2, 1, 2, 3>(a, st);
+        return big >= 192 ? tile_launch<4, 2, 2, 4, 2>(a, st) : tile_launch<2, 2, 2, 2, 2>(a, st);
+    }
+    if (plan.codes) {
+        uint8_t *codes = (uint8_t*)workspace, *scales = codes + plan.codes;
         if (int rc = quantize_launch(x, x_dtype, m, k, codes, scales, st)) return rc;
         a.x = codes; a.x_scales = scales;
         x_dtype = NERFX_TYPE_MX4;
     }
-    if (plan == MX4_TILE) {
-        const int64_t big = ((a.m + 255) / 256) * ((a.n + 255) / 256), small = ((a.m + 63) / 64) * ((a.n + 63) / 64);
-        if (small <= 512 && Mx4Tile<1, 2, 1, 2, 3>::lds_bytes(mx4_blocks(k)) <= 160 * 1024) return tile_launch<1, 2, 1, 2, 3>(a, st);
-        return big >= 192 ? tile_launch<4, 2, 2, 4, 2>(a, st) : tile_launch<2, 2, 2, 2, 2>(a, st);
-    }
-    auto by_type = [&](auto skinny, auto str) { return plan == MX4_SKINNY ? skinny(a, st) : str(a, st); };
+    auto by_type = [&](auto skinny, auto str) { return plan.kind == MX4_SKINNY ? skinny(a, st) : str(a, st); };
     switch (x_dtype) {
         case NERFX_TYPE_F32: return by_type(skinny_launch<NERFX_TYPE_F32>, stream_launch<NERFX_TYPE_F32>);
         case NERFX_TYPE_BF16: return by_type(skinny_launch<NERFX_TYPE_BF16>, stream_launch<NERFX_TYPE_BF16>);
