@@ -40,15 +40,35 @@ __device__ __forceinline__ Mx4Raw<DT, N> mx4_load_whole(const char* row, int at)
     return v;
 }
 
+// A row's last values, fewer than N, are read as its last N and moved down: one by one each would be waited for.
 template <int DT, int N>
 __device__ __forceinline__ Mx4Raw<DT, N> mx4_load(const char* row, int at, int k) {
+    using Raw = Mx4Raw<DT, N>;
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
-    Mx4Raw<DT, N> v;
+    Raw v;
     if (at + N <= k) {
         v = mx4_load_whole<DT, N>(row, at);
+    } else if (at >= k) {
+#pragma unroll
+        for (int i = 0; i < Raw::WORDS; ++i) v.w[i] = 0u;
+    } else if (k >= N) {
+        v = mx4_load_whole<DT, N>(row, k - N);
+        const int down = N - k % N;                            // the same for every lane
+        if (SIZE == 2 && (down & 1)) {
+#pragma unroll
+            for (int i = 0; i < Raw::WORDS; ++i) v.w[i] = v.w[i] >> 16 | (i + 1 < Raw::WORDS ? v.w[i + 1] << 16 : 0u);
+        }
+        const int words = SIZE == 2 ? down / 2 : down;
+#pragma unroll
+        for (int bit = 1; bit < Raw::WORDS; bit *= 2) {
+            if (words & bit) {
+#pragma unroll
+                for (int i = 0; i < Raw::WORDS; ++i) v.w[i] = i + bit < Raw::WORDS ? v.w[i + bit] : 0u;
+            }
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < Mx4Raw<DT, N>::WORDS; ++i) {
+        for (int i = 0; i < Raw::WORDS; ++i) {
             if constexpr (SIZE == 4) {
                 v.w[i] = at + i < k ? *(const uint32_t*)(row + (int64_t)(at + i) * 4) : 0u;
             } else {
