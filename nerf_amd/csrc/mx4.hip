@@ -505,7 +505,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 // of K; each lane's 16-byte load is a block of W, which is an operand of the matrix instruction as it
 // is (16 x 16 x 128).  Rows of x in a float type are quantised by the workgroup into LDS, a block a thread, while the first
 // loads of W are on their way.
-constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024;
+constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024, SKINNY_FLOATS = 128 * 1024;
 
 __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
     const float v = mx4_activate(acc + (a.bias ? a.bias[n] : 0.f), a.activ);
@@ -758,9 +758,10 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 }
 
 // How a product is done, by its sizes:
-//  skinny  up to 64 rows of x, as long as float rows fit in LDS as codes (else by way of the workspace): W is read once, by
-//          as many workgroups as it has 16 rows (one row by 4096 x 4096: 62 us with tiles).  Not for a result in blocks, which
-//          are of 32 columns;
+//  skinny  up to 64 rows of x: W is read once, by as many workgroups as it has 16 rows (one row by 4096 x 4096: 5.7 us, 11 with
+//          tiles).  Each of them quantises float rows for itself, up to 128 KB of them (64 x 1000 fp32 by 1000: 15 us, 7.6 with
+//          tiles; 32 x 2048 bf16 by 256: 7 and 8.5), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
+//          Not for a result in blocks, which are of 32 columns;
 //  stream  otherwise up to 256 values a row, or 512 and up to 256 columns: float rows are quantised in registers, once for every
 //          256 columns (16,384 x 4096 by 128: 40 us, 54 with tiles; by 512: 82, and 69 with tiles);
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
@@ -782,7 +783,8 @@ static Mx4Plan mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype) {
     const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
     const int64_t nb = mx4_blocks(k);
     Mx4Plan plan{};
-    if (!blocks_out && m <= SKINNY_ROWS) {
+    const int64_t x_bytes = m * k * (x_dtype == NERFX_TYPE_F32 ? 4 : 2);
+    if (!blocks_out && m <= (!is_float || x_bytes <= SKINNY_FLOATS ? SKINNY_ROWS : 16)) {
         plan.kind = MX4_SKINNY;
         if (is_float && m * nb * 17 > SKINNY_LDS) { plan.codes = m * nb * 16; plan.scales = (m * nb + 15) / 16 * 16; }
     } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20) {

@@ -165,7 +165,8 @@ def test_linear(ops, dtype, m, n, k):
 # Columns in several groups; tiles of each size, with rows of one stage and more, and too long for their scales to be in LDS.
 @pytest.mark.parametrize("m,n,k", [(70, 300, 200), (300, 1000, 256), (5000, 520, 33), (600, 2100, 64), (20000, 257, 256), (70, 100, 30000),
                                    (100, 70, 8200), (65, 65, 513), (2100, 1600, 300), (1700, 2500, 1100), (2100, 1600, 520), (6200, 2050, 290),
-                                   (5000, 3000, 700), (12300, 1030, 545)])
+                                   (5000, 3000, 700), (12300, 1030, 545), (16, 20, 8200),
+                                   (3, 5, 60000), (33, 100, 4096)])
 def test_linear_many_columns_and_tiles(ops, m, n, k):
     x, w, bias = pair(m, n, k, torch.bfloat16, 8)
     check_linear(ops, x, w, bias, "relu", what=f"{m} x {n} by {k}")
