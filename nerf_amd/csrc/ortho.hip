@@ -77,12 +77,13 @@ __device__ __forceinline__ void store_from_float(void* p, int64_t i, float v, in
     else if (dtype == NERFX_TYPE_F16) ((_Float16*)p)[i] = (_Float16)v;
     else ((__bf16*)p)[i] = (__bf16)v;
 }
-// What is orthogonalised, at flat index i: the gradient, or the optimiser's mix of it and the (new) momentum.
-__device__ __forceinline__ float update_at(const OrthoCall& a, const OrthoMat& q, int64_t i, float unscale) {
-    const float g = load_as_float(q.grad, i, a.dtype);
+// What is orthogonalised: the gradient, or the optimiser's mix of it and the (new) momentum.
+__device__ __forceinline__ float update_of(const OrthoCall& a, float g, float mom, float unscale) {
     if (!a.muon) return g;
-    const float mom = q.momentum[i];
     return a.nesterov ? fmaf(a.momentum, mom, a.rest * (g * unscale)) : mom;
+}
+__device__ __forceinline__ float update_at(const OrthoCall& a, const OrthoMat& q, int64_t i, float unscale) {
+    return update_of(a, load_as_float(q.grad, i, a.dtype), a.muon ? q.momentum[i] : 0.f, unscale);
 }
 
 // The matrix that this block works on, and the block's number within it.  (All of a row of the table is read at
@@ -113,11 +114,26 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable t, cha
     const bool skip = a.found_inf && *a.found_inf != 0.f;
     const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
     double acc = 0;
-    for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < total; i += (int64_t)parts * 256) {
-        if (a.muon && !skip)
-            q.momentum[i] = fmaf(a.momentum, q.momentum[i], a.rest * (((const float*)q.grad)[i] * unscale));
-        const double u = update_at(a, q, i, unscale);
-        acc = fma(u, u, acc);
+    const int64_t step = (int64_t)parts * 256;
+    constexpr int AT_ONCE = 8;                                 // loads in flight: a momentum's store would end the next one's
+    for (int64_t i0 = (int64_t)b * 256 + threadIdx.x; i0 < total; i0 += AT_ONCE * step) {
+        float g[AT_ONCE], mom[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int64_t i = min(i0 + j * step, total - 1);
+            g[j] = load_as_float(q.grad, i, a.dtype);
+            mom[j] = a.muon ? q.momentum[i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            if (i0 + j * step >= total) break;
+            float u = g[j];
+            if (a.muon) {
+                if (!skip) q.momentum[i0 + j * step] = mom[j] = fmaf(a.momentum, mom[j], a.rest * (g[j] * unscale));
+                u = update_of(a, g[j], mom[j], unscale);
+            }
+            acc = fma((double)u, (double)u, acc);
+        }
     }
     __shared__ double part[4];
 #pragma unroll
@@ -133,6 +149,16 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __res
     const OrthoMat q = t->mat[which_matrix(*t, ORTHO_PREP_GRID, b)];
     const OrthoCall a = t->call;
     __shared__ float tile[PREP_TILE][PREP_TILE + 1];
+    const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
+    const int x0 = b / (q.n / PREP_TILE) * PREP_TILE, y0 = b % (q.n / PREP_TILE) * PREP_TILE;   // of X
+    // G's rows run along X's columns, or, if G is tall, along X's rows
+    const int r0 = q.tall ? y0 : x0, c0 = q.tall ? x0 : y0;
+    float own[PREP_TILE * PREP_TILE / 256];                    // on its way while the norm is put together
+#pragma unroll
+    for (int j = 0; j < PREP_TILE * PREP_TILE / 256; ++j) {
+        const int e = threadIdx.x + 256 * j, r = min(r0 + e / PREP_TILE, q.rows - 1), c = min(c0 + e % PREP_TILE, q.cols - 1);
+        own[j] = update_at(a, q, (int64_t)r * q.cols + c, unscale);
+    }
     const double* sums = (const double*)(work + ortho_sums_at(q));
     __shared__ double part[4];
     double total = 0;
@@ -149,14 +175,10 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __res
     if (norm < (double)a.eps) lift = max(0, min(120, norm > 0 ? ilogb((double)a.eps / norm) - a.growth : 0));
     factor = ldexp(factor, lift);
     if (b == 0 && threadIdx.x == 0) *(int*)(work + ortho_lift_at(q)) = lift;
-    const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
-    const int x0 = b / (q.n / PREP_TILE) * PREP_TILE, y0 = b % (q.n / PREP_TILE) * PREP_TILE;   // of X
-    // G's rows run along X's columns, or, if G is tall, along X's rows
-    const int r0 = q.tall ? y0 : x0, c0 = q.tall ? x0 : y0;
-    for (int e = threadIdx.x; e < PREP_TILE * PREP_TILE; e += 256) {
-        const int r = e / PREP_TILE, c = e % PREP_TILE;
-        float v = 0.f;
-        if (r0 + r < q.rows && c0 + c < q.cols) v = (float)(update_at(a, q, (int64_t)(r0 + r) * q.cols + c0 + c, unscale) * factor);
+#pragma unroll
+    for (int j = 0; j < PREP_TILE * PREP_TILE / 256; ++j) {
+        const int e = threadIdx.x + 256 * j, r = e / PREP_TILE, c = e % PREP_TILE;
+        const float v = r0 + r < q.rows && c0 + c < q.cols ? (float)(own[j] * factor) : 0.f;
         if (q.tall) tile[c][r] = v; else tile[r][c] = v;
     }
     __syncthreads();
@@ -277,11 +299,11 @@ struct SplitTile {
 };
 
 // Number t of a lower triangle's tiles, row after row -> (row, column).
-__device__ __forceinline__ void triangle_at(int64_t t, int& i, int& j) {
-    i = (int)((sqrt(8.0 * (double)t + 1.0) - 1.0) * 0.5);
-    while ((int64_t)i * (i + 1) / 2 > t) --i;
-    while ((int64_t)(i + 1) * (i + 2) / 2 <= t) ++i;
-    j = (int)(t - (int64_t)i * (i + 1) / 2);
+__device__ __forceinline__ void triangle_at(int t, int& i, int& j) {
+    i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) / 2 > t) --i;
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    j = t - i * (i + 1) / 2;
 }
 
 template <int T, int WAVES, int STAGES, int KIND>
@@ -320,9 +342,10 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
                     own[i][j][e] = split_load4(Q, tj * T + Tile::col_of(wave) + 32 * j + (lane & 31),
                                                ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e, q.m);
     }
+    int lift = 0;                                                        // see the kernel that made X
+    if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) lift = *(const int*)(work + ortho_lift_at(q));
     tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K);
-    if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {            // see the kernel that made X
-        const int lift = *(const int*)(work + ortho_lift_at(q));
+    if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {
         beta = ldexpf(beta, KIND == ORTHO_GRAM ? -2 * lift : -lift);
         alpha = ldexpf(alpha, -lift);
     }
