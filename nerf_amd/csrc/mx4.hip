@@ -375,9 +375,10 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
     const int nb = mx4_blocks(a.k), stages = mx4_stages(nb);
-    const int n_tiles = (a.n + T::TP - 1) / T::TP;
-    const int n0 = (int)(blockIdx.x % n_tiles) * T::TP;
-    const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * T::TQ;
+    int m_tile, n_tile;
+    band_at(xcd_place(), (int)((a.m + T::TQ - 1) / T::TQ), (a.n + T::TP - 1) / T::TP, m_tile, n_tile);
+    const int n0 = n_tile * T::TP;
+    const int64_t m0 = (int64_t)m_tile * T::TQ;
     const int wp = wave / WQ * 32 * FP, wq = wave % WQ * 32 * FQ;
     const uint32_t pitch = (uint32_t)nb * MX4_BLOCK_BYTES, lds0 = lds_address(lds);
     const char *P = (const char*)a.w + (int64_t)n0 * pitch, *Q = (const char*)a.x + m0 * pitch;

@@ -88,8 +88,7 @@ __device__ __forceinline__ float update_at(const OrthoCall& a, const OrthoMat& q
 
 // The matrix that this block works on, and the block's number within it.  (All of a row of the table is read at
 // once: walking it would wait for each entry in turn.)
-__device__ __forceinline__ int which_matrix(const OrthoTable& t, int grid, int& block) {
-    const int b = blockIdx.x;
+__device__ __forceinline__ int which_matrix(const OrthoTable& t, int grid, int b, int& block) {
     int k = 0, start = 0;
 #pragma unroll
     for (int i = 1; i < ORTHO_GROUP; ++i) {
@@ -105,7 +104,7 @@ enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
 // neither overflows nor vanishes there, and a sum of 2^30 of them keeps fp32's precision.
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable t, char* work) {
     int b;
-    const OrthoMat q = t.mat[which_matrix(t, ORTHO_NORM_GRID, b)];
+    const OrthoMat q = t.mat[which_matrix(t, ORTHO_NORM_GRID, blockIdx.x, b)];
     const OrthoCall& a = t.call;
     if (blockIdx.x == 0)                                       // for the launches behind this one
         for (int i = threadIdx.x; i < (int)(sizeof(OrthoTable) / 4); i += 256) ((uint32_t*)work)[i] = ((const uint32_t*)&t)[i];
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable t, cha
 // X and X^T from what is orthogonalised: one 64 x 64 tile of X per block, through LDS, zeros in the padding.
 __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __restrict__ t, char* __restrict__ work) {
     int b;
-    const OrthoMat q = t->mat[which_matrix(*t, ORTHO_PREP_GRID, b)];
+    const OrthoMat q = t->mat[which_matrix(*t, ORTHO_PREP_GRID, blockIdx.x, b)];
     const OrthoCall a = t->call;
     __shared__ float tile[PREP_TILE][PREP_TILE + 1];
     const float unscale = a.grad_scale ? 1.0f / *a.grad_scale : 1.0f;
@@ -312,7 +311,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     extern __shared__ __align__(16) char lds[];
     constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;       // the result is symmetric: half of the tiles
     int b;
-    const OrthoMat q = t->mat[which_matrix(*t, SYM ? ORTHO_SYM_GRID : ORTHO_FULL_GRID, b)];
+    const OrthoMat q = t->mat[which_matrix(*t, SYM ? ORTHO_SYM_GRID : ORTHO_FULL_GRID, xcd_place(), b)];
     int ti, tj;
     if constexpr (SYM) {
         triangle_at(b, ti, tj);
