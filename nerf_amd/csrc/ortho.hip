@@ -297,6 +297,58 @@ struct SplitTile {
     static __device__ __forceinline__ int col_of(int wave) { return wave % (WAVES / 2) * (2 * T / WAVES); }
 };
 
+// A wave's 32 x 32 results on their way to a split matrix and to its transpose.  They go through LDS, one orientation after the
+// other, and leave as whole lines of 128 bytes: stored from the registers, in pieces of 2 and 8 bytes, they were a quarter of a
+// small matrix's time (a field's six: 129 us, 122 so).
+struct SplitLines {
+    static constexpr int PITCH = SPLIT_BLOCK_BYTES + 16, BYTES = 32 * PITCH;
+    char* lds;
+    half4_t hi[4], lo[4];
+
+    // Rows 8 e + 4 (lane / 32) .. + 3 of column lane % 32.
+    __device__ __forceinline__ void take(int e, const float (&v)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            _Float16 h, l;
+            split16(v[k], h, l);
+            hi[e][k] = h;
+            lo[e][k] = l;
+        }
+    }
+    __device__ __forceinline__ void store(char* dst, int row, int col, int width) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                char* p = lds + (8 * e + 4 * (lane >> 5) + k) * PITCH + 2 * (lane & 31);
+                *(_Float16*)p = hi[e][k];
+                *(_Float16*)(p + 64) = lo[e][k];
+            }
+        leave(dst, row, col, width);
+    }
+    __device__ __forceinline__ void store_transposed(char* dst, int row, int col, int width) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            char* p = lds + (lane & 31) * PITCH + 2 * (8 * e + 4 * (lane >> 5));
+            *(half4_t*)p = hi[e];
+            *(half4_t*)(p + 64) = lo[e];
+        }
+        leave(dst, row, col, width);
+    }
+
+private:
+    __device__ __forceinline__ void leave(char* dst, int row, int col, int width) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 3), piece = 16 * (lane & 7);
+            *(u32x4_t*)(split_at(dst, row + r, col, width) + piece) = *(const u32x4_t*)(lds + r * PITCH + piece);
+        }
+    }
+};
+
 // Number t of a lower triangle's tiles, row after row -> (row, column).
 __device__ __forceinline__ void triangle_at(int t, int& i, int& j) {
     i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -350,6 +402,9 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     }
     const OrthoCall a = t->call;
     const bool skip = KIND == ORTHO_LAST && a.found_inf && *a.found_inf != 0.f;
+    if constexpr (KIND != ORTHO_LAST) __syncthreads();                   // the stages have been read: their place is the waves' own now
+    SplitLines lines{lds + wave * SplitLines::BYTES};
+    static_assert(WAVES * SplitLines::BYTES <= Tile::LDS_BYTES, "a place for each wave");
 #pragma unroll
     for (int i = 0; i < Tile::FP; ++i)
 #pragma unroll
@@ -368,28 +423,9 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
                     for (int k = 0; k < 4; ++k)
                         v[k] = fmaf(beta, tile.acc[i][j][4 * e + k], alpha * ((float)own[i][j][e].hi[k] + (float)own[i][j][e].lo[k]));
                 }
-                if constexpr (SYM) {
-                    char* dst = KIND == ORTHO_GRAM ? A : B;
-                    if (ti != tj) split_store4(dst, col, row, q.m, v);             // the mirrored tile
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        _Float16 hi, lo;
-                        split16(v[k], hi, lo);
-                        char* p = split_at(dst, row + k, col, q.m);
-                        *(_Float16*)p = hi;
-                        *(_Float16*)(p + 64) = lo;
-                    }
-                } else if constexpr (KIND == ORTHO_APPLY) {
-                    split_store4(work + ortho_xt_at(q, from ^ 1), col, row, q.m, v);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        _Float16 hi, lo;
-                        split16(v[k], hi, lo);
-                        char* p = split_at(X, row + k, col, q.n);
-                        *(_Float16*)p = hi;
-                        *(_Float16*)(p + 64) = lo;
-                    }
-                } else if (!skip) {                                                // into the caller's matrix
+                if constexpr (KIND != ORTHO_LAST) {
+                    lines.take(e, v);
+                } else if (!skip) {                            // into the caller's matrix
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int r = q.tall ? col : row + k, c = q.tall ? row + k : col;
@@ -399,6 +435,12 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
                         else store_from_float(q.out, at, v[k], a.dtype);
                     }
                 }
+            }
+            if constexpr (KIND != ORTHO_LAST) {
+                const int r = row0 - 4 * (lane >> 5), c = col - (lane & 31);
+                char* dst = KIND == ORTHO_GRAM ? A : KIND == ORTHO_POLY ? B : X;
+                lines.store(dst, r, c, SYM ? q.m : q.n);
+                if (!SYM || ti != tj) lines.store_transposed(SYM ? dst : work + ortho_xt_at(q, from ^ 1), c, r, q.m);
             }
         }
 }
