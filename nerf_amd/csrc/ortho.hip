@@ -274,6 +274,24 @@ struct SplitTile {
         for (int kb = 0; kb < STAGES; ++kb)
             if (kb < steps) fetch(kb);
         Frags f0, f1;
+        if (whole(K)) {                                      // all there is, in LDS at once: no waits between the stages
+            landed<0>();
+            read(f0, lds, 0, wave, lane);
+            read(f1, lds, 1, wave, lane);
+            for (int kb = 0; kb < steps - 1; ++kb) {
+                Frags g0, g1;
+                read(g0, lds + (kb + 1) * STAGE_BYTES, 0, wave, lane);
+                read(g1, lds + (kb + 1) * STAGE_BYTES, 1, wave, lane);
+                multiply(f0);
+                multiply(f1);
+                f0 = g0;
+                f1 = g1;
+            }
+            multiply(f0);
+            multiply(f1);
+            add_cross();
+            return;
+        }
         wait(steps - 1);
         read(f0, lds, 0, wave, lane);
         for (int kb = 0; kb < steps - 1; ++kb) {             // fragments are read one half stage ahead of their use
@@ -287,6 +305,17 @@ struct SplitTile {
         read(f1, lds + ((steps - 1) % STAGES) * STAGE_BYTES, 1, wave, lane);
         multiply(f0);
         multiply(f1);
+        add_cross();
+    }
+    // Whether rows of K values lie in LDS altogether.
+    static __device__ __forceinline__ bool whole(int K) { return STAGES == 8 && K <= STAGES * SPLIT_BLOCK; }
+    // If they do: values k .. k + 3 of Q's row r (of the tile).
+    static __device__ __forceinline__ Split4 here(const char* lds, int r, int k) {
+        const char* block = lds + k / SPLIT_BLOCK * STAGE_BYTES + (T + r) * SPLIT_BLOCK_BYTES + 2 * (k & 4);
+        const int chunk = k % SPLIT_BLOCK / 8, turn = (T + r) >> 1 & 7;
+        return {*(const half4_t*)(block + (chunk ^ turn) * 16), *(const half4_t*)(block + ((chunk + 4) ^ turn) * 16)};
+    }
+    __device__ __forceinline__ void add_cross() {
 #pragma unroll
         for (int i = 0; i < FP; ++i)
 #pragma unroll
@@ -381,21 +410,24 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     Tile tile;
     // element (row, col) of a 32 x 32 accumulator: col = lane % 32, row = 8 (e / 4) + 4 (lane / 32) + e % 4
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // the element itself, A[row][col] = A[col][row] or X[row][col] = X^T[col][row], is on its way from the start
+    // the element itself, A[row][col] = A[col][row] or X[row][col] = X^T[col][row], is on its way from the start, or in LDS
     Split4 own[Tile::FP][Tile::FQ][4];
-    if constexpr (KIND != ORTHO_GRAM) {
+    auto each_own = [&](auto load) {
 #pragma unroll
         for (int i = 0; i < Tile::FP; ++i)
 #pragma unroll
             for (int j = 0; j < Tile::FQ; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    own[i][j][e] = split_load4(Q, tj * T + Tile::col_of(wave) + 32 * j + (lane & 31),
-                                               ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e, q.m);
-    }
+                    own[i][j][e] = load(Tile::col_of(wave) + 32 * j + (lane & 31), ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e);
+    };
+    if constexpr (KIND != ORTHO_GRAM)
+        if (!Tile::whole(K)) each_own([&](int r, int k) { return split_load4(Q, tj * T + r, k, q.m); });
     int lift = 0;                                                        // see the kernel that made X
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) lift = *(const int*)(work + ortho_lift_at(q));
     tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K);
+    if constexpr (KIND != ORTHO_GRAM)
+        if (Tile::whole(K)) each_own([&](int r, int k) { return Tile::here(lds, r, k); });
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {
         beta = ldexpf(beta, KIND == ORTHO_GRAM ? -2 * lift : -lift);
         alpha = ldexpf(alpha, -lift);
