@@ -247,7 +247,9 @@ struct SplitTile {
                 }
     }
 
-    __device__ __forceinline__ void run(char* lds, const char* P, const char* Q, int K) {
+    // `seen(kb, stage)` is called once per stage, while it is in LDS.
+    template <class Seen>
+    __device__ __forceinline__ void run(char* lds, const char* P, const char* Q, int K, Seen seen) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t pitch = (uint32_t)K / SPLIT_BLOCK * SPLIT_BLOCK_BYTES;
         const int steps = K / SPLIT_BLOCK;
@@ -279,6 +281,7 @@ struct SplitTile {
             read(f0, lds, 0, wave, lane);
             read(f1, lds, 1, wave, lane);
             for (int kb = 0; kb < steps - 1; ++kb) {
+                seen(kb, lds + kb * STAGE_BYTES);
                 Frags g0, g1;
                 read(g0, lds + (kb + 1) * STAGE_BYTES, 0, wave, lane);
                 read(g1, lds + (kb + 1) * STAGE_BYTES, 1, wave, lane);
@@ -287,6 +290,7 @@ struct SplitTile {
                 f0 = g0;
                 f1 = g1;
             }
+            seen(steps - 1, lds + (steps - 1) * STAGE_BYTES);
             multiply(f0);
             multiply(f1);
             add_cross();
@@ -296,6 +300,7 @@ struct SplitTile {
         read(f0, lds, 0, wave, lane);
         for (int kb = 0; kb < steps - 1; ++kb) {             // fragments are read one half stage ahead of their use
             read(f1, lds + (kb % STAGES) * STAGE_BYTES, 1, wave, lane);
+            seen(kb, lds + (kb % STAGES) * STAGE_BYTES);
             multiply(f0);
             wait(min(STAGES - 2, steps - 2 - kb));           // stage kb + 1 is there, and every wave has read all of stage kb,
             if (kb + STAGES < steps) fetch(kb + STAGES);     // whose place this one takes
@@ -303,17 +308,18 @@ struct SplitTile {
             multiply(f1);
         }
         read(f1, lds + ((steps - 1) % STAGES) * STAGE_BYTES, 1, wave, lane);
+        seen(steps - 1, lds + ((steps - 1) % STAGES) * STAGE_BYTES);
         multiply(f0);
         multiply(f1);
         add_cross();
     }
     // Whether rows of K values lie in LDS altogether.
     static __device__ __forceinline__ bool whole(int K) { return STAGES == 8 && K <= STAGES * SPLIT_BLOCK; }
-    // If they do: values k .. k + 3 of Q's row r (of the tile).
-    static __device__ __forceinline__ Split4 here(const char* lds, int r, int k) {
-        const char* block = lds + k / SPLIT_BLOCK * STAGE_BYTES + (T + r) * SPLIT_BLOCK_BYTES + 2 * (k & 4);
-        const int chunk = k % SPLIT_BLOCK / 8, turn = (T + r) >> 1 & 7;
-        return {*(const half4_t*)(block + (chunk ^ turn) * 16), *(const half4_t*)(block + ((chunk + 4) ^ turn) * 16)};
+    // In a stage: its values k .. k + 3 of Q's row r (of the tile).
+    static __device__ __forceinline__ Split4 here(const char* stage, int r, int k) {
+        const char* row = stage + (T + r) * SPLIT_BLOCK_BYTES + 2 * (k & 4);
+        const int turn = (T + r) >> 1 & 7;
+        return {*(const half4_t*)(row + (k / 8 ^ turn) * 16), *(const half4_t*)(row + (k / 8 + 4 ^ turn) * 16)};
     }
     __device__ __forceinline__ void add_cross() {
 #pragma unroll
@@ -409,25 +415,25 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     using Tile = SplitTile<T, WAVES, STAGES>;
     Tile tile;
     // element (row, col) of a 32 x 32 accumulator: col = lane % 32, row = 8 (e / 4) + 4 (lane / 32) + e % 4
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // the element itself, A[row][col] = A[col][row] or X[row][col] = X^T[col][row], is on its way from the start, or in LDS
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the element itself, A[row][col] = A[col][row] or X[row][col] = X^T[col][row], comes by in one of the stages
     Split4 own[Tile::FP][Tile::FQ][4];
-    auto each_own = [&](auto load) {
+    auto keep_own = [&](int kb, const char* stage) {
+        if constexpr (KIND != ORTHO_GRAM) {
 #pragma unroll
-        for (int i = 0; i < Tile::FP; ++i)
+            for (int i = 0; i < Tile::FP; ++i) {
+                if (kb != (ti * T + Tile::row_of(wave)) / SPLIT_BLOCK + i) continue;
 #pragma unroll
-            for (int j = 0; j < Tile::FQ; ++j)
+                for (int j = 0; j < Tile::FQ; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    own[i][j][e] = load(Tile::col_of(wave) + 32 * j + (lane & 31), ti * T + Tile::row_of(wave) + 32 * i + 4 * (lane >> 5) + 8 * e);
+                    for (int e = 0; e < 4; ++e)
+                        own[i][j][e] = Tile::here(stage, Tile::col_of(wave) + 32 * j + (lane & 31), 4 * (lane >> 5) + 8 * e);
+            }
+        }
     };
-    if constexpr (KIND != ORTHO_GRAM)
-        if (!Tile::whole(K)) each_own([&](int r, int k) { return split_load4(Q, tj * T + r, k, q.m); });
     int lift = 0;                                                        // see the kernel that made X
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) lift = *(const int*)(work + ortho_lift_at(q));
-    tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K);
-    if constexpr (KIND != ORTHO_GRAM)
-        if (Tile::whole(K)) each_own([&](int r, int k) { return Tile::here(lds, r, k); });
+    tile.run(lds, P + (int64_t)ti * T * K * 4, Q + (int64_t)tj * T * K * 4, K, keep_own);
     if constexpr (KIND == ORTHO_GRAM || KIND == ORTHO_LAST) {
         beta = ldexpf(beta, KIND == ORTHO_GRAM ? -2 * lift : -lift);
         alpha = ldexpf(alpha, -lift);

@@ -40,10 +40,6 @@ __device__ __forceinline__ void split_store4(char* base, int64_t r, int k, int n
     *(half4_t*)(p + 64) = lo;
 }
 struct Split4 { half4_t hi, lo; };
-__device__ __forceinline__ Split4 split_load4(const char* base, int64_t r, int k, int n_cols) {
-    const char* p = split_at(const_cast<char*>(base), r, k, n_cols);
-    return {*(const half4_t*)p, *(const half4_t*)(p + 64)};
-}
 #endif
 
 }  // namespace nerfx
