@@ -100,6 +100,37 @@ __device__ __forceinline__ int which_matrix(const OrthoTable& t, int grid, int b
 }
 enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
 
+// Matrices with a side of up to 16 are kept and multiplied in fp32: sums of so few terms leave nothing for the 2^-23 of two halves to
+// average out in (8 x 60: 6e-7 off float64, in halves 1.0e-6), and there is next to nothing to
+// compute.  X and X^T, A and B take the same places, an element its 4 bytes.
+__host__ __device__ inline bool ortho_tiny(const OrthoMat& q) { return (q.rows < q.cols ? q.rows : q.cols) <= 16; }
+
+// 16 rows of P times 16 rows of Q, over values k0, k0 + 1 .. + 15, then step values on, up to K (a multiple of 16): element i of the
+// result is that of P's row 4 (lane / 16) + i and Q's row lane % 16.
+__device__ __forceinline__ f32x4_t tiny_product(const float* P, int64_t p_pitch, const float* Q, int64_t q_pitch, int k0, int step, int K) {
+    const int lane = threadIdx.x & 63;
+    P += (lane & 15) * p_pitch + 4 * (lane >> 4);
+    Q += (lane & 15) * q_pitch + 4 * (lane >> 4);
+    f32x4_t sum[4] = {};
+    for (int k = k0; k < K; k += step) {
+        const f32x4_t a = *(const f32x4_t*)(P + k), b = *(const f32x4_t*)(Q + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], sum[j], 0, 0, 0);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// The parts of a sum that a workgroup's waves have, added up: in the first wave.
+template <int WAVES>
+__device__ __forceinline__ f32x4_t tiny_sum(f32x4_t v, float* lds) {
+    *(f32x4_t*)(lds + 4 * threadIdx.x) = v;
+    __syncthreads();
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    if (threadIdx.x < 64)
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) sum += *(const f32x4_t*)(lds + 4 * (threadIdx.x + 64 * w));
+    return sum;
+}
+
 // Momentum, and partial sums of squares of what is orthogonalised.  In double: a fp32 gradient's square
 // neither overflows nor vanishes there, and a sum of 2^30 of them keeps fp32's precision.
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoTable t, char* work) {
@@ -187,8 +218,13 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __res
         const int r = e / (PREP_TILE / 4), k = (e % (PREP_TILE / 4)) * 4;
         const float row[4] = {tile[r][k], tile[r][k + 1], tile[r][k + 2], tile[r][k + 3]};
         const float col[4] = {tile[k][r], tile[k + 1][r], tile[k + 2][r], tile[k + 3][r]};
-        split_store4(x, x0 + r, y0 + k, q.n, row);
-        split_store4(xt, y0 + r, x0 + k, q.m, col);
+        if (ortho_tiny(q)) {
+            *(f32x4_t*)((float*)x + (int64_t)(x0 + r) * q.n + y0 + k) = (f32x4_t){row[0], row[1], row[2], row[3]};
+            *(f32x4_t*)((float*)xt + (int64_t)(y0 + r) * q.m + x0 + k) = (f32x4_t){col[0], col[1], col[2], col[3]};
+        } else {
+            split_store4(x, x0 + r, y0 + k, q.n, row);
+            split_store4(xt, y0 + r, x0 + k, q.m, col);
+        }
     }
 }
 
@@ -392,6 +428,56 @@ __device__ __forceinline__ void triangle_at(int t, int& i, int& j) {
     j = t - i * (i + 1) / 2;
 }
 
+// The result for row r and column c of X (or of X^T, as G lies), into the caller's matrix.
+__device__ __forceinline__ void ortho_out(const OrthoCall& a, const OrthoMat& q, int row, int col, float v) {
+    const int r = q.tall ? col : row, c = q.tall ? row : col;
+    if (r >= q.rows || c >= q.cols) return;
+    const int64_t at = (int64_t)r * q.cols + c;
+    if (a.muon) q.param[at] = fmaf(-q.lr, v, q.param[at] * a.decay);
+    else store_from_float(q.out, at, v, a.dtype);
+}
+
+// A tile of ortho_product_kernel for a matrix in fp32: the first 16 rows are all there are.
+template <int T, int WAVES, int KIND>
+__device__ __forceinline__ void ortho_tiny_product(const OrthoTable& t, const OrthoMat& q, char* work, char* lds, int ti, int tj, float alpha,
+                                                   float beta, int from) {
+    static_assert(T == 16 * WAVES, "a wave has 16 columns");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = 4 * (lane >> 4);
+    float *X = (float*)(work + q.base), *A = (float*)(work + ortho_a_at(q)), *B = (float*)(work + ortho_b_at(q));
+    if (ti != 0 || ((KIND == ORTHO_GRAM || KIND == ORTHO_POLY) && tj != 0)) return;
+    const int lift = *(const int*)(work + ortho_lift_at(q));
+    if constexpr (KIND == ORTHO_GRAM) {
+        const f32x4_t v = tiny_sum<WAVES>(tiny_product(X, q.n, X, q.n, 16 * wave, 16 * WAVES, q.n), (float*)lds);
+        if (wave == 0)                                         // symmetric: a row for a column
+            *(f32x4_t*)(A + (lane & 15) * q.m + row) = v * ldexpf(beta, -2 * lift);
+    } else if constexpr (KIND == ORTHO_POLY) {
+        if (wave != 0) return;
+        const f32x4_t v = tiny_product(A, q.m, A, q.m, 0, 16, 16), own = *(const f32x4_t*)(A + (lane & 15) * q.m + row);
+        f32x4_t b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = fmaf(beta, v[i], alpha * own[i]);
+        *(f32x4_t*)(B + (lane & 15) * q.m + row) = b;
+    } else {
+        const int col = tj * T + 16 * wave + (lane & 15);
+        const float* XT = (const float*)(work + ortho_xt_at(q, from));
+        const f32x4_t v = tiny_product(B, q.m, XT + (int64_t)(tj * T + 16 * wave) * q.m, q.m, 0, 16, 16);
+        const f32x4_t own = *(const f32x4_t*)(XT + (int64_t)col * q.m + row);
+        const float xa = KIND == ORTHO_LAST ? ldexpf(alpha, -lift) : alpha, xb = KIND == ORTHO_LAST ? ldexpf(beta, -lift) : beta;
+        f32x4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaf(xb, v[i], xa * own[i]);
+        if constexpr (KIND == ORTHO_APPLY) {
+            *(f32x4_t*)((float*)(work + ortho_xt_at(q, from ^ 1)) + (int64_t)col * q.m + row) = x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[(int64_t)(row + i) * q.n + col] = x[i];
+        } else {
+            if (t.call.found_inf && *t.call.found_inf != 0.f) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ortho_out(t.call, q, row + i, col, x[i]);
+        }
+    }
+}
+
 template <int T, int WAVES, int STAGES, int KIND>
 __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTable* __restrict__ t, char* __restrict__ work, float alpha,
                                                                 float beta, int from) {
@@ -409,6 +495,10 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     char* X = work + q.base;
     char* A = work + ortho_a_at(q);
     char* B = work + ortho_b_at(q);
+    if (ortho_tiny(q)) {
+        ortho_tiny_product<T, WAVES, KIND>(*t, q, work, lds, ti, tj, alpha, beta, from);
+        return;
+    }
     const char* P = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : B;
     const char* Q = KIND == ORTHO_GRAM ? X : KIND == ORTHO_POLY ? A : work + ortho_xt_at(q, from);
     const int K = KIND == ORTHO_GRAM ? q.n : q.m;
@@ -465,13 +555,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
                     lines.take(e, v);
                 } else if (!skip) {                            // into the caller's matrix
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = q.tall ? col : row + k, c = q.tall ? row + k : col;
-                        if (r >= q.rows || c >= q.cols) continue;
-                        const int64_t at = (int64_t)r * q.cols + c;
-                        if (a.muon) q.param[at] = fmaf(-q.lr, v[k], q.param[at] * a.decay);
-                        else store_from_float(q.out, at, v[k], a.dtype);
-                    }
+                    for (int k = 0; k < 4; ++k) ortho_out(a, q, row + k, col, v[k]);
                 }
             }
             if constexpr (KIND != ORTHO_LAST) {
@@ -533,6 +617,59 @@ __device__ __forceinline__ float16_t_ small_product(const char* P, int p0, int p
 
 struct OrthoSteps { float coef[3 * ORTHO_MAX_STEPS]; int32_t steps; float sx, sa, sb; };
 
+// What ortho_small_kernel does from there on, for a matrix in fp32.  In LDS: X (16 x n), X^T (n x 16), A and B, rows four values
+// further apart than they are long; and a place for sums.  All of it is zeros.
+__device__ __forceinline__ void ortho_tiny_steps(const OrthoTable& t, const OrthoSteps& c, const OrthoMat& q, char* lds, int lift,
+                                                 double factor, float unscale, bool skip) {
+    constexpr int PITCH = 20;
+    const OrthoCall& a = t.call;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = 64 * SMALL_WAVES, total = q.rows * q.cols;
+    const int xp = q.n + 4, row = 4 * (lane >> 4);
+    float *X = (float*)lds, *XT = X + 16 * xp, *A = XT + q.n * PITCH, *B = A + 16 * PITCH, *sums = B + 16 * PITCH;
+    __syncthreads();                                           // what the norm was put together in is cleared
+    for (int i = tid; i < total; i += threads) {
+        const int r = i / q.cols, k = i - r * q.cols;
+        const float v = (float)(update_at(a, q, i, unscale) * factor);
+        X[(q.tall ? k : r) * xp + (q.tall ? r : k)] = v;
+        XT[(q.tall ? r : k) * PITCH + (q.tall ? k : r)] = v;
+    }
+    __syncthreads();
+    for (int step = 0; step < c.steps; ++step) {
+        const bool last = step == c.steps - 1;
+        const f32x4_t gram = tiny_sum<SMALL_WAVES>(tiny_product(X, xp, X, xp, 16 * wave, 16 * SMALL_WAVES, q.n), sums);
+        if (wave == 0) {                                       // LDS of one wave: no barrier between A and what reads it
+            *(f32x4_t*)(A + (lane & 15) * PITCH + row) = gram * ldexpf(c.sa / (c.sx * c.sx), -2 * lift);
+            __builtin_amdgcn_wave_barrier();
+            const f32x4_t v = tiny_product(A, PITCH, A, PITCH, 0, 16, 16), own = *(const f32x4_t*)(A + (lane & 15) * PITCH + row);
+            const float pa = c.coef[3 * step + 1] * (c.sb / c.sa), pb = c.coef[3 * step + 2] * (c.sb / c.sa / c.sa);
+            f32x4_t b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = fmaf(pb, v[i], pa * own[i]);
+            *(f32x4_t*)(B + (lane & 15) * PITCH + row) = b;
+        }
+        __syncthreads();
+        const float xa = last ? ldexpf(c.coef[3 * step] / c.sx, -lift) : c.coef[3 * step];
+        const float xb = last ? ldexpf(1.0f / (c.sb * c.sx), -lift) : 1.0f / c.sb;
+        for (int c0 = 16 * wave; c0 < q.n; c0 += 16 * SMALL_WAVES) {               // a wave's own rows of X^T and columns of X
+            float* at = XT + (c0 + (lane & 15)) * PITCH + row;
+            const f32x4_t v = tiny_product(B, PITCH, XT + c0 * PITCH, PITCH, 0, 16, 16), own = *(const f32x4_t*)at;
+            f32x4_t x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = fmaf(xb, v[i], xa * own[i]);
+            __builtin_amdgcn_wave_barrier();
+            *(f32x4_t*)at = x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[(row + i) * xp + c0 + (lane & 15)] = x[i];
+        }
+        __syncthreads();
+    }
+    if (skip) return;
+    for (int i = tid; i < total; i += threads) {
+        const int r = i / q.cols, k = i - r * q.cols;
+        ortho_out(a, q, q.tall ? k : r, q.tall ? r : k, X[(q.tall ? k : r) * xp + (q.tall ? r : k)]);
+    }
+}
+
 __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const OrthoTable t, const OrthoSteps c) {
     extern __shared__ __align__(256) char lds[];
     const OrthoMat q = t.mat[blockIdx.x];
@@ -568,6 +705,10 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void ortho_small_kernel(const Ort
     factor = ldexp(factor, lift);
     __syncthreads();
     if (tid < SMALL_WAVES) part[tid] = 0;
+    if (side <= 16) {
+        ortho_tiny_steps(t, c, q, lds, lift, factor, unscale, skip);
+        return;
+    }
     for (int i = tid; i < total; i += threads) {
         const int r = i / q.cols, k = i - r * q.cols;
         const float v = (float)(update_at(a, q, i, unscale) * factor);

@@ -75,6 +75,23 @@ def test_orthogonalize_one_by_one_and_together(ops, dtype):
         check(ops.orthogonalize(m), want, f"{tuple(m.shape)} alone")
 
 
+@pytest.mark.parametrize("with_large", [None, (70, 300), (1100, 1300)])
+def test_orthogonalize_with_a_side_of_up_to_16(ops, with_large):
+    """Kept in fp32 (17 is not): by themselves, and beside matrices that take other tiles; norms far below eps, and a NaN that stays in its matrix."""
+    shapes = [(1, 256), (2, 2), (16, 16), (16, 17), (17, 16), (17, 17), (9, 250), (250, 15)]
+    if with_large:
+        shapes += [with_large, (16, 2048), (2100, 13), (1, 5000)]
+    mats = [matrix(s, i) for i, s in enumerate(shapes)]
+    for m, out in zip(mats, ops.orthogonalize(mats)):
+        check(out, exact(m), str(tuple(m.shape)))
+    faint = [m * 1e-12 for m in mats]
+    for m, out in zip(faint, ops.orthogonalize(faint)):
+        check(out, exact(m), f"faint {tuple(m.shape)}")
+    mats[2][3, 5] = float("nan")
+    for i, (m, out) in enumerate(zip(mats, ops.orthogonalize(mats))):
+        assert bool(torch.isnan(out).all()) if i == 2 else bool(torch.isfinite(out).all()), i
+
+
 def test_orthogonalize_large(ops):
     """Sizes that take the large tiles, neither side a multiple of one."""
     for shape in ((1750, 1665), (1030, 4100)):
