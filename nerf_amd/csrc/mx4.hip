@@ -11,8 +11,8 @@ namespace nerfx {
 
 // ---- to and from -----------------------------------------------------------------------------------------------------
 // Four lanes make a block, eight values each: every load and store of a wave is one run of memory, 16 bytes a lane wherever the
-// row begins (the memory pipes take any address; value by value an odd row length cost eight times the time).  Bound by memory
-// (524,288 x 256 bf16: 5.4 TB/s to, 5.4 TB/s from), as long as nothing but the conversion instructions touches the values: where
+// row begins: the memory pipes take any address (100,000 x 300 bf16 by 301 in all: 194 us value by value, 76 so).  Bound by memory
+// (524,288 x 256 bf16: 56 us either way, 6.1 TB/s), as long as nothing but the conversion instructions touches the values: where
 // rows are whole blocks the matrix is one run, and no division finds the row.
 
 // Part `q`, eight values, begins at `at` of its row; -> its place in memory, row * k + at.  RUN: k is a multiple of 32, every part
@@ -168,7 +168,6 @@ __device__ __forceinline__ float mx4_activate(float v, int activ) {
     return v;
 }
 
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ i32x8_t mx4_operand(u32x4_t c) { return {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0}; }
 
@@ -186,8 +185,8 @@ __device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
 // y from 32 x 32 accumulators (bias included) of rows m0 .. of x and, tile after tile, of neighbouring columns.  A lane holds row
 // m0 + lane % 32 and, with h = lane / 32, columns n0 + 8 q + 4 h + i of it in element 4 q + i: written from there, a store would
 // touch 32 rows with 32 bytes each.  So a wave collects 128 bytes of each of its rows in LDS (one tile of fp32, two of 16 bits,
-// eight of blocks) and writes them as lines (524,288 x 256 by 256 x 256, bf16: 138 -> 114 us).  Rows lie 144 bytes apart there: a phase's
-// sixteen on different banks.
+// eight of blocks) and writes them as lines (524,288 x 256 by 256 x 256, bf16: 138 us without, 114 with).  Rows lie 144 bytes apart
+// there: a phase's sixteen on different banks.
 struct Mx4Lines {
     static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
     char* lds;
@@ -342,6 +341,9 @@ __global__ __launch_bounds__(256) void mx4_prepare_kernel(const Mx4PrepareArgs a
 // (4096 x 4096 by 8192, x in blocks: 93 us by way of registers, 85 so, 3 of them for the order).  Fragments are read one step (64
 // values) ahead of their use.  Rows behind the last one and blocks behind a row's end are read from the last ones: the results of
 // the former are not stored, the codes of the latter are cleared on one side.
+// Bound by its loads: for 4096 x 4096 results 4,096 more of K take 34 us in tiles of 256; 22 of these are the products (6.2 PFLOP/s,
+// all that the instructions do by themselves), without loads it is 25.  LDS holds two stages of that tile; four of 128 x 128 in
+// their place change nothing.
 template <int FP, int WP, int FQ, int WQ, int S>
 struct Mx4Tile {
     static constexpr int WAVES = WP * WQ, TP = 32 * FP * WP, TQ = 32 * FQ * WQ, STAGES = S;
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 // Up to 64 rows of x: the weight is read once and nothing else counts.  A workgroup takes 16 rows of W, its waves parts
 // of K; each lane's 16-byte load is a block of W, which is an operand of the matrix instruction as it
 // is (16 x 16 x 128).  Rows of x in a float type are quantised by the workgroup into LDS, a block a thread, while the first
-// loads of W are on their way.
+// loads of W are on their way (one row by 4096 x 4096: 5.7 us, of which a launch is 3 and 9 MB at 5 TB/s are 2).
 constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024, SKINNY_FLOATS = 128 * 1024;
 
 __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
@@ -602,7 +604,8 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4
 // Up to 256 columns and 512 values a row: a layer of a field for a batch of samples.  Bound by memory: x is read once, in
 // whatever type it has, and y written once.  W stays in LDS (its rows (2 KS + 1) * 16 bytes apart: sixteen rows of a read on
 // sixteen different banks); a wave takes 32 rows of x, a lane two blocks of every 64 values of its row, quantises them in
-// registers, where they are operands of the matrix instruction as they are, and goes over W's columns.
+// registers, where they are operands of the matrix instruction as they are, and goes over W's columns (524,288 x 256 bf16 by 256:
+// 110 us, 4.9 TB/s).
 constexpr int STREAM_WAVES = 8, STREAM_ROWS = 32 * STREAM_WAVES;
 
 __host__ __device__ inline int stream_row_bytes(int ks) { return (2 * ks + 1) * 16; }

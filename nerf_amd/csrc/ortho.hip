@@ -17,6 +17,11 @@
 
 namespace nerfx {
 
+// Four values of a row of the caller's, which begins wherever it begins.
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 f16x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
 constexpr int ORTHO_GROUP = 32;                 // matrices per launch: the table has to fit the kernel arguments
 constexpr int ORTHO_MAX_SIDE = 32768;
 constexpr int ORTHO_MAX_STEPS = 32;
@@ -101,8 +106,8 @@ __device__ __forceinline__ int which_matrix(const OrthoTable& t, int grid, int b
 enum { ORTHO_GRAM, ORTHO_POLY, ORTHO_APPLY, ORTHO_LAST };
 
 // Matrices with a side of up to 16 are kept and multiplied in fp32: sums of so few terms leave nothing for the 2^-23 of two halves to
-// average out in (8 x 60: 6e-7 off float64, in halves 1.0e-6), and there is next to nothing to
-// compute.  X and X^T, A and B take the same places, an element its 4 bytes.
+// average out in (8 x 60: 6e-7 off float64, in halves 1.0e-6), and there is next to nothing to compute.  X and X^T, A and B take
+// the same places, an element its 4 bytes.
 __host__ __device__ inline bool ortho_tiny(const OrthoMat& q) { return (q.rows < q.cols ? q.rows : q.cols) <= 16; }
 
 // 16 rows of P times 16 rows of Q, over values k0, k0 + 1 .. + 15, then step values on, up to K (a multiple of 16): element i of the
@@ -368,6 +373,37 @@ struct SplitTile {
     static __device__ __forceinline__ int col_of(int wave) { return wave % (WAVES / 2) * (2 * T / WAVES); }
 };
 
+// The result for X's row and column, into the caller's matrix.
+__device__ __forceinline__ void ortho_out(const OrthoCall& a, const OrthoMat& q, int row, int col, float v) {
+    const int r = q.tall ? col : row, c = q.tall ? row : col;
+    if (r >= q.rows || c >= q.cols) return;
+    const int64_t at = (int64_t)r * q.cols + c;
+    if (a.muon) q.param[at] = fmaf(-q.lr, v, q.param[at] * a.decay);
+    else store_from_float(q.out, at, v, a.dtype);
+}
+// Those for four neighbours in the caller's row r: 16 bytes, wherever the row begins.
+__device__ __forceinline__ void ortho_out4(const OrthoCall& a, const OrthoMat& q, int r, int c, f32x4_t v) {
+    const int64_t at = (int64_t)r * q.cols + c;
+    if (c + 4 > q.cols) {
+        for (int i = 0; c + i < q.cols; ++i) {
+            if (a.muon) q.param[at + i] = fmaf(-q.lr, v[i], q.param[at + i] * a.decay);
+            else store_from_float(q.out, at + i, v[i], a.dtype);
+        }
+    } else if (a.muon) {
+        f32x4_any_t* p = (f32x4_any_t*)(q.param + at);
+        f32x4_any_t w = *p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = fmaf(-q.lr, v[i], w[i] * a.decay);
+        *p = w;
+    } else if (a.dtype == NERFX_TYPE_F32) {
+        *(f32x4_any_t*)((float*)q.out + at) = v;
+    } else if (a.dtype == NERFX_TYPE_F16) {
+        *(f16x4_any_t*)((_Float16*)q.out + at) = (f16x4_any_t){(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    } else {
+        *(bf16x4_any_t*)((__bf16*)q.out + at) = (bf16x4_any_t){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    }
+}
+
 // A wave's 32 x 32 results on their way to a split matrix and to its transpose.  They go through LDS, one orientation after the
 // other, and leave as whole lines of 128 bytes: stored from the registers, in pieces of 2 and 8 bytes, they were a quarter of a
 // small matrix's time (a field's six: 129 us, 122 so).
@@ -409,6 +445,27 @@ struct SplitLines {
         leave(dst, row, col, width);
     }
 
+    // The same for the caller's matrix, in fp32 and as that lies.
+    __device__ __forceinline__ void take_out(int e, const float (&v)[4], bool tall) {
+        const int lane = threadIdx.x & 63, row = 8 * e + 4 * (lane >> 5);
+        if (tall) {
+            *(f32x4_t*)(lds + (lane & 31) * PITCH + 4 * row) = (f32x4_t){v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *(float*)(lds + (row + k) * PITCH + 4 * (lane & 31)) = v[k];
+        }
+    }
+    // row, col: of X.
+    __device__ __forceinline__ void leave_out(const OrthoCall& a, const OrthoMat& q, int row, int col) const {
+        const int lane = threadIdx.x & 63, c = (q.tall ? row : col) + 4 * (lane & 7);
+        if (c >= q.cols) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = 8 * i + (lane >> 3), r = (q.tall ? col : row) + at;
+            if (r < q.rows) ortho_out4(a, q, r, c, *(const f32x4_t*)(lds + at * PITCH + 16 * (lane & 7)));
+        }
+    }
+
 private:
     __device__ __forceinline__ void leave(char* dst, int row, int col, int width) const {
         const int lane = threadIdx.x & 63;
@@ -426,15 +483,6 @@ __device__ __forceinline__ void triangle_at(int t, int& i, int& j) {
     while (i * (i + 1) / 2 > t) --i;
     while ((i + 1) * (i + 2) / 2 <= t) ++i;
     j = t - i * (i + 1) / 2;
-}
-
-// The result for row r and column c of X (or of X^T, as G lies), into the caller's matrix.
-__device__ __forceinline__ void ortho_out(const OrthoCall& a, const OrthoMat& q, int row, int col, float v) {
-    const int r = q.tall ? col : row, c = q.tall ? row : col;
-    if (r >= q.rows || c >= q.cols) return;
-    const int64_t at = (int64_t)r * q.cols + c;
-    if (a.muon) q.param[at] = fmaf(-q.lr, v, q.param[at] * a.decay);
-    else store_from_float(q.out, at, v, a.dtype);
 }
 
 // A tile of ortho_product_kernel for a matrix in fp32: the first 16 rows are all there are.
@@ -530,7 +578,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
     }
     const OrthoCall a = t->call;
     const bool skip = KIND == ORTHO_LAST && a.found_inf && *a.found_inf != 0.f;
-    if constexpr (KIND != ORTHO_LAST) __syncthreads();                   // the stages have been read: their place is the waves' own now
+    __syncthreads();                                                     // the stages have been read: their place is the waves' own now
     SplitLines lines{lds + wave * SplitLines::BYTES};
     static_assert(WAVES * SplitLines::BYTES <= Tile::LDS_BYTES, "a place for each wave");
 #pragma unroll
@@ -541,7 +589,6 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
             const int col = tj * T + Tile::col_of(wave) + 32 * j + (lane & 31);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = row0 + 8 * e;
                 float v[4];
                 if constexpr (KIND == ORTHO_GRAM) {
 #pragma unroll
@@ -551,12 +598,11 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
                     for (int k = 0; k < 4; ++k)
                         v[k] = fmaf(beta, tile.acc[i][j][4 * e + k], alpha * ((float)own[i][j][e].hi[k] + (float)own[i][j][e].lo[k]));
                 }
-                if constexpr (KIND != ORTHO_LAST) {
-                    lines.take(e, v);
-                } else if (!skip) {                            // into the caller's matrix
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) ortho_out(a, q, row + k, col, v[k]);
-                }
+                if constexpr (KIND != ORTHO_LAST) lines.take(e, v);
+                else lines.take_out(e, v, q.tall);
+            }
+            if constexpr (KIND == ORTHO_LAST) {                // into the caller's matrix
+                if (!skip) lines.leave_out(a, q, row0 - 4 * (lane >> 5), col - (lane & 31));
             }
             if constexpr (KIND != ORTHO_LAST) {
                 const int r = row0 - 4 * (lane >> 5), c = col - (lane & 31);
@@ -570,7 +616,7 @@ __global__ __launch_bounds__(64 * WAVES) void ortho_product_kernel(const OrthoTa
 // ---- small matrices: one launch ---------------------------------------------------------------------------------------
 // A matrix whose smaller side is at most 64 and whose larger one is at most 256 fits in LDS with everything that the steps
 // need (X, X^T, A and B: 160 KB), so that a workgroup takes all of its steps by itself.  What bounds the other way there is
-// the number of launches: 17 of 5 us each.  Only for groups of nothing but such matrices; in a group with a larger one they
+// the number of launches: 17 of 6 us each.  Only for groups of nothing but such matrices; in a group with a larger one they
 // ride along in its launches.
 //
 // A row takes 128 bytes for every 32 of its columns, as in memory; 16-byte chunk c (of a pair of blocks: 0 .. 15) of row r lies at
@@ -886,10 +932,11 @@ static int64_t lay_out(OrthoTable& t, int grid, F blocks_of) {
 
 // The tile a product takes, by how many of them there are:
 //  128  where whole rounds of them fill at least four fifths of the 256 CUs: half of the operand traffic of 64
-//       (2048 x 2048 by 2048: 50 us; 55 in tiles of 64);
-//  64   with two stages, five workgroups to a CU, where they would not: of a symmetric result 136 tiles of 128 take as long as
-//       all 256 (50 us), 528 of 64 take 41; three and four stages hold fewer workgroups and take 44 and 50;
-//  64   with eight stages where there is at most one to a CU: all of a K of 256 is on its way at once.
+//       (2048 x 2048 by 2048: 57 us; 67 in tiles of 64);
+//  64   with two stages, four workgroups to a CU, where they would not: a symmetric result's 136 tiles of 128 take 46 us, 528 of
+//       64 take 39; three stages hold fewer workgroups and take 43;
+//  64   with eight stages where there is at most one to a CU: all of a K of 256 is on its way at once (a field's six matrices in
+//       all: 112 us, 119 with two).
 enum { ORTHO_TILE_128, ORTHO_TILE_64, ORTHO_TILE_64_DEEP };
 struct OrthoShape { int kind; int64_t blocks; };
 static OrthoShape choose(OrthoTable& t, int grid, int pad) {
