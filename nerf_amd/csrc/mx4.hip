@@ -182,6 +182,12 @@ __device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
     else if (activ == NERFX_ACT_SILU) each([](float x) { return mx4_activate(x, NERFX_ACT_SILU); });
 }
 
+__device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, int64_t at, float v) {
+    if (a.y_dtype == NERFX_TYPE_F32) ((float*)a.y)[at] = v;
+    else if (a.y_dtype == NERFX_TYPE_BF16) ((__bf16*)a.y)[at] = (__bf16)v;
+    else ((_Float16*)a.y)[at] = (_Float16)v;
+}
+
 // y from 32 x 32 accumulators (bias included) of rows m0 .. of x and, tile after tile, of neighbouring columns.  A lane holds row
 // m0 + lane % 32 and, with h = lane / 32, columns n0 + 8 q + 4 h + i of it in element 4 q + i: written from there, a store would
 // touch 32 rows with 32 bytes each.  So a wave collects 128 bytes of each of its rows in LDS (one tile of fp32, two of 16 bits,
@@ -189,6 +195,7 @@ __device__ __forceinline__ void mx4_activate16(float (&v)[16], int activ) {
 // there: a phase's sixteen on different banks.
 struct Mx4Lines {
     static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
+    static constexpr int FEW = 4;
     char* lds;
     int begin = 0, end = 0;                                    // bytes of y's rows that are collected
 
@@ -200,7 +207,15 @@ struct Mx4Lines {
         for (int e = 0; e < 16; ++e) v[e] = acc[e];
         mx4_activate16(v, a.activ);
         char* row = lds + (lane & 31) * PITCH;
-        if (a.y_dtype == NERFX_TYPE_MX4) {                     // the tile's 32 columns are a block of y
+        int to, row_bytes;                                     // bytes of a row that are there with this tile, and of all of it
+        if (a.n <= FEW && a.y_dtype != NERFX_TYPE_MX4) {       // heads: next to nothing to write
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int n = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
+                if (8 * (e >> 2) < FEW && m < a.m && n < a.n) mx4_store(a, m * a.n + n, v[e]);
+            }
+            return;
+        } else if (a.y_dtype == NERFX_TYPE_MX4) {                     // the tile's 32 columns are a block of y
             using Raw = Mx4Raw<NERFX_TYPE_F32, 16>;
             Raw raw;
 #pragma unroll
@@ -217,12 +232,14 @@ struct Mx4Lines {
             if (h == 0 && m < a.m) a.y_scales[m * mx4_blocks(a.n) + n0 / MX4_BLOCK] = (uint8_t)byte;
             open(n0 / 2);
             *(u32x2_t*)(row + n0 / 2 - begin + 8 * h) = w;
-            close(a, m0, n0 / 2 + 16, mx4_blocks(a.n) * 16);
+            to = n0 / 2 + 16;
+            row_bytes = mx4_blocks(a.n) * 16;
         } else if (a.y_dtype == NERFX_TYPE_F32) {
             open(4 * n0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) *(f32x4_t*)(row + 32 * q + 16 * h) = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            close(a, m0, 4 * n0 + 128, 4 * a.n);
+            to = 4 * n0 + 128;
+            row_bytes = 4 * a.n;
         } else {
             // two 16-bit values a word; word 2 q + p holds columns 8 q + 4 h + 2 p, + 1
             uint32_t w[8];
@@ -243,31 +260,36 @@ struct Mx4Lines {
             open(2 * n0);
             *(u32x4_t*)(row + 2 * n0 - begin + 32 * h) = {w[0], w[1], w[4], w[5]};
             *(u32x4_t*)(row + 2 * n0 - begin + 32 * h + 16) = {w[2], w[3], w[6], w[7]};
-            close(a, m0, 2 * n0 + 64, 2 * a.n);
+            to = 2 * n0 + 64;
+            row_bytes = 2 * a.n;
         }
+        end = to;
+        if (end - begin == 128 || end >= row_bytes) flush(a, m0, row_bytes);   // lines are there, or the rows end
     }
 
 private:
     __device__ __forceinline__ void open(int at) { if (end == 0) begin = at; }
-    // Bytes up to `to` are there: out with them, if they make lines or the rows (of row_bytes) end.
-    __device__ __forceinline__ void close(const Mx4LinearArgs& a, int64_t m0, int to, int row_bytes) {
-        end = to;
-        if (to - begin == 128 || to >= row_bytes) flush(a, m0, row_bytes);
-    }
-
 public:
     // Also needed behind the last tile of some columns, where they end in the middle of a row's line.
     __device__ __forceinline__ void flush(const Mx4LinearArgs& a, int64_t m0, int row_bytes) {
         const int lane = threadIdx.x & 63, at = begin + 16 * (lane & 7);
         const int there = min(end, row_bytes) - at;            // bytes of this lane's piece
+        u32x4_t piece[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) piece[i] = *(const u32x4_t*)(lds + (8 * i + (lane >> 3)) * PITCH + 16 * (lane & 7));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = 8 * i + (lane >> 3);
-            const char* piece = lds + r * PITCH + 16 * (lane & 7);
-            char* y = (char*)a.y + (m0 + r) * row_bytes + at;
-            if (m0 + r >= a.m) continue;
-            if (there >= 16) *(u32x4_any_t*)y = *(const u32x4_t*)piece;
-            else for (int c = 0; c < there; c += 2) *(uint16_t*)(y + c) = *(const uint16_t*)(piece + c);
+            const int64_t m = m0 + 8 * i + (lane >> 3);
+            if (m < a.m && there >= 16) *(u32x4_any_t*)((char*)a.y + m * row_bytes + at) = piece[i];
+        }
+        if ((min(end, row_bytes) - begin) % 16 != 0) {         // rows that end in the middle of one
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const int64_t m = m0 + 8 * i + (lane >> 3);
+                const char* left = lds + (8 * i + (lane >> 3)) * PITCH + 16 * (lane & 7);
+                if (m < a.m && there < 16)
+                    for (int c = 0; c < there; c += 2) *(uint16_t*)((char*)a.y + m * row_bytes + at + c) = *(const uint16_t*)(left + c);
+            }
         }
         end = 0;
     }
@@ -511,11 +533,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024, SKINNY_FLOATS = 128 * 1024;
 
 __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
-    const float v = mx4_activate(acc + (a.bias ? a.bias[n] : 0.f), a.activ);
-    const int64_t at = m * a.n + n;
-    if (a.y_dtype == NERFX_TYPE_F32) ((float*)a.y)[at] = v;
-    else if (a.y_dtype == NERFX_TYPE_BF16) ((__bf16*)a.y)[at] = (__bf16)v;
-    else ((_Float16*)a.y)[at] = (_Float16)v;
+    mx4_store(a, m * a.n + n, mx4_activate(acc + (a.bias ? a.bias[n] : 0.f), a.activ));
 }
 
 template <int DT, int MT>
