@@ -11,7 +11,7 @@ namespace nerfx {
 
 // ---- to and from -----------------------------------------------------------------------------------------------------
 // Four lanes make a block, eight values each: every load and store of a wave is one run of memory, 16 bytes a lane wherever the
-// row begins: the memory pipes take any address (100,000 x 300 bf16 by 301 in all: 194 us value by value, 76 so).  Bound by memory
+// row begins: the memory pipes take any address (100,000 x 300 bf16 by 301, both ways: 194 us value by value, 76 so).  Bound by memory
 // (524,288 x 256 bf16: 56 us either way, 6.1 TB/s), as long as nothing but the conversion instructions touches the values: where
 // rows are whole blocks the matrix is one run, and no division finds the row.
 
@@ -195,7 +195,7 @@ __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, int64_t at, fl
 // there: a phase's sixteen on different banks.
 struct Mx4Lines {
     static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
-    static constexpr int FEW = 4;
+    static constexpr int FEW = 4;                              // 1M x 3 fp32: 26 us from the registers, 38 by way of LDS; x 8: 49 and 41
     char* lds;
     int begin = 0, end = 0;                                    // bytes of y's rows that are collected
 
@@ -623,7 +623,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4
 // whatever type it has, and y written once.  W stays in LDS (its rows (2 KS + 1) * 16 bytes apart: sixteen rows of a read on
 // sixteen different banks); a wave takes 32 rows of x, a lane two blocks of every 64 values of its row, quantises them in
 // registers, where they are operands of the matrix instruction as they are, and goes over W's columns (524,288 x 256 bf16 by 256:
-// 110 us, 4.9 TB/s).
+// 112 us, 4.8 TB/s).
 constexpr int STREAM_WAVES = 8, STREAM_ROWS = 32 * STREAM_WAVES;
 
 __host__ __device__ inline int stream_row_bytes(int ks) { return (2 * ks + 1) * 16; }
@@ -785,10 +785,10 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //          tiles; 32 x 2048 bf16 by 256: 7 and 8.5), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
 //          Not for a result in blocks, which are of 32 columns;
 //  stream  otherwise up to 256 values a row, or 512 and up to 256 columns: float rows are quantised in registers, once for every
-//          256 columns (16,384 x 4096 by 128: 40 us, 54 with tiles; by 512: 82, and 69 with tiles);
+//          256 columns (16,384 x 4096 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles);
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
 //          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit): a small product lasts as
-//          long as one tile does (256 x 4096 by 4096: 13 us, 21 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 28 and 27);
+//          long as one tile does (256 x 4096 by 4096: 13 us, 19 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 27 and 24);
 //          else 128 x 128.
 enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
 // Steps of 64 values that a row is worked on in: what the stream kernel is made for.
