@@ -935,9 +935,11 @@ static int64_t lay_out(OrthoTable& t, int grid, F blocks_of) {
 //       (2048 x 2048 by 2048: 57 us; 67 in tiles of 64);
 //  64   with two stages, four workgroups to a CU, where they would not: a symmetric result's 136 tiles of 128 take 46 us, 528 of
 //       64 take 39; three stages hold fewer workgroups and take 43;
+//  64   with four stages where there are at most two to a CU, which is what LDS holds then: nothing but stages ahead hides
+//       the way of a load there (408 tiles, K up to 2048: 32 us, 38 with two);
 //  64   with eight stages where there is at most one to a CU: all of a K of 256 is on its way at once (a field's six matrices in
 //       all: 112 us, 119 with two).
-enum { ORTHO_TILE_128, ORTHO_TILE_64, ORTHO_TILE_64_DEEP };
+enum { ORTHO_TILE_128, ORTHO_TILE_64, ORTHO_TILE_64_MORE, ORTHO_TILE_64_DEEP };
 struct OrthoShape { int kind; int64_t blocks; };
 static OrthoShape choose(OrthoTable& t, int grid, int pad) {
     auto blocks = [&](int tile) {
@@ -951,7 +953,7 @@ static OrthoShape choose(OrthoTable& t, int grid, int pad) {
         if (big * 5 >= (big + 255) / 256 * 256 * 4) return {ORTHO_TILE_128, big};
     }
     const int64_t small = blocks(64);
-    return {small <= 256 ? ORTHO_TILE_64_DEEP : ORTHO_TILE_64, small};
+    return {small <= 256 ? ORTHO_TILE_64_DEEP : small <= 512 ? ORTHO_TILE_64_MORE : ORTHO_TILE_64, small};
 }
 
 template <int T, int WAVES, int STAGES, int KIND>
@@ -966,6 +968,7 @@ template <int KIND>
 static int product(const OrthoShape& s, char* work, float alpha, float beta, int from, hipStream_t stream) {
     if (s.kind == ORTHO_TILE_128) return product_as<128, 8, 4, KIND>(s.blocks, work, alpha, beta, from, stream);
     if (s.kind == ORTHO_TILE_64) return product_as<64, 4, 2, KIND>(s.blocks, work, alpha, beta, from, stream);
+    if (s.kind == ORTHO_TILE_64_MORE) return product_as<64, 4, 4, KIND>(s.blocks, work, alpha, beta, from, stream);
     return product_as<64, 4, 8, KIND>(s.blocks, work, alpha, beta, from, stream);
 }
 

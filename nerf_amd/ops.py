@@ -1,6 +1,7 @@
 """Tensor-level wrappers over the C ABI: validate, allocate outputs with torch,
 pass raw device pointers and the current HIP stream.  No arithmetic happens here.
 """
+import bisect
 import contextlib
 import ctypes as C
 import functools
@@ -829,7 +830,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
 
     lr' = lr * sqrt(max(1, rows / cols)) ("original") or lr * 0.2 sqrt(max(rows, cols)) ("match_rms_adamw").
     Where `found_inf` (one device float) is not zero nothing changes.  `params` and `momenta` are contiguous fp32
-    tensors that share no memory; all matrices share the launches and none of them waits for the host."""
+    tensors that share no memory, with each other or with `grads`; all matrices share the launches and none of them waits for the host."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_step: params, grads and momenta pair up")
@@ -855,9 +856,12 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     spans.sort()
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise RuntimeError("muon_step: two of `params` and `momenta` share memory")
-    held = {m.data_ptr() for m in momenta if m.numel()}
-    if any(g.data_ptr() in held for g in grads):
-        raise RuntimeError("muon_step: a gradient is one of the `momenta`, which are written first")
+    starts = [a for a, _ in spans]
+    for g in grads:
+        if g.numel() and g.is_contiguous():                 # any other is copied below
+            k = bisect.bisect_left(starts, g.data_ptr() + 4 * g.numel()) - 1
+            if k >= 0 and spans[k][1] > g.data_ptr():
+                raise RuntimeError("muon_step: a gradient shares memory with `params` or `momenta`, which are written")
     for name, t in (("grad_scale", grad_scale), ("found_inf", found_inf)):
         if t is not None and not (t.is_cuda and t.device == dev and t.dtype == torch.float32 and t.numel() == 1):
             raise RuntimeError(f"muon_step: `{name}` must be one fp32 element on {dev}")

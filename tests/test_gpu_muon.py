@@ -99,6 +99,22 @@ def test_orthogonalize_large(ops):
         check(ops.orthogonalize(m), exact(m), str(shape))
 
 
+def test_orthogonalize_past_32_bits(ops):
+    """A workspace of more than 2^32 bytes: two blocks in far corners of zeros are what they are next to each other."""
+    a, b = matrix((300, 200), 21), matrix((130, 260), 22)
+    near = torch.zeros(430, 460, device="cuda")
+    far = torch.zeros(17000, 16500, device="cuda")
+    for m in (near, far):
+        m[:300, :200] = a
+        m[-130:, -260:] = b
+    want, got = exact(near), ops.orthogonalize(far)
+    check(got[:300, :200], want[:300, :200], "the first block")
+    check(got[-130:, -260:], want[-130:, -260:], "the last block")
+    got[:300, :200] = 0
+    got[-130:, -260:] = 0
+    assert not bool(got.any())
+
+
 def test_orthogonalize_structures(ops):
     stack = torch.stack([matrix((40, 70), i) for i in range(3)])
     out = ops.orthogonalize(stack)
@@ -219,7 +235,10 @@ def test_muon_step(ops, nesterov, decay, rule):
 def test_muon_step_refuses(ops):
     w, g, m = (matrix((8, 6), i) for i in range(3))
     big = matrix((16, 6), 3)
-    for args in (([w], [g], [w]), ([w], [m], [m]), ([w], [g], [m.half()]), ([w], [g.t()], [m]), ([w], [g[0]], [m]), ([w.t()], [g.t()], [m.t().contiguous()]),
+    ends_in, begins_in = big[4:12], m.new_zeros(16, 6)
+    over = begins_in[:8]
+    for args in (([w], [g], [w]), ([w], [m], [m]), ([w], [w], [m]), ([big[:8]], [ends_in], [m]), ([w], [begins_in[3:11]], [over]),
+                 ([w], [g], [m.half()]), ([w], [g.t()], [m]), ([w], [g[0]], [m]), ([w.t()], [g.t()], [m.t().contiguous()]),
                  ([w, w], [g, g], [m, m.clone()]), ([big[:8], big[4:12]], [g, g], [m, m.clone()]), ([w.cpu()], [g], [m])):
         before = [t.clone() for t in (w, m, big)]
         with pytest.raises(RuntimeError):

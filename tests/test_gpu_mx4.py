@@ -292,6 +292,23 @@ def test_linear_from_and_to_any_place(ops, dtype, m, n, k):
         assert torch.equal(q.scales, ops.mx4_quantize(x).scales) and torch.equal(q.codes, ops.mx4_quantize(x).codes), at
 
 
+@pytest.mark.parametrize("m,n,k", [(9_000_000, 256, 64), (9_000_000, 257, 33), (280_000, 8200, 290)])
+def test_linear_past_32_bits(ops, m, n, k):
+    """Results of more than 2^32 bytes: the last rows are those of a call of their own."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(m, k, generator=g, device="cuda").to(torch.bfloat16)
+    w = ops.mx4_quantize(torch.randn(n, k, generator=g, device="cuda"))
+    y = ops.mx4_linear(x, w, None, "relu")
+    for rows in (slice(m - 3000, m), slice(m // 2 - 11, m // 2 + 2989), slice(0, 3000)):
+        assert torch.equal(y[rows], ops.mx4_linear(x[rows].clone(), w, None, "relu"))
+    del y
+    q = ops.mx4_quantize(x)
+    back = q.dequantize(torch.bfloat16)
+    tail = ops.mx4_quantize(x[m - 3000:].clone())
+    assert torch.equal(q.codes[m - 3000:], tail.codes) and torch.equal(q.scales[m - 3000:], tail.scales)
+    assert torch.equal(back[m - 3000:], tail.dequantize(torch.bfloat16))
+
+
 def test_linear_refuses(ops):
     x, w, bias = pair(4, 8, 64, torch.float32, 6)
     qw = ops.mx4_quantize(w)
@@ -332,3 +349,21 @@ def test_linear_on_streams_and_in_graphs(ops):
             torch.cuda.synchronize()
             want = ops.mx4_linear(x, qw, bias, "silu")
             assert torch.equal(got, want) and torch.equal(back, ops.mx4_quantize(want).dequantize()), f"replay {i}"
+
+
+def test_two_products_of_one_weight_at_once(ops):
+    """Workspaces are each call's own: two streams go over the same weight with inputs of their own."""
+    x, w, bias = pair(700, 900, 600, torch.float32, 9)
+    qw = ops.mx4_quantize(w)
+    inputs = [x, x.flip(0).contiguous()]
+    want = [ops.mx4_linear(v, qw, bias, "silu") for v in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, side in enumerate(streams):
+            with torch.cuda.stream(side):
+                got[i].append(ops.mx4_linear(inputs[i], qw, bias, "silu"))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
