@@ -5,6 +5,7 @@ import bisect
 import contextlib
 import ctypes as C
 import functools
+import math
 import struct
 import weakref
 from typing import Optional, Tuple
@@ -735,9 +736,12 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _AS_IT_IS = contextlib.nullcontext()
 
 
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # without the look whether torch is ready
+
+
 def _on(dev):
-    """torch.cuda.device(dev), or nothing where that is the current one."""
-    return _AS_IT_IS if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    """torch.cuda.device(dev), or nothing where that is the current one.  (There is a tensor on `dev`: torch is ready.)"""
+    return _AS_IT_IS if _CURRENT_DEVICE() == dev.index else torch.cuda.device(dev)
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object around it
@@ -899,12 +903,12 @@ class Mx4:
         self.codes, self.scales, self.k = codes, scales, k
 
     @classmethod
-    def _new(cls, rows: int, k: int, dev) -> "Mx4":
-        """An unwritten one."""
+    def _new(cls, rows: int, k: int, like: Tensor) -> "Mx4":
+        """An unwritten one, where `like` is."""
         self = object.__new__(cls)
         blocks = (k + 31) // 32
-        self.codes = torch.empty((rows, 16 * blocks), device=dev, dtype=torch.uint8)
-        self.scales = torch.empty((rows, blocks), device=dev, dtype=torch.uint8)
+        self.codes = like.new_empty((rows, 16 * blocks), dtype=torch.uint8)
+        self.scales = self.codes.new_empty((rows, blocks))
         self.k = k
         return self
 
@@ -934,7 +938,7 @@ class Mx4:
             raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {self.codes.device}")
         codes, dev = self.codes, self.codes.device
         rows = codes.shape[0]
-        out = torch.empty((rows, self.k), device=dev, dtype=dtype)
+        out = codes.new_empty((rows, self.k), dtype=dtype)
         with _on(dev):
             check(lib.nerfx_mx4_dequantize(codes.data_ptr(), self.scales.data_ptr(), rows, self.k, _TYPES[dtype], out.data_ptr(),
                                            _stream_on(dev)))
@@ -952,7 +956,7 @@ def _mx4_input(x: Tensor, name: str) -> Tensor:
         raise ValueError(f"{name}: the last dimension must hold 1..2^20 values (got {tuple(x.shape)})")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"4-bit numbers carry no gradient: detach `{name}` or call under no_grad")
-    return x.detach().contiguous()
+    return x if x.is_contiguous() else x.detach().contiguous()
 
 
 def mx4_quantize(x: Tensor) -> Mx4:
@@ -963,7 +967,7 @@ def mx4_quantize(x: Tensor) -> Mx4:
         raise ValueError(f"mx4_quantize takes a matrix (got shape {tuple(x.shape)})")
     rows, k = x.shape
     dev = x.device
-    out = Mx4._new(rows, k, dev)
+    out = Mx4._new(rows, k, x)
     with _on(dev):
         check(lib.nerfx_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, out.codes.data_ptr(), out.scales.data_ptr(),
                                      _stream_on(dev)))
@@ -998,18 +1002,17 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
             raise RuntimeError("4-bit numbers carry no gradient: detach `bias` or call under no_grad")
         if tuple(bias.shape) != (n,) or bias.device != dev:
             raise ValueError(f"bias must be ({n},) on {dev}")
-        bias = _dev(bias.detach(), "bias")
-    m = 1
-    for s in lead:
-        m *= s
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().to(torch.float32).contiguous()
+    m = math.prod(lead)
     if out_dtype == "mx4":
-        out = Mx4._new(m, n, dev)
+        out = Mx4._new(m, n, src)
         y, y_scales, yt = out.codes, out.scales, _lib.TYPE_MX4
     else:
         out_dtype = default if out_dtype is None else out_dtype
         if out_dtype not in _TYPES:
             raise TypeError(f"mx4_linear gives fp32, bf16, fp16 or \"mx4\" (asked for {out_dtype})")
-        out = y = torch.empty((*lead, n), device=dev, dtype=out_dtype)
+        out = y = src.new_empty((*lead, n), dtype=out_dtype)
         y_scales, yt = None, _TYPES[out_dtype]
     need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt, yt)
     ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
