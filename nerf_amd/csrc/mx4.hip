@@ -15,44 +15,56 @@ namespace nerfx {
 // (524,288 x 256 bf16: 56 us either way, 6.1 TB/s), as long as nothing but the conversion instructions touches the values: where
 // rows are whole blocks the matrix is one run, and no division finds the row.
 
-// Part `q`, eight values, begins at `at` of its row; -> its place in memory, row * k + at.  RUN: k is a multiple of 32, every part
+// Part `q`, N values, begins at `at` of its row; -> its place in memory, row * k + at.  RUN: k is a multiple of 32, every part
 // is whole and the row is of no interest.
-template <bool RUN>
+template <bool RUN, int N>
 __device__ __forceinline__ int64_t mx4_place(uint64_t q, int k, int& at) {
     at = 0;
-    if constexpr (RUN) return (int64_t)q * 8;
-    const uint32_t nb = mx4_blocks(k);
-    const uint64_t block = q >> 2, row = block >> 32 ? block / nb : (uint32_t)block / nb;
-    at = (int)(block - row * nb) * MX4_BLOCK + (int)(q & 3) * 8;
+    if constexpr (RUN) return (int64_t)q * N;
+    const uint32_t nb = mx4_blocks(k), parts = MX4_BLOCK / N;
+    const uint64_t block = q / parts, row = block >> 32 ? block / nb : (uint32_t)block / nb;
+    at = (int)(block - row * nb) * MX4_BLOCK + (int)(q % parts) * N;
     return (int64_t)row * k + at;
 }
 
-// N values (a multiple of 8, at most 32) from `row + at` on: all there, or zeros behind k.
-template <int DT, int N>
+// N values (a multiple of 8, at most 32) from `row + at` on: all there, or zeros behind k.  ODD: 16-bit rows may begin in the middle
+// of a word, where the pipes are half as fast (260,000 x 3 bf16 by 295: 51 us); read are then the words that hold a value, one more
+// of them if the first begins with half of one, and moved.
+template <int DT, int N, bool ODD>
 __device__ __forceinline__ Mx4Raw<DT, N> mx4_load_whole(const char* row, int at) {
+    constexpr int WORDS = Mx4Raw<DT, N>::WORDS;
+    const char* from = row + (int64_t)at * (DT == NERFX_TYPE_F32 ? 4 : 2);
+    const uint32_t half = ODD ? (uint32_t)(uintptr_t)from & 2 : 0;
+    from -= half;
     Mx4Raw<DT, N> v;
 #pragma unroll
-    for (int i = 0; i < Mx4Raw<DT, N>::WORDS / 4; ++i) {
-        const u32x4_t w = *(const u32x4_any_t*)(row + (int64_t)at * (DT == NERFX_TYPE_F32 ? 4 : 2) + 16 * i);
+    for (int i = 0; i < WORDS / 4; ++i) {
+        const u32x4_t w = *(const u32x4_any_t*)(from + 16 * i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v.w[4 * i + j] = w[j];
     }
+    if constexpr (ODD) {
+        const uint32_t last = *(const uint32_t*)(from + 4 * WORDS - (half ? 0 : 4));
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) v.w[i] = __builtin_amdgcn_alignbit(i + 1 < WORDS ? v.w[i + 1] : last, v.w[i], 8 * half);
+    }
     return v;
 }
+static bool mx4_odd(const void* x, int k, int dtype) { return dtype != NERFX_TYPE_F32 && ((k & 1) || ((uintptr_t)x & 3)); }
 
 // A row's last values, fewer than N, are read as its last N and moved down: one by one each would be waited for.
-template <int DT, int N>
+template <int DT, int N, bool ODD>
 __device__ __forceinline__ Mx4Raw<DT, N> mx4_load(const char* row, int at, int k) {
     using Raw = Mx4Raw<DT, N>;
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
     Raw v;
     if (at + N <= k) {
-        v = mx4_load_whole<DT, N>(row, at);
+        v = mx4_load_whole<DT, N, ODD>(row, at);
     } else if (at >= k) {
 #pragma unroll
         for (int i = 0; i < Raw::WORDS; ++i) v.w[i] = 0u;
     } else if (k >= N) {
-        v = mx4_load_whole<DT, N>(row, k - N);
+        v = mx4_load_whole<DT, N, ODD>(row, k - N);
         const int down = N - k % N;                            // the same for every lane
         if (SIZE == 2 && (down & 1)) {
 #pragma unroll
@@ -81,16 +93,19 @@ __device__ __forceinline__ Mx4Raw<DT, N> mx4_load(const char* row, int at, int k
     return v;
 }
 
+// Rows of whole blocks, one run of memory; others; others that may begin in the middle of a word.
+enum { MX4_RUN, MX4_ANY, MX4_ODD };
+
 // Part q's codes are stored, `scale(byte)` stores its block's scale.
-template <int DT, bool RUN, class Scale>
+template <int DT, int ROWS, class Scale>
 __device__ __forceinline__ void mx4_quantize_part(const void* x, int64_t q, int k, uint32_t* codes, Scale scale) {
     using Raw = Mx4Raw<DT, 8>;
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
     int at;
-    const int64_t place = mx4_place<RUN>(q, k, at);
+    const int64_t place = mx4_place<ROWS == MX4_RUN, 8>(q, k, at);
     Raw v;
-    if constexpr (RUN) v = mx4_load_whole<DT, 8>((const char*)x + place * SIZE, 0);
-    else v = mx4_load<DT, 8>((const char*)x + (place - at) * SIZE, at, k);
+    if constexpr (ROWS == MX4_RUN) v = mx4_load_whole<DT, 8, false>((const char*)x + place * SIZE, 0);
+    else v = mx4_load<DT, 8, ROWS == MX4_ODD>((const char*)x + (place - at) * SIZE, at, k);
     uint32_t top = v.top_bits();
     top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
@@ -99,50 +114,48 @@ __device__ __forceinline__ void mx4_quantize_part(const void* x, int64_t q, int 
     if ((q & 3) == 0) scale((uint8_t)byte);
 }
 
-template <int DT, bool RUN>
+template <int DT, int ROWS>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ x, int64_t parts, int k,
                                                            uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256)
-        mx4_quantize_part<DT, RUN>(x, q, k, codes, [&](uint8_t byte) { scales[q >> 2] = byte; });
+        mx4_quantize_part<DT, ROWS>(x, q, k, codes, [&](uint8_t byte) { scales[q >> 2] = byte; });
 }
 
+// Sixteen bytes of the result a lane: with eight fp32 values to a lane a store is half of every line it touches (400,000 x 256: 176 us).
+template <int DT> constexpr int MX4_OUT = DT == NERFX_TYPE_F32 ? 4 : 8;
 template <int DT, bool RUN>
-__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const void* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              int64_t parts, int k, void* __restrict__ out) {
-    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2;
+    constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, N = MX4_OUT<DT>;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < parts; q += (int64_t)gridDim.x * 256) {
         int at;
-        char* dst = (char*)out + mx4_place<RUN>(q, k, at) * SIZE;
+        char* dst = (char*)out + mx4_place<RUN, N>(q, k, at) * SIZE;
         if (!RUN && at >= k) continue;
-        const uint32_t c = codes[q], byte = scales[q >> 2];
+        const uint32_t byte = scales[q / (MX4_BLOCK / N)];
         const float scale = Mx4Raw<DT, 8>::scale_value(byte);
-        uint32_t w[8 * SIZE / 4];
+        u32x4_any_t w;
+        if constexpr (DT == NERFX_TYPE_F32) {
+            const uint32_t c = ((const uint16_t*)codes)[q];
+            const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
+            const float v[4] = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, v[i]);
+        } else {
+            const uint32_t c = ((const uint32_t*)codes)[q];
 #define NERFX_PAIR(s)                                                                                                                  \
-        if constexpr (DT == NERFX_TYPE_F32) {                                                                                          \
-            const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, s);                                                      \
-            const float lo = v[0], hi = v[1];                                                                                          \
-            w[2 * s] = __builtin_bit_cast(uint32_t, lo); w[2 * s + 1] = __builtin_bit_cast(uint32_t, hi);                              \
-        } else if constexpr (DT == NERFX_TYPE_BF16) {                                                                                  \
-            w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, s));                               \
-        } else {                                                                                                                       \
-            w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, s));                                \
-        }
-        NERFX_PAIR(0) NERFX_PAIR(1) NERFX_PAIR(2) NERFX_PAIR(3)
+            if constexpr (DT == NERFX_TYPE_BF16) w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, s)); \
+            else w[s] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, s));
+            NERFX_PAIR(0) NERFX_PAIR(1) NERFX_PAIR(2) NERFX_PAIR(3)
 #undef NERFX_PAIR
-        if (byte == 255u) {
-#pragma unroll
-            for (int i = 0; i < 2 * SIZE; ++i) w[i] = DT == NERFX_TYPE_F32 ? 0x7fc00000u : DT == NERFX_TYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
         }
-        if (RUN || at + 8 <= k) {
-#pragma unroll
-            for (int i = 0; i < SIZE / 2; ++i) {
-                const u32x4_any_t piece = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-                if constexpr (RUN) __builtin_nontemporal_store(piece, (u32x4_any_t*)(dst + 16 * i));
-                else *(u32x4_any_t*)(dst + 16 * i) = piece;
-            }
+        if (byte == 255u) w = DT == NERFX_TYPE_F32 ? 0x7fc00000u : DT == NERFX_TYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+        if constexpr (RUN) {
+            __builtin_nontemporal_store(w, (u32x4_any_t*)dst);
+        } else if (at + N <= k) {
+            *(u32x4_any_t*)dst = w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < N; ++i) {
                 if (at + i >= k) continue;
                 if constexpr (SIZE == 4) *(uint32_t*)(dst + 4 * i) = w[i];
                 else *(uint16_t*)(dst + 2 * i) = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
@@ -332,7 +345,7 @@ struct Mx4PrepareArgs {
     int64_t m;
     int32_t n, k, w_groups;
 };
-template <int DT, bool RUN>
+template <int DT, int ROWS>
 __global__ __launch_bounds__(256) void mx4_prepare_kernel(const Mx4PrepareArgs a) {
     const int nb = mx4_blocks(a.k);
     if ((int)blockIdx.x < a.w_groups) {
@@ -345,7 +358,7 @@ __global__ __launch_bounds__(256) void mx4_prepare_kernel(const Mx4PrepareArgs a
     } else {
         const int64_t parts = a.m * nb * 4, stage_bytes = mx4_ordered_bytes(a.m);
         for (int64_t q = first; q < parts; q += step)
-            mx4_quantize_part<DT, RUN>(a.x, q, a.k, a.codes, [&](uint8_t byte) {
+            mx4_quantize_part<DT, ROWS>(a.x, q, a.k, a.codes, [&](uint8_t byte) {
                 const uint64_t block = (uint64_t)q >> 2, row = block >> 32 ? block / nb : (uint32_t)block / nb;
                 const int b = (int)(block - row * nb);
                 uint8_t* to = a.x_ordered + b / MX4_STAGE * stage_bytes + row * MX4_STAGE;
@@ -439,12 +452,6 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
         for (int j = 0; j < FQ; ++j) sq[j] = T::scales(stage, q_row + 32 * j, h);
     };
     float16_t_ acc[FP][FQ];
-#pragma unroll
-    for (int i = 0; i < FP; ++i)
-#pragma unroll
-        for (int j = 0; j < FQ; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     auto multiply = [&](const typename T::Frags& f, auto step) {
         constexpr int s = decltype(step)::value;
 #pragma unroll
@@ -461,6 +468,16 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     for (int c = threadIdx.x; c < T::TP; c += 64 * T::WAVES) bias_lds[c] = a.bias && c <= p_last ? a.bias[n0 + c] : 0.f;
     for (int st = 0; st < min(S, stages); ++st) fetch(st);
     landed<0>();
+#pragma unroll
+    for (int i = 0; i < FP; ++i)                               // sums begin as the bias, in the other kernel as here: the same results
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4_t b = *(const f32x4_t*)(bias_lds + wp + 32 * i + 8 * q + 4 * h);
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = b[e];
+        }
     take_scales(0);
     T::read(f0, lds, 0, p_row, q_row, h);
     for (int st = 0; st < stages - 1; ++st) {
@@ -506,19 +523,13 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
     }
     __syncthreads();                                           // the stages have been read: their place is the waves' own now
     Mx4Lines lines{lds + wave * Mx4Lines::BYTES};
-    static_assert(T::WAVES * Mx4Lines::BYTES <= T::BIAS_AT, "the bias is still needed");
+    static_assert(T::WAVES * Mx4Lines::BYTES <= T::LDS_BYTES, "a place for each wave");
 #pragma unroll
     for (int j = 0; j < FQ; ++j) {
 #pragma unroll
         for (int i = 0; i < FP; ++i) {
             const int n = n0 + wp + 32 * i;
             if (n >= a.n) break;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4_t b = *(const f32x4_t*)(bias_lds + wp + 32 * i + 8 * q + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += b[e];
-            }
             lines.add(a, acc[i][j], m0 + wq + 32 * j, n);
         }
         lines.rest(a, m0 + wq + 32 * j);
@@ -561,7 +572,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4
         using Raw = Mx4Raw<DT, 32>;
         for (int q = threadIdx.x; q < m * nb; q += 64 * SKINNY_WAVES) {
             const int r = q / nb, b = q - r * nb;
-            const Raw v = mx4_load<DT, 32>((const char*)a.x + (int64_t)r * a.k * (DT == NERFX_TYPE_F32 ? 4 : 2), b * 32, a.k);
+            const Raw v = mx4_load<DT, 32, false>((const char*)a.x + (int64_t)r * a.k * (DT == NERFX_TYPE_F32 ? 4 : 2), b * 32, a.k);
             const uint32_t byte = Raw::scale_byte(v.top_bits());
             const float scale = Raw::scale_value(byte);
             *(u32x4_t*)(lds + q * 16) = {v.codes(0, scale), v.codes(1, scale), v.codes(2, scale), v.codes(3, scale)};
@@ -632,7 +643,7 @@ __host__ __device__ inline int stream_lds(int ks, int columns) {
     return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4) + STREAM_WAVES * Mx4Lines::BYTES;
 }
 
-template <int DT, int KS>
+template <int DT, int KS, bool ODD>
 __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4LinearArgs a, int columns) {
     extern __shared__ __align__(16) char lds[];
     constexpr int SIZE = DT == NERFX_TYPE_F32 ? 4 : 2, SB = KS > 4 ? 8 : 4;
@@ -686,7 +697,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
                     Raw raw[AT_ONCE];
 #pragma unroll
                     for (int u = 0; u < AT_ONCE; ++u)                      // behind the row's last whole block: that one again
-                        if (s0 + u < KS) raw[u] = mx4_load_whole<DT, 32>(row, min(2 * (s0 + u) + h, whole - 1) * MX4_BLOCK);
+                        if (s0 + u < KS) raw[u] = mx4_load_whole<DT, 32, ODD>(row, min(2 * (s0 + u) + h, whole - 1) * MX4_BLOCK);
 #pragma unroll
                     for (int u = 0; u < AT_ONCE; ++u) {
                         if (s0 + u < KS) take(raw[u], s0 + u);
@@ -695,7 +706,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
                 }
             }
             if (nb != 2 * KS || whole != nb) {                             // rows that end earlier: a part of a block, and zeros
-                Raw tail = mx4_load<DT, 32>(row, whole * MX4_BLOCK, a.k);
+                Raw tail = mx4_load<DT, 32, ODD>(row, whole * MX4_BLOCK, a.k);
                 const uint32_t byte = Raw::scale_byte(tail.top_bits());
                 const float scale = Raw::scale_value(byte);
                 const u32x4_t codes = {tail.codes(0, scale), tail.codes(1, scale), tail.codes(2, scale), tail.codes(3, scale)};
@@ -739,18 +750,26 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 static dim3 mx4_grid(int64_t parts) { return dim3((unsigned)std::min<int64_t>((parts + 255) / 256, 256 * 32)); }
 
+// f(type, rows) for a float type and how its rows lie.
+template <class F>
+static int mx4_by_rows(const void* x, int k, int dtype, F f) {
+    using F32 = std::integral_constant<int, NERFX_TYPE_F32>; using BF16 = std::integral_constant<int, NERFX_TYPE_BF16>;
+    using F16 = std::integral_constant<int, NERFX_TYPE_F16>;
+    using Run = std::integral_constant<int, MX4_RUN>; using Any = std::integral_constant<int, MX4_ANY>; using Odd = std::integral_constant<int, MX4_ODD>;
+    const bool odd = mx4_odd(x, k, dtype);
+    if (k % MX4_BLOCK == 0) return dtype == NERFX_TYPE_F32 ? f(F32{}, Run{}) : dtype == NERFX_TYPE_BF16 ? f(BF16{}, Run{}) : f(F16{}, Run{});
+    if (dtype == NERFX_TYPE_F32) return f(F32{}, Any{});
+    if (dtype == NERFX_TYPE_BF16) return odd ? f(BF16{}, Odd{}) : f(BF16{}, Any{});
+    return odd ? f(F16{}, Odd{}) : f(F16{}, Any{});
+}
+
 static int quantize_launch(const void* x, int dtype, int64_t rows, int k, uint8_t* codes, uint8_t* scales, hipStream_t stream) {
     const int64_t parts = rows * mx4_blocks(k) * 4;
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, stream, x, parts, k, (uint32_t*)codes, scales);
         return launch_status("mx4_quantize_kernel");
     };
-    if (k % MX4_BLOCK == 0) {
-        return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32, true>)
-             : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, true>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, true>);
-    }
-    return dtype == NERFX_TYPE_F32 ? go(mx4_quantize_kernel<NERFX_TYPE_F32, false>)
-         : dtype == NERFX_TYPE_BF16 ? go(mx4_quantize_kernel<NERFX_TYPE_BF16, false>) : go(mx4_quantize_kernel<NERFX_TYPE_F16, false>);
+    return mx4_by_rows(x, k, dtype, [&](auto type, auto rows) { return go(mx4_quantize_kernel<decltype(type)::value, decltype(rows)::value>); });
 }
 
 static int prepare_launch(Mx4PrepareArgs& a, int dtype, hipStream_t stream) {
@@ -760,13 +779,8 @@ static int prepare_launch(Mx4PrepareArgs& a, int dtype, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, dim3(a.w_groups + mx4_grid(parts).x), dim3(256), 0, stream, a);
         return launch_status("mx4_prepare_kernel");
     };
-    const bool run = a.k % MX4_BLOCK == 0;
-    switch (dtype) {
-        case NERFX_TYPE_F32: return run ? go(mx4_prepare_kernel<NERFX_TYPE_F32, true>) : go(mx4_prepare_kernel<NERFX_TYPE_F32, false>);
-        case NERFX_TYPE_BF16: return run ? go(mx4_prepare_kernel<NERFX_TYPE_BF16, true>) : go(mx4_prepare_kernel<NERFX_TYPE_BF16, false>);
-        case NERFX_TYPE_F16: return run ? go(mx4_prepare_kernel<NERFX_TYPE_F16, true>) : go(mx4_prepare_kernel<NERFX_TYPE_F16, false>);
-        default: return go(mx4_prepare_kernel<NERFX_TYPE_MX4, true>);
-    }
+    if (dtype == NERFX_TYPE_MX4) return go(mx4_prepare_kernel<NERFX_TYPE_MX4, MX4_RUN>);
+    return mx4_by_rows(a.x, a.k, dtype, [&](auto type, auto rows) { return go(mx4_prepare_kernel<decltype(type)::value, decltype(rows)::value>); });
 }
 
 template <int FP, int WP, int FQ, int WQ, int S>
@@ -784,8 +798,10 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //          tiles).  Each of them quantises float rows for itself, up to 128 KB of them (64 x 1000 fp32 by 1000: 15 us, 7.6 with
 //          tiles; 32 x 2048 bf16 by 256: 7 and 8.5), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
 //          Not for a result in blocks, which are of 32 columns;
-//  stream  otherwise up to 256 values a row, or 512 and up to 256 columns: float rows are quantised in registers, once for every
-//          256 columns (16,384 x 4096 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles);
+//  stream  otherwise up to 256 values a row (of floats, up to 512 bytes), or 512 and up to 256 columns: float rows are quantised in
+//          registers, once for every 256 columns (16,384 x 4096 bf16 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles).
+//          Not for up to 16,384 float rows of 512 bytes or more: what counts there is how long one wave takes, and it reads its rows
+//          piece by piece (1000 x 256 fp32 by 256: 11.1 us, 6.2 with tiles; 130,000: 49 and 54);
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
 //          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit): a small product lasts as
 //          long as one tile does (256 x 4096 by 4096: 13 us, 19 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 27 and 24);
@@ -805,11 +821,11 @@ static Mx4Plan mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype) {
     const bool is_float = x_dtype != NERFX_TYPE_MX4, blocks_out = y_dtype == NERFX_TYPE_MX4;
     const int64_t nb = mx4_blocks(k);
     Mx4Plan plan{};
-    const int64_t x_bytes = m * k * (x_dtype == NERFX_TYPE_F32 ? 4 : 2);
-    if (!blocks_out && m <= (!is_float || x_bytes <= SKINNY_FLOATS ? SKINNY_ROWS : 16)) {
+    const int row_bytes = !is_float ? 0 : x_dtype == NERFX_TYPE_F32 ? 4 * k : 2 * k;       // to be quantised
+    if (!blocks_out && m <= (m * row_bytes <= SKINNY_FLOATS ? SKINNY_ROWS : 16)) {
         plan.kind = MX4_SKINNY;
         if (is_float && m * nb * 17 > SKINNY_LDS) { plan.codes = m * nb * 16; plan.scales = (m * nb + 15) / 16 * 16; }
-    } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20) {
+    } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20 && (row_bytes <= 512 || n <= 256) && (row_bytes < 512 || m > 16384)) {
         plan.kind = MX4_STREAM;
     } else {
         plan.kind = MX4_TILE;
@@ -854,14 +870,20 @@ static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, columns);
         return launch_status("mx4_stream_kernel");
     };
-    switch (stream_steps(a.k)) {
-        case 1: return go(mx4_stream_kernel<DT, 1>, 1);
-        case 2: return go(mx4_stream_kernel<DT, 2>, 2);
-        case 3: return go(mx4_stream_kernel<DT, 3>, 3);
-        case 4: return go(mx4_stream_kernel<DT, 4>, 4);
-        case 5: return go(mx4_stream_kernel<DT, 5>, 5);
-        default: return go(mx4_stream_kernel<DT, 8>, 8);
-    }
+    auto by_steps = [&](auto odd) {
+        constexpr bool ODD = decltype(odd)::value;
+        switch (stream_steps(a.k)) {
+            case 1: return go(mx4_stream_kernel<DT, 1, ODD>, 1);
+            case 2: return go(mx4_stream_kernel<DT, 2, ODD>, 2);
+            case 3: return go(mx4_stream_kernel<DT, 3, ODD>, 3);
+            case 4: return go(mx4_stream_kernel<DT, 4, ODD>, 4);
+            case 5: return go(mx4_stream_kernel<DT, 5, ODD>, 5);
+            default: return go(mx4_stream_kernel<DT, 8, ODD>, 8);
+        }
+    };
+    if constexpr (DT == NERFX_TYPE_BF16 || DT == NERFX_TYPE_F16)
+        if (mx4_odd(a.x, a.k, DT)) return by_steps(std::true_type{});
+    return by_steps(std::false_type{});
 }
 
 static int check_mx4(int64_t rows, int k) {
@@ -890,9 +912,9 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
     if (rows == 0) return 0;
     NERFX_REQUIRE(codes && scales && out, "codes / scales / out is NULL");
     NERFX_REQUIRE(((uintptr_t)codes & 3) == 0, "codes are not aligned to 4 bytes");
-    const int64_t parts = rows * mx4_blocks(k) * 4;
+    const int64_t parts = rows * mx4_blocks(k) * (MX4_BLOCK / (dtype == NERFX_TYPE_F32 ? MX4_OUT<NERFX_TYPE_F32> : MX4_OUT<NERFX_TYPE_BF16>));
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)codes, scales, parts, k, out);
+        hipLaunchKernelGGL(kernel, mx4_grid(parts), dim3(256), 0, (hipStream_t)stream, codes, scales, parts, k, out);
         return launch_status("mx4_dequantize_kernel");
     };
     if (k % MX4_BLOCK == 0) {
