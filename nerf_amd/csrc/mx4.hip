@@ -635,12 +635,12 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void mx4_skinny_kernel(const Mx4
 // sixteen different banks); a wave takes 32 rows of x, a lane two blocks of every 64 values of its row, quantises them in
 // registers, where they are operands of the matrix instruction as they are, and goes over W's columns (524,288 x 256 bf16 by 256:
 // 112 us, 4.8 TB/s).
-constexpr int STREAM_WAVES = 8, STREAM_ROWS = 32 * STREAM_WAVES;
+constexpr int STREAM_WAVES = 8;                                // at most
 
 __host__ __device__ inline int stream_row_bytes(int ks) { return (2 * ks + 1) * 16; }
 __host__ __device__ inline int stream_scale_bytes(int ks) { return ks > 4 ? 16 : 8; }      // both halves of a row
-__host__ __device__ inline int stream_lds(int ks, int columns) {
-    return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4) + STREAM_WAVES * Mx4Lines::BYTES;
+__host__ __device__ inline int stream_lds(int ks, int columns, int waves) {
+    return columns * (stream_row_bytes(ks) + stream_scale_bytes(ks) + 4) + waves * Mx4Lines::BYTES;
 }
 
 template <int DT, int KS, bool ODD>
@@ -652,20 +652,33 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void mx4_stream_kernel(const Mx4
     char* scale_lds = lds + columns * stream_row_bytes(KS);
     float* bias_lds = (float*)(scale_lds + columns * stream_scale_bytes(KS));
     char* line_lds = (char*)(bias_lds + columns) + wave * Mx4Lines::BYTES;
-    for (int c = threadIdx.x; c < columns; c += 64 * STREAM_WAVES) bias_lds[c] = a.bias && c0 + c < a.n ? a.bias[c0 + c] : 0.f;
-    for (int c = threadIdx.x; c < columns * 2 * KS; c += 64 * STREAM_WAVES) {
-        const int r = c / (2 * KS), b = c - r * 2 * KS;
-        u32x4_t v = {0, 0, 0, 0};
-        uint32_t s = 127u;
-        if (c0 + r < a.n && b < nb) {
-            v = *((const u32x4_t*)a.w + (int64_t)(c0 + r) * nb + b);
-            s = a.w_scales[(int64_t)(c0 + r) * nb + b];
+    const int threads = blockDim.x;
+    for (int c = threadIdx.x; c < columns; c += threads) bias_lds[c] = a.bias && c0 + c < a.n ? a.bias[c0 + c] : 0.f;
+    constexpr int W_AT_ONCE = 4;
+    for (int first = threadIdx.x; first < columns * 2 * KS; first += W_AT_ONCE * threads) {
+        u32x4_t v[W_AT_ONCE];
+        uint32_t s[W_AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < W_AT_ONCE; ++i) {
+            const int c = first + i * threads, r = c / (2 * KS), b = c - r * 2 * KS;
+            v[i] = {0, 0, 0, 0};
+            s[i] = 127u;
+            if (r < columns && c0 + r < a.n && b < nb) {
+                v[i] = *((const u32x4_t*)a.w + (int64_t)(c0 + r) * nb + b);
+                s[i] = a.w_scales[(int64_t)(c0 + r) * nb + b];
+            }
         }
-        *(u32x4_t*)(lds + r * stream_row_bytes(KS) + b * 16) = v;
-        scale_lds[r * 2 * SB + (b & 1) * SB + (b >> 1)] = (char)s;
+#pragma unroll
+        for (int i = 0; i < W_AT_ONCE; ++i) {
+            const int c = first + i * threads, r = c / (2 * KS), b = c - r * 2 * KS;
+            if (r >= columns) break;
+            *(u32x4_t*)(lds + r * stream_row_bytes(KS) + b * 16) = v[i];
+            scale_lds[r * 2 * SB + (b & 1) * SB + (b >> 1)] = (char)s[i];
+        }
     }
     __syncthreads();
-    for (int64_t m0 = (int64_t)blockIdx.x * STREAM_ROWS + 32 * wave; m0 < a.m; m0 += (int64_t)gridDim.x * STREAM_ROWS) {
+    const int rows = threads >> 1;                             // 32 a wave
+    for (int64_t m0 = (int64_t)blockIdx.x * rows + 32 * wave; m0 < a.m; m0 += (int64_t)gridDim.x * rows) {
         const int64_t m = min(m0 + (lane & 31), a.m - 1);
         u32x4_t xc[KS];
         uint32_t xs[(KS + 3) / 4] = {};
@@ -799,9 +812,7 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //          tiles; 32 x 2048 bf16 by 256: 7 and 8.5), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
 //          Not for a result in blocks, which are of 32 columns;
 //  stream  otherwise up to 256 values a row (of floats, up to 512 bytes), or 512 and up to 256 columns: float rows are quantised in
-//          registers, once for every 256 columns (16,384 x 4096 bf16 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles).
-//          Not for up to 16,384 float rows of 512 bytes or more: what counts there is how long one wave takes, and it reads its rows
-//          piece by piece (1000 x 256 fp32 by 256: 11.1 us, 6.2 with tiles; 130,000: 49 and 54);
+//          registers, once for every 256 columns (16,384 x 4096 bf16 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles);
 //  tile    everything else, float rows by way of the workspace: a tile of x is read by every tile of columns.  256 x 256 where
 //          that makes 192 tiles or more; 64 x 64 where there are no more than 512 (two a compute unit): a small product lasts as
 //          long as one tile does (256 x 4096 by 4096: 13 us, 19 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 27 and 24);
@@ -825,7 +836,7 @@ static Mx4Plan mx4_plan(int64_t m, int n, int k, int x_dtype, int y_dtype) {
     if (!blocks_out && m <= (m * row_bytes <= SKINNY_FLOATS ? SKINNY_ROWS : 16)) {
         plan.kind = MX4_SKINNY;
         if (is_float && m * nb * 17 > SKINNY_LDS) { plan.codes = m * nb * 16; plan.scales = (m * nb + 15) / 16 * 16; }
-    } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20 && (row_bytes <= 512 || n <= 256) && (row_bytes < 512 || m > 16384)) {
+    } else if (k <= (n <= 256 ? 512 : 256) && n <= 1 << 20 && (row_bytes <= 512 || n <= 256)) {
         plan.kind = MX4_STREAM;
     } else {
         plan.kind = MX4_TILE;
@@ -857,15 +868,26 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 
 template <int DT>
 static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
-    const int64_t row_tiles = (a.m + STREAM_ROWS - 1) / STREAM_ROWS;
-    // up to 256 columns in LDS at a time; few rows: the columns are spread over workgroups until the device is full
-    const int tiles = (a.n + 31) / 32;
-    const int groups = (int)std::min<int64_t>(tiles, std::max<int64_t>((tiles + 7) / 8, 256 / row_tiles));
+    // Few rows: smaller workgroups and fewer columns in each until the device is full.  A lane's row is a line of its own, so that
+    // the loads of eight waves take a CU 3.5 us for every 256 bytes a row (1000 x 128 fp32 by 295: 6.7 us with one wave, 10.7 with
+    // eight); and a wave brings 256 blocks of W at a time, for which it may wait twice.  Half of the device is enough below eight waves
+    // (16,000 x 256 bf16 by 256: 9.2 us with 125 workgroups of four, 10.3 with 250 of two), not with them (32,000 x 128 fp32 by 256:
+    // 17.6 us with 125 of eight, 12.9 with 250 of four).
+    const int tiles = (a.n + 31) / 32, ks = stream_steps(a.k);
+    int waves = 2 * STREAM_WAVES, groups;
+    int64_t row_tiles;
+    do {
+        waves /= 2;
+        row_tiles = (a.m + 32 * waves - 1) / (32 * waves);
+        const int most = std::min(8, std::max(1, 8 * waves / ks));             // tiles of columns
+        groups = (tiles + most - 1) / most;
+    } while (waves > 1 && row_tiles * groups < (waves == STREAM_WAVES ? 192 : 120));
+    groups = (int)std::min<int64_t>(tiles, std::max<int64_t>(groups, 256 / row_tiles));
     const int per = (tiles + groups - 1) / groups;
     const int columns = 32 * per;
-    const dim3 grid((unsigned)std::min<int64_t>(row_tiles, 512), (unsigned)((tiles + per - 1) / per)), block(64 * STREAM_WAVES);
+    const dim3 grid((unsigned)std::min<int64_t>(row_tiles, 512), (unsigned)((tiles + per - 1) / per)), block(64 * waves);
     auto go = [&](auto kernel, int ks) {
-        const size_t lds = stream_lds(ks, columns);
+        const size_t lds = stream_lds(ks, columns, waves);
         NERFX_OPT_IN_LDS(kernel, lds);
         hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, columns);
         return launch_status("mx4_stream_kernel");
