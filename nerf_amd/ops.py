@@ -900,25 +900,42 @@ class Mx4:
             raise ValueError("Mx4: codes and scales must be contiguous")
         if codes.data_ptr() % 16:
             raise ValueError("Mx4: codes must be aligned to 16 bytes")
-        self.codes, self.scales, self.k = codes, scales, k
+        self._codes, self._scales, self._both = codes, scales, None
+        self.shape: Tuple[int, int] = (codes.shape[0], k)
+        self.k, self.device = k, codes.device
 
     @classmethod
     def _new(cls, rows: int, k: int, like: Tensor) -> "Mx4":
-        """An unwritten one, where `like` is."""
+        """An unwritten one, where `like` is: one allocation, made two tensors of when they are asked for."""
         self = object.__new__(cls)
-        blocks = (k + 31) // 32
-        self.codes = like.new_empty((rows, 16 * blocks), dtype=torch.uint8)
-        self.scales = self.codes.new_empty((rows, blocks))
-        self.k = k
+        self._codes = self._scales = None
+        self._both = like.new_empty((rows * ((k + 31) // 32) * 17,), dtype=torch.uint8)
+        self.shape, self.k, self.device = (rows, k), k, like.device
         return self
 
-    @property
-    def shape(self) -> Tuple[int, int]:
-        return self.codes.shape[0], self.k
+    def _split(self) -> None:
+        rows, blocks = self.shape[0], (self.k + 31) // 32
+        self._codes = self._both[:rows * blocks * 16].view(rows, blocks * 16)
+        self._scales = self._both[rows * blocks * 16:].view(rows, blocks)
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> Tensor:
+        if self._codes is None:
+            self._split()
+        return self._codes
+
+    @property
+    def scales(self) -> Tensor:
+        if self._scales is None:
+            self._split()
+        return self._scales
+
+    def _pointers(self):
+        """Where the codes and the scales are."""
+        if self._both is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self._both.data_ptr()
+        return at, at + self.shape[0] * ((self.k + 31) // 32) * 16
 
     @staticmethod
     def cat(parts) -> "Mx4":
@@ -934,13 +951,14 @@ class Mx4:
         """The values the codes stand for (exact in fp32 and bf16)."""
         if dtype not in _TYPES:
             raise TypeError(f"dequantize gives fp32, bf16 or fp16 (asked for {dtype})")
-        if not self.codes.is_cuda:
-            raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {self.codes.device}")
-        codes, dev = self.codes, self.codes.device
-        rows = codes.shape[0]
-        out = codes.new_empty((rows, self.k), dtype=dtype)
+        dev, held = self.device, self._codes if self._both is None else self._both
+        if not held.is_cuda:
+            raise RuntimeError(f"nerf_amd runs on ROCm devices only: `codes` is on {dev}")
+        rows = self.shape[0]
+        out = held.new_empty((rows, self.k), dtype=dtype)
+        codes, scales = self._pointers()
         with _on(dev):
-            check(lib.nerfx_mx4_dequantize(codes.data_ptr(), self.scales.data_ptr(), rows, self.k, _TYPES[dtype], out.data_ptr(),
+            check(lib.nerfx_mx4_dequantize(codes, scales, rows, self.k, _TYPES[dtype], out.data_ptr(),
                                            _stream_on(dev)))
         return out
 
@@ -969,8 +987,7 @@ def mx4_quantize(x: Tensor) -> Mx4:
     dev = x.device
     out = Mx4._new(rows, k, x)
     with _on(dev):
-        check(lib.nerfx_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, out.codes.data_ptr(), out.scales.data_ptr(),
-                                     _stream_on(dev)))
+        check(lib.nerfx_mx4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, *out._pointers(), _stream_on(dev)))
     return out
 
 
@@ -986,13 +1003,14 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
         raise ValueError(f"unknown activation {activation!r}")
     n, k = weight.shape
     if isinstance(x, Mx4):
-        lead, dt, src, scales, dev = (x.shape[0],), _lib.TYPE_MX4, x.codes, x.scales, x.device
-        if not x.codes.is_cuda:
+        lead, dt, src, dev, width, default = (x.shape[0],), _lib.TYPE_MX4, x._codes if x._both is None else x._both, x.device, x.k, torch.float32
+        if not src.is_cuda:
             raise RuntimeError(f"nerf_amd runs on ROCm devices only: `x` is on {dev}")
-        width, default = x.k, torch.float32
+        codes, scales = x._pointers()
     else:
         src = _mx4_input(x, "x")
-        lead, dt, scales, dev, width, default = src.shape[:-1], _TYPES[src.dtype], None, src.device, src.shape[-1], src.dtype
+        lead, dt, dev, width, default = src.shape[:-1], _TYPES[src.dtype], src.device, src.shape[-1], src.dtype
+        codes, scales = src.data_ptr(), None
     if width != k:
         raise ValueError(f"x has {width} columns, weight {k}")
     if weight.device != dev:
@@ -1007,18 +1025,18 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
     m = math.prod(lead)
     if out_dtype == "mx4":
         out = Mx4._new(m, n, src)
-        y, y_scales, yt = out.codes, out.scales, _lib.TYPE_MX4
+        (y, y_scales), yt = out._pointers(), _lib.TYPE_MX4
     else:
         out_dtype = default if out_dtype is None else out_dtype
         if out_dtype not in _TYPES:
             raise TypeError(f"mx4_linear gives fp32, bf16, fp16 or \"mx4\" (asked for {out_dtype})")
-        out = y = src.new_empty((*lead, n), dtype=out_dtype)
-        y_scales, yt = None, _TYPES[out_dtype]
+        out = src.new_empty((*lead, n), dtype=out_dtype)
+        y, y_scales, yt = out.data_ptr(), None, _TYPES[out_dtype]
     need = lib.nerfx_mx4_linear_workspace_bytes(m, n, k, dt, yt)
     ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need > 0 else None
     with _on(dev):
-        check(lib.nerfx_mx4_linear(src.data_ptr(), dt, _at(scales), m, k, weight.codes.data_ptr(), weight.scales.data_ptr(), n, _at(bias),
-                                   _LINEAR_ACTS[activation], y.data_ptr(), yt, _at(y_scales), _at(ws), max(need, 0), _stream_on(dev)))
+        check(lib.nerfx_mx4_linear(codes, dt, scales, m, k, *weight._pointers(), n, _at(bias), _LINEAR_ACTS[activation], y, yt, y_scales,
+                                   _at(ws), max(need, 0), _stream_on(dev)))
     return out
 
 
