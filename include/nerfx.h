@@ -367,8 +367,8 @@ typedef struct {
 /* out = the matrix nearest to orthogonal that `steps` (1..32) Newton-Schulz steps make of grad:
  * X = grad / max(|grad|_F, eps), then X <- a X + (b S + c S S) X with S = X X^T, (a, b, c) =
  * coefficients[3 k ..] in step k (host array); a matrix with more rows than columns is worked on
- * transposed.  Sums are fp32 (the norm fp64), products take both factors to 22 bits, whatever the
- * `dtype` (NERFX_TYPE_*) of grad and out.  A zero matrix gives zeros; a matrix with an infinity or
+ * transposed.  Sums are fp32 (the norm fp64), products take both factors to 22 bits (24 where a side
+ * is 16 or less), whatever the `dtype` (NERFX_TYPE_*) of grad and out.  A zero matrix gives zeros; a matrix with an infinity or
  * a NaN gives NaN.  `mats` is a host array; all matrices share the launches.  Coefficients
  * that would let a singular value grow beyond 64 are refused.  `workspace`:
  * nerfx_orthogonalize_workspace_bytes(mats, count) bytes (0 for groups of matrices of up to 64 x 256), aligned to 16;
@@ -382,7 +382,8 @@ int nerfx_orthogonalize(const nerfx_matrix_t* mats /* host */, int count, int dt
  *   momentum <- mu momentum + (1 - mu) g,   g = grad / *grad_scale (if given)
  *   u = nesterov ? mu momentum + (1 - mu) g : momentum
  *   param <- (1 - lr weight_decay) param - lr' orthogonalize(u),   lr' by `adjust_lr` (NERFX_LR_*)
- * Nothing changes where *found_inf != 0 (device float, may be NULL).  No two matrices may share memory.
+ * Nothing changes where *found_inf != 0 (device float, may be NULL).  No two matrices may share memory, nor
+ * a gradient with what is written.
  * The same workspace as nerfx_orthogonalize. */
 int nerfx_muon_step(const nerfx_matrix_t* mats /* host */, int count, double lr, double momentum, int nesterov,
                     double weight_decay, int adjust_lr, const float* coefficients /* host */, int steps, float eps,
@@ -402,7 +403,8 @@ int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
  * x_scales its scales; NULL otherwise), W (n, k) as codes and scales (n <= 2^24), bias (n) fp32 or NULL, sums in fp32,
  * activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as above along n, y its codes and
- * y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes.
+ * y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes, floats to their own size.  The first call of a
+ * kind on a device opts its kernel into its LDS size: make it outside of graph capture.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
 int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,
