@@ -4,7 +4,11 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <exception>
+#include <map>
+#include <mutex>
 #include <string>
+#include <utility>
 
 #include "../../include/nerfx.h"
 
@@ -35,27 +39,30 @@ inline int launch_status(const char* what) {
 
 // ---- dynamic LDS beyond the default limit ---------------------------------------
 // hipFuncSetAttribute(MaxDynamicSharedMemorySize) is a setting of one kernel ON ONE DEVICE: a host
-// thread that drives several GPUs must make it on each.  `LdsOptIn` remembers, per device, the largest
-// size a kernel has been opted into (one static instance per kernel instantiation); `ensure` makes the
-// call for the current device when a launch needs more.  Two threads racing here at worst both make
-// the same call.
-struct LdsOptIn {
-    static constexpr int MAX_DEVICES = 64;
-    size_t bytes[MAX_DEVICES] = {};
-    int ensure(const void* kern, size_t lds_bytes) {
-        int dev = 0;
-        NERFX_HIP(hipGetDevice(&dev));
-        if (dev < 0 || dev >= MAX_DEVICES || lds_bytes > __atomic_load_n(&bytes[dev], __ATOMIC_RELAXED)) {
+// thread that drives several GPUs must make it on each.  The largest size asked for so far is
+// remembered by kernel and device, wherever the launch is written (a launch in a generic lambda serves
+// every kernel of one signature), and raised under a lock: a thread that needs less than another
+// neither lowers the limit nor the record.
+inline int opt_in_lds(const void* kern, size_t lds_bytes) {
+    int dev = 0;
+    NERFX_HIP(hipGetDevice(&dev));
+    static std::mutex lock;
+    static std::map<std::pair<const void*, int>, size_t> most;
+    try {
+        std::lock_guard<std::mutex> hold(lock);
+        size_t& had = most[{kern, dev}];
+        if (lds_bytes > had) {
             NERFX_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes));
-            if (dev >= 0 && dev < MAX_DEVICES) __atomic_store_n(&bytes[dev], lds_bytes, __ATOMIC_RELAXED);
+            had = lds_bytes;
         }
-        return 0;
+    } catch (const std::exception& e) {                        // no memory for the record
+        return fail(NERFX_E_NOMEM, "LDS limit of a kernel: %s", e.what());
     }
-};
+    return 0;
+}
 #define NERFX_OPT_IN_LDS(kern, lds_bytes)                                            \
     do {                                                                             \
-        static ::nerfx::LdsOptIn _opt_in;                                            \
-        if (int _rc = _opt_in.ensure((const void*)(kern), (lds_bytes))) return _rc;  \
+        if (int _rc = ::nerfx::opt_in_lds((const void*)(kern), (lds_bytes))) return _rc; \
     } while (0)
 
 // ---- encoders ---------------------------------------------------------------

@@ -406,9 +406,10 @@ __global__ __launch_bounds__(256) void unfold_kernel(nerfx_model::FoldSpots f, i
 #define WGRAD_ROUNDS 2
 #endif
 static int resident_workgroups() {
-    static int slots[LdsOptIn::MAX_DEVICES] = {};                   // per device: two workgroups per CU
+    constexpr int MAX_DEVICES = 64;
+    static int slots[MAX_DEVICES] = {};                             // per device: two workgroups per CU
     int dev = 0, cus = 256;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= LdsOptIn::MAX_DEVICES) return 2 * 256;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= MAX_DEVICES) return 2 * 256;
     if (!__atomic_load_n(&slots[dev], __ATOMIC_RELAXED)) {
         if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) cus = 256;
         __atomic_store_n(&slots[dev], 2 * cus, __ATOMIC_RELAXED);

@@ -854,7 +854,7 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     const size_t lds = std::max(codes, sums);
     const dim3 grid((unsigned)((a.n + 15) / 16)), block(64 * SKINNY_WAVES);
     auto go = [&](auto kernel) {
-        NERFX_OPT_IN_LDS(kernel, lds);
+        NERFX_OPT_IN_LDS(kernel, std::max<size_t>(SKINNY_LDS, SKINNY_WAVES * 4 * 1024));       // of any call
         hipLaunchKernelGGL(kernel, grid, block, lds, stream, a);
         return launch_status("mx4_skinny_kernel");
     };
@@ -888,7 +888,7 @@ static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)std::min<int64_t>(row_tiles, 512), (unsigned)((tiles + per - 1) / per)), block(64 * waves);
     auto go = [&](auto kernel, int ks) {
         const size_t lds = stream_lds(ks, columns, waves);
-        NERFX_OPT_IN_LDS(kernel, lds);
+        NERFX_OPT_IN_LDS(kernel, stream_lds(ks, 256, STREAM_WAVES));           // of any call
         hipLaunchKernelGGL(kernel, grid, block, lds, stream, a, columns);
         return launch_status("mx4_stream_kernel");
     };

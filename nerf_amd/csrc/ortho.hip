@@ -987,7 +987,7 @@ static int small_run(OrthoTable& t, const float* coef, int steps, const OrthoSca
     int n = 0;
     for (int k = 0; k < t.call.count; ++k) n = std::max(n, t.mat[k].n);
     const size_t lds = 2 * SMALL_M * 256 + (size_t)n * 512;
-    NERFX_OPT_IN_LDS(ortho_small_kernel, lds);
+    NERFX_OPT_IN_LDS(ortho_small_kernel, 2 * SMALL_M * 256 + SMALL_N * 512);       // of any call
     hipLaunchKernelGGL(ortho_small_kernel, dim3((unsigned)t.call.count), dim3(64 * SMALL_WAVES), lds, stream, t, c);
     return launch_status("ortho_small_kernel");
 }
