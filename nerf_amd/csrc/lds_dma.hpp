@@ -37,6 +37,13 @@ template <int N>
 __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// Between lanes of one wave that hand values on by way of LDS, behind the writes and behind the reads.  The hardware keeps a wave's LDS
+// accesses in order by itself; the compiler, to which each lane is a thread, need not.  No instruction comes of it.
+__device__ __forceinline__ void wave_lds_in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 #endif
 
 }  // namespace nerfx

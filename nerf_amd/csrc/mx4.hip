@@ -287,6 +287,7 @@ public:
     __device__ __forceinline__ void flush(const Mx4LinearArgs& a, int64_t m0, int row_bytes) {
         const int lane = threadIdx.x & 63, at = begin + 16 * (lane & 7);
         const int there = min(end, row_bytes) - at;            // bytes of this lane's piece
+        wave_lds_in_order();                                   // written by other lanes
         u32x4_t piece[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) piece[i] = *(const u32x4_t*)(lds + (8 * i + (lane >> 3)) * PITCH + 16 * (lane & 7));
@@ -304,6 +305,7 @@ public:
                     for (int c = 0; c < there; c += 2) *(uint16_t*)((char*)a.y + m * row_bytes + at + c) = *(const uint16_t*)(left + c);
             }
         }
+        wave_lds_in_order();                                   // the next tile is written there
         end = 0;
     }
     __device__ __forceinline__ void rest(const Mx4LinearArgs& a, int64_t m0) {

@@ -458,22 +458,27 @@ struct SplitLines {
     // row, col: of X.
     __device__ __forceinline__ void leave_out(const OrthoCall& a, const OrthoMat& q, int row, int col) const {
         const int lane = threadIdx.x & 63, c = (q.tall ? row : col) + 4 * (lane & 7);
-        if (c >= q.cols) return;
+        wave_lds_in_order();
+        if (c < q.cols) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 8 * i + (lane >> 3), r = (q.tall ? col : row) + at;
-            if (r < q.rows) ortho_out4(a, q, r, c, *(const f32x4_t*)(lds + at * PITCH + 16 * (lane & 7)));
+            for (int i = 0; i < 4; ++i) {
+                const int at = 8 * i + (lane >> 3), r = (q.tall ? col : row) + at;
+                if (r < q.rows) ortho_out4(a, q, r, c, *(const f32x4_t*)(lds + at * PITCH + 16 * (lane & 7)));
+            }
         }
+        wave_lds_in_order();
     }
 
 private:
     __device__ __forceinline__ void leave(char* dst, int row, int col, int width) const {
         const int lane = threadIdx.x & 63;
+        wave_lds_in_order();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = 8 * i + (lane >> 3), piece = 16 * (lane & 7);
             *(u32x4_t*)(split_at(dst, row + r, col, width) + piece) = *(const u32x4_t*)(lds + r * PITCH + piece);
         }
+        wave_lds_in_order();
     }
 };
 
@@ -685,7 +690,7 @@ __device__ __forceinline__ void ortho_tiny_steps(const OrthoTable& t, const Orth
         const f32x4_t gram = tiny_sum<SMALL_WAVES>(tiny_product(X, xp, X, xp, 16 * wave, 16 * SMALL_WAVES, q.n), sums);
         if (wave == 0) {                                       // LDS of one wave: no barrier between A and what reads it
             *(f32x4_t*)(A + (lane & 15) * PITCH + row) = gram * ldexpf(c.sa / (c.sx * c.sx), -2 * lift);
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_in_order();
             const f32x4_t v = tiny_product(A, PITCH, A, PITCH, 0, 16, 16), own = *(const f32x4_t*)(A + (lane & 15) * PITCH + row);
             const float pa = c.coef[3 * step + 1] * (c.sb / c.sa), pb = c.coef[3 * step + 2] * (c.sb / c.sa / c.sa);
             f32x4_t b;
@@ -702,7 +707,7 @@ __device__ __forceinline__ void ortho_tiny_steps(const OrthoTable& t, const Orth
             f32x4_t x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = fmaf(xb, v[i], xa * own[i]);
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_in_order();
             *(f32x4_t*)at = x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) X[(row + i) * xp + c0 + (lane & 15)] = x[i];
