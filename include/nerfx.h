@@ -401,10 +401,10 @@ int nerfx_mx4_quantize(const void* x, int dtype, int64_t rows, int k, uint8_t* c
 int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int k, int dtype, void* out,
                          void* stream);
 /* y (m, n) = activ(x W^T + bias): x (m, k) in x_dtype, quantised as above on its way (NERFX_TYPE_MX4: x is its codes,
- * x_scales its scales; NULL otherwise), W (n, k) as codes and scales (n <= 2^24), bias (n) fp32 or NULL, sums in fp32,
- * activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as above along n, y its codes and
- * y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes, floats to their own size.  The first call of a
- * kind on a device opts its kernel into its LDS size: make it outside of graph capture.
+ * x_scales its scales; NULL otherwise), W (n, k) as codes and scales (n <= 2^24; 1 to 2^20 for a result in blocks),
+ * bias (n) fp32 or NULL, sums in fp32, activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as
+ * above along n, y its codes and y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes, floats to their own
+ * size.  The first call of a kind on a device opts its kernel into its LDS size: make it outside of graph capture.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
 int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,

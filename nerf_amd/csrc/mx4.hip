@@ -950,9 +950,15 @@ extern "C" int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales,
 }
 
 static bool mx4_type(int dtype) { return float_type(dtype) || dtype == NERFX_TYPE_MX4; }
+// Columns of a result: one in blocks is a matrix that the other calls take.
+static int check_columns(int n, int y_dtype) {
+    NERFX_REQUIRE(n >= 0 && n <= 1 << 24, "n %d out of range [0, 2^24]", n);
+    NERFX_REQUIRE(y_dtype != NERFX_TYPE_MX4 || (n >= 1 && n <= 1 << 20), "n %d of a result in blocks out of range [1, 2^20]", n);
+    return 0;
+}
 
 extern "C" int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype) {
-    if (check_mx4(m, k) || n < 0 || n > 1 << 24 || !mx4_type(x_dtype) || !mx4_type(y_dtype)) return -1;
+    if (check_mx4(m, k) || !mx4_type(x_dtype) || !mx4_type(y_dtype) || check_columns(n, y_dtype)) return -1;
     const Mx4Plan plan = mx4_plan(m, n, k, x_dtype, y_dtype);
     return plan.w_ordered + plan.x_ordered + plan.codes + plan.scales;
 }
@@ -961,9 +967,9 @@ extern "C" int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_sca
                                 const uint8_t* w_scales, int n, const float* bias, int activ, void* y, int y_dtype,
                                 uint8_t* y_scales, void* workspace, int64_t workspace_bytes, void* stream) {
     if (int rc = check_mx4(m, k)) return rc;
-    NERFX_REQUIRE(n >= 0 && n <= 1 << 24, "n %d out of range [0, 2^24]", n);
     NERFX_REQUIRE(mx4_type(x_dtype), "unknown type %d of x", x_dtype);
     NERFX_REQUIRE(mx4_type(y_dtype), "unknown type %d of y", y_dtype);
+    if (int rc = check_columns(n, y_dtype)) return rc;
     NERFX_REQUIRE(activ >= NERFX_ACT_NONE && activ <= NERFX_ACT_SILU, "unknown activation %d", activ);
     if (m == 0 || n == 0) return 0;
     NERFX_REQUIRE(x && w_codes && w_scales && y && (x_dtype != NERFX_TYPE_MX4 || x_scales) && (y_dtype != NERFX_TYPE_MX4 || y_scales),

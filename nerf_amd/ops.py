@@ -889,8 +889,7 @@ class Mx4:
     tensors.  Held as given: no copy."""
 
     def __init__(self, codes: Tensor, scales: Tensor, k: int):
-        if not 1 <= k <= 1 << 20:
-            raise ValueError(f"Mx4: k must be 1..2^20 (got {k})")
+        self._check_k(k)
         blocks = (k + 31) // 32
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or \
                 tuple(scales.shape) != (codes.shape[0], blocks) or codes.shape[1] != 16 * blocks or codes.device != scales.device:
@@ -904,9 +903,15 @@ class Mx4:
         self.shape: Tuple[int, int] = (codes.shape[0], k)
         self.k, self.device = k, codes.device
 
+    @staticmethod
+    def _check_k(k: int) -> None:
+        if not 1 <= k <= 1 << 20:
+            raise ValueError(f"Mx4: k must be 1..2^20 (got {k})")
+
     @classmethod
     def _new(cls, rows: int, k: int, like: Tensor) -> "Mx4":
         """An unwritten one, where `like` is: one allocation, made two tensors of when they are asked for."""
+        cls._check_k(k)
         self = object.__new__(cls)
         self._codes = self._scales = None
         self._both = like.new_empty((rows * ((k + 31) // 32) * 17,), dtype=torch.uint8)
@@ -996,7 +1001,7 @@ def mx4_linear(x, weight: Mx4, bias: Optional[Tensor] = None, activation: Option
     `mx4_quantize` answers.  `x` (..., k): fp32, bf16 or fp16, quantised as `mx4_quantize` does on its way, or an `Mx4`; `weight`
     (n, k); `bias` (n) fp32; `activation` None, "relu", "leaky_relu" (slope 0.01) or "silu".  -> (..., n) in `out_dtype`
     (default: x's type, fp32 for an `Mx4`), or, with out_dtype="mx4", the result quantised on its way out: an `Mx4` of
-    prod(...) rows, what the next layer takes.  No gradient."""
+    prod(...) rows, what the next layer takes (n from 1 to 2^20 then).  No gradient."""
     if not isinstance(weight, Mx4):
         raise TypeError("weight must be an Mx4 (see mx4_quantize)")
     if activation not in _LINEAR_ACTS:
