@@ -370,7 +370,8 @@ typedef struct {
  * transposed.  Sums are fp32 (the norm fp64), products take both factors to 22 bits (24 where a side
  * is 16 or less), whatever the `dtype` (NERFX_TYPE_*) of grad and out.  A zero matrix gives zeros; a matrix with an infinity or
  * a NaN gives NaN.  `mats` is a host array; all matrices share the launches.  Coefficients
- * that would let a singular value grow beyond 64 are refused.  `workspace`:
+ * that would let a singular value grow beyond 64 are refused, and such that take the small ones (the product of the a's)
+ * below a 64th of the largest before the last step.  `workspace`:
  * nerfx_orthogonalize_workspace_bytes(mats, count) bytes (0 for groups of matrices of up to 64 x 256), aligned to 16;
  * it holds nothing between calls.  The first call on a device opts kernels into their LDS sizes: make it outside of
  * graph capture. */

@@ -899,10 +899,12 @@ static int check_sizes(const nerfx_matrix_t* mats, int count) {
 
 // Largest singular value after each step, for start values up to 1: the maximum of |a s + b s^3 + c s^5| over
 // [0, top] by sampling (the polynomial's own maximum lies within the margin of a sample).  It says which
-// power-of-two scales keep X, A and B inside f16.
+// power-of-two scales keep X, A and B inside f16, from above.  From below: small singular values go with the product of the a's.
+// Where X shrinks to less than a 64th of its largest before the last step, its halves run out of f16's small numbers (a = 0.03 five
+// times: 3e-4 off, 0.01: 2.6e-2), and the coefficients are refused.
 struct OrthoScales { float x, a, b; int growth; };
 static int scales_for(const float* coef, int steps, OrthoScales& s) {
-    double top = 1.001, x = top, ga = 0, gb = 0, all = 1;
+    double top = 1.001, x = top, ga = 0, gb = 0, all = 1, small = 1, least = 1;
     for (int k = 0; k < steps; ++k) {
         const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
         NERFX_REQUIRE(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), "coefficient %d is not finite", k);
@@ -915,10 +917,14 @@ static int scales_for(const float* coef, int steps, OrthoScales& s) {
         }
         ga = std::max(ga, top * top);
         x = std::max(x, top);
+        least = std::min(least, small);
+        small *= std::fabs(a);
         top = next * 1.01;
         all *= gain * 1.01;
         NERFX_REQUIRE(top <= 64, "step %d lets singular values grow to %.3g: coefficients out of range", k, top);
     }
+    NERFX_REQUIRE(least * 64 >= x, "coefficients out of range: they shrink small singular values to %.3g before the last step, with %.3g for the largest",
+                  least, x);
     auto scale = [](double bound) { return (float)std::exp2(std::floor(std::log2(32768 / std::max(bound * 1.02, 1e-3)))); };
     s = {scale(x), scale(ga), scale(gb), (int)std::ceil(std::log2(all))};
     return 0;

@@ -792,7 +792,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
 
     `mats`: a matrix, a stack of them (b, r, c), or a list of matrices of any shapes (fp32, bf16 or fp16, one
     type and device); all of them share the launches.  `coefficients`: (a, b, c), or one such triple per
-    step.  -> the same structure in the same type.  Results are held to fp32's precision before that
+    step (include/nerfx.h says which are refused).  -> the same structure in the same type.  Results are held to fp32's precision before that
     last rounding.  Not differentiable."""
     listed = list(mats) if isinstance(mats, (list, tuple)) else list(mats.unbind(0)) if mats.dim() == 3 else [mats]
     schedule = _ns_schedule(coefficients, steps)
