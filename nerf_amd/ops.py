@@ -773,6 +773,12 @@ def _ns_array(rows):
     return (C.c_float * (3 * len(rows)))(*[float(v) for r in rows for v in r])
 
 
+def check_ns_schedule(coefficients, steps: int, eps: float) -> None:
+    """Raises where `orthogonalize` and `muon_step` would refuse these, whatever the matrices."""
+    if lib.nerfx_orthogonalize(None, 0, _lib.TYPE_F32, _ns_schedule(coefficients, steps), steps, eps, None, 0, None):
+        raise ValueError(lib.nerfx_last_error().decode())
+
+
 def _matrix_table(rows):
     """rows of (grad, out, param, momentum, rows, cols) -> the C array of nerfx_matrix_t."""
     n = len(rows)

@@ -168,13 +168,9 @@ class Muon(Adam):
     def __init__(self, params: Iterable[Tensor], lr: float = 5e-4, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, ns_coefficients=ops.NS_COEFFICIENTS, ns_steps: int = 5, ns_eps: float = 1e-7,
                  adjust_lr: str = "match_rms_adamw", betas=(0.9, 0.999), eps: float = 1e-8):
-        if not 0 <= momentum < 1 or ns_eps <= 0 or weight_decay < 0:
-            raise ValueError("invalid Muon hyper-parameters")
-        if adjust_lr not in ("original", "match_rms_adamw"):
-            raise ValueError(f"unknown adjust_lr {adjust_lr!r}")
-        ops._ns_schedule(ns_coefficients, ns_steps)          # a bad schedule fails here, not in the first step
         own = dict(momentum=momentum, nesterov=nesterov, ns_coefficients=ns_coefficients, ns_steps=ns_steps, ns_eps=ns_eps,
                    adjust_lr=adjust_lr, weight_decay=weight_decay)
+        self._check(own)
         groups = list(params)
         if not groups or not isinstance(groups[0], dict):
             groups = [{"params": groups}]
@@ -190,7 +186,19 @@ class Muon(Adam):
                 chosen = [p for p, is_matrix in zip(members, matrix) if is_matrix == muon]
                 if chosen:
                     split.append({**(own if muon else {}), **group, "params": chosen, "muon": muon})
+        for group in split:
+            if group["muon"]:
+                self._check(group)
         super().__init__(split, lr=lr, betas=betas, eps=eps)
+
+    @staticmethod
+    def _check(own) -> None:
+        """What a group of matrices is stepped by: refused here, not in the first step."""
+        if not 0 <= own["momentum"] < 1 or not own["ns_eps"] > 0 or not 0 <= own["weight_decay"] < float("inf"):
+            raise ValueError("invalid Muon hyper-parameters")
+        if own["adjust_lr"] not in ("original", "match_rms_adamw"):
+            raise ValueError(f"unknown adjust_lr {own['adjust_lr']!r}")
+        ops.check_ns_schedule(own["ns_coefficients"], own["ns_steps"], own["ns_eps"])
 
     def _flatten(self, group) -> None:
         if not group["muon"]:
