@@ -179,9 +179,10 @@ class Muon(Adam):
             group = dict(group)
             members, kind = group.pop("params"), group.pop("muon", None)
             members = [members] if isinstance(members, Tensor) else list(members)
-            if kind and any(p.dim() != 2 for p in members):
+            tensors = [p[1] if isinstance(p, tuple) else p for p in members]                # (name, parameter) pairs stay pairs
+            if kind and any(p.dim() != 2 for p in tensors):
                 raise ValueError("nerf_amd.optim.Muon: a group of matrices holds 2-D parameters only")
-            matrix = [p.dim() == 2 and min(p.shape) >= self.MATRIX_SIDE if kind is None else bool(kind) for p in members]
+            matrix = [p.dim() == 2 and min(p.shape) >= self.MATRIX_SIDE if kind is None else bool(kind) for p in tensors]
             for muon in (True, False):
                 chosen = [p for p, is_matrix in zip(members, matrix) if is_matrix == muon]
                 if chosen:

@@ -18,3 +18,20 @@ def test_what_a_group_names_for_itself_is_checked_too(bad):
     for kind in (True, None):
         with pytest.raises(ValueError):
             Muon([{"params": [torch.nn.Parameter(torch.zeros(32, 32))], "muon": kind, **bad}])
+
+
+def test_named_parameters_are_split_as_plain_ones_are(monkeypatch):
+    """torch's optimisers, and so `Adam`, take (name, parameter) pairs too; here up to where the device is looked at."""
+    from nerf_amd.optim import Adam, Muon
+    model = torch.nn.Sequential(torch.nn.Linear(40, 32), torch.nn.Linear(32, 3))
+    monkeypatch.setattr(Adam, "_flatten", lambda self, group: None)
+    monkeypatch.setattr(Muon, "_flatten", lambda self, group: None)
+    assert len(Adam(model.named_parameters()).param_groups[0]["params"]) == 4
+    plain, named = Muon(model.parameters()), Muon(model.named_parameters())
+    in_groups = Muon([{"params": list(model.named_parameters())}])
+    for other in (named, in_groups):
+        assert [[id(p) for p in g["params"]] for g in other.param_groups] == [[id(p) for p in g["params"]] for g in plain.param_groups]
+        assert [g["param_names"] for g in other.param_groups] == [["0.weight"], ["0.bias", "1.weight", "1.bias"]]
+    assert [g["muon"] for g in plain.param_groups] == [True, False]
+    with pytest.raises(ValueError, match="2-D"):
+        Muon([{"params": [("0.bias", model[0].bias)], "muon": True}])
