@@ -796,14 +796,14 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
     """The (semi-)orthogonal matrix near each of `mats` that `steps` Newton-Schulz steps reach: every
     singular value of X = G / max(|G|, eps) goes through a s + b s^3 + c s^5 once per step, singular vectors stay.
 
-    `mats`: a matrix, a stack of them (b, r, c), or a list of matrices of any shapes (fp32, bf16 or fp16, one
+    `mats`: a matrix, a stack of them (b, r, c), or a list or tuple of matrices of any shapes (fp32, bf16 or fp16, one
     type and device); all of them share the launches.  `coefficients`: (a, b, c), or one such triple per
     step (include/nerfx.h says which are refused).  -> the same structure in the same type.  Results are held to fp32's precision before that
     last rounding.  Not differentiable."""
     listed = list(mats) if isinstance(mats, (list, tuple)) else list(mats.unbind(0)) if mats.dim() == 3 else [mats]
     schedule = _ns_schedule(coefficients, steps)
     if not listed:
-        return torch.empty_like(mats) if isinstance(mats, Tensor) else []
+        return torch.empty_like(mats) if isinstance(mats, Tensor) else () if isinstance(mats, tuple) else []
     if not all(isinstance(t, Tensor) for t in listed):
         raise TypeError("mats must be tensors")
     dtype, dev, grad = listed[0].dtype, listed[0].device, torch.is_grad_enabled()
@@ -826,7 +826,7 @@ def orthogonalize(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
     ws, need = _ns_workspace(table, len(srcs), dev)
     with _on(dev):
         check(lib.nerfx_orthogonalize(table, len(srcs), _TYPES[dtype], schedule, steps, eps, _at(ws), need, _stream_on(dev)))
-    return outs if stacked is None else stacked
+    return stacked if stacked is not None else tuple(outs) if isinstance(mats, tuple) else outs
 
 
 def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
