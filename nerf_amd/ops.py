@@ -959,7 +959,7 @@ class Mx4:
         return Mx4(self.codes.to(device), self.scales.to(device), self.k)
 
     def dequantize(self, dtype=torch.float32) -> Tensor:
-        """The values the codes stand for (exact in fp32 and bf16)."""
+        """The values the codes stand for (exact in fp32 and bf16; from 2^128 on, which only stored scales of 253 and 254 reach, infinite)."""
         if dtype not in _TYPES:
             raise TypeError(f"dequantize gives fp32, bf16 or fp16 (asked for {dtype})")
         dev, held = self.device, self._codes if self._both is None else self._both
