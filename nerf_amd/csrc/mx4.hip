@@ -820,11 +820,8 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 //          long as one tile does (256 x 4096 by 4096: 13 us, 19 with 128 x 128; 1024 x 4096 by 4096, 1024 tiles: 27 and 24);
 //          else 128 x 128.
 enum { MX4_SKINNY, MX4_STREAM, MX4_TILE };
-// Steps of 64 values that a row is worked on in: what the stream kernel is made for.
-static int stream_steps(int k) {
-    const int ks = (k + 63) / 64;
-    return ks <= 5 ? ks : 8;
-}
+// Steps of 64 values that a row is worked on in; the stream kernel is made for each number of them.
+static int stream_steps(int k) { return (k + 63) / 64; }
 struct Mx4Plan {
     int kind;
     int64_t w_ordered, x_ordered, codes;                       // bytes of the workspace, in this order; all multiples of 16
@@ -902,6 +899,8 @@ static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
             case 3: return go(mx4_stream_kernel<DT, 3, ODD>, 3);
             case 4: return go(mx4_stream_kernel<DT, 4, ODD>, 4);
             case 5: return go(mx4_stream_kernel<DT, 5, ODD>, 5);
+            case 6: return go(mx4_stream_kernel<DT, 6, ODD>, 6);
+            case 7: return go(mx4_stream_kernel<DT, 7, ODD>, 7);
             default: return go(mx4_stream_kernel<DT, 8, ODD>, 8);
         }
     };
