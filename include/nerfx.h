@@ -406,6 +406,8 @@ int nerfx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
  * bias (n) fp32 or NULL, sums in fp32, activ NERFX_ACT_*, y in y_dtype (NERFX_TYPE_MX4: the fp32 result is quantised as
  * above along n, y its codes and y_scales its scales; NULL otherwise).  Codes aligned to 16 bytes, floats to their own
  * size.  The first call of a kind on a device opts its kernel into its LDS size: make it outside of graph capture.
+ * y shares no memory with x, W or bias.  How sums are divided goes by m: a row's last bits may depend on how many come
+ * with it.  More than 2^22 tiles of results (of 256 x 256 where there are many) are refused.
  * `workspace`: nerfx_mx4_linear_workspace_bytes bytes, aligned to 16; it holds nothing between calls. */
 int64_t nerfx_mx4_linear_workspace_bytes(int64_t m, int n, int k, int x_dtype, int y_dtype);
 int nerfx_mx4_linear(const void* x, int x_dtype, const uint8_t* x_scales, int64_t m, int k,

@@ -5,7 +5,10 @@ a weight), every layer one `ops.mx4_linear` whose input was quantised on its way
 take 4.25 bits a value in memory, sums are fp32, biases and both output activations too.  It goes wherever a field goes
 that is not trained: `forward`, `BoundedVolumeRaymarcher.render_volume(train=False)`, `nerf_amd.infer`.  Its layers are
 calls of their own, so that the width is not bound to what the fused kernels of `NeRF` hold on chip (256): a wider field, for
-which there are no such kernels, is served this way.  Up to 256 the bf16 kernels are faster and closer; there it saves memory only."""
+which there are no such kernels, is served this way.  Up to 256 the bf16 kernels are faster and closer; there it saves memory only.
+
+It is a coarse form: encoded points, activations and weights are all rounded to 4 bits, and nothing trains or calibrates the field
+for it.  Against the fp32 frame a field as it is made has 49 dB (bf16: 88), one after 2,000 steps on a smooth pattern 19 dB (bf16: 57)."""
 import copy
 from typing import Optional, Tuple
 

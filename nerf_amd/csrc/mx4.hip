@@ -208,7 +208,8 @@ __device__ __forceinline__ void mx4_store(const Mx4LinearArgs& a, int64_t at, fl
 // there: a phase's sixteen on different banks.
 struct Mx4Lines {
     static constexpr int PITCH = 144, BYTES = 32 * PITCH;      // of LDS, for one wave
-    static constexpr int FEW = 4;                              // 1M x 3 fp32: 26 us from the registers, 38 by way of LDS; x 8: 49 and 41
+    // Columns that are stored from the registers (1M x 128 in blocks by 3, fp32: 16 us, 23 by way of LDS; by 8: 24 and 18).
+    static constexpr int FEW = 4;
     char* lds;
     int begin = 0, end = 0;                                    // bytes of y's rows that are collected
 
@@ -542,7 +543,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void mx4_tile_kernel(const Mx4LinearA
 // Up to 64 rows of x: the weight is read once and nothing else counts.  A workgroup takes 16 rows of W, its waves parts
 // of K; each lane's 16-byte load is a block of W, which is an operand of the matrix instruction as it
 // is (16 x 16 x 128).  Rows of x in a float type are quantised by the workgroup into LDS, a block a thread, while the first
-// loads of W are on their way (one row by 4096 x 4096: 5.7 us, of which a launch is 3 and 9 MB at 5 TB/s are 2).
+// loads of W are on their way (one row by 4096 x 4096: 5.2 us a call in a captured graph; a launch
+// behind another is 1.5 of it and 9 MB at 5 TB/s are 2).
 constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 8, SKINNY_AHEAD = 4, SKINNY_LDS = 64 * 1024, SKINNY_FLOATS = 128 * 1024;
 
 __device__ __forceinline__ void mx4_store_one(const Mx4LinearArgs& a, int64_t m, int n, float acc) {
@@ -809,9 +811,9 @@ static int tile_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 }
 
 // How a product is done, by its sizes:
-//  skinny  up to 64 rows of x: W is read once, by as many workgroups as it has 16 rows (one row by 4096 x 4096: 5.7 us, 11 with
-//          tiles).  Each of them quantises float rows for itself, up to 128 KB of them (64 x 1000 fp32 by 1000: 15 us, 7.6 with
-//          tiles; 32 x 2048 bf16 by 256: 7 and 8.5), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
+//  skinny  up to 64 rows of x: W is read once, by as many workgroups as it has 16 rows (one row by 4096 x 4096: 5.2 us, 10.2 with
+//          tiles).  Each of them quantises float rows for itself, up to 128 KB of them (64 x 1000 fp32 by 1000: 15 us, 6.9 with
+//          tiles; 32 x 2048 bf16 by 256: 6.7 and 7.8), or 16 rows: by way of the workspace, if their codes do not fit in LDS.
 //          Not for a result in blocks, which are of 32 columns;
 //  stream  otherwise up to 256 values a row (of floats, up to 512 bytes), or 512 and up to 256 columns: float rows are quantised in
 //          registers, once for every 256 columns (16,384 x 4096 bf16 by 128: 31 us, 42 with tiles; by 512: 80, and 57 with tiles);
@@ -868,10 +870,10 @@ static int skinny_launch(const Mx4LinearArgs& a, hipStream_t stream) {
 template <int DT>
 static int stream_launch(const Mx4LinearArgs& a, hipStream_t stream) {
     // Few rows: smaller workgroups and fewer columns in each until the device is full.  A lane's row is a line of its own, so that
-    // the loads of eight waves take a CU 3.5 us for every 256 bytes a row (1000 x 128 fp32 by 295: 6.7 us with one wave, 10.7 with
-    // eight); and a wave brings 256 blocks of W at a time, for which it may wait twice.  Half of the device is enough below eight waves
-    // (16,000 x 256 bf16 by 256: 9.2 us with 125 workgroups of four, 10.3 with 250 of two), not with them (32,000 x 128 fp32 by 256:
-    // 17.6 us with 125 of eight, 12.9 with 250 of four).
+    // the loads of eight waves take a CU 3.5 us for every 256 bytes a row (1000 x 128 fp32 by 295: 6.9 us with one wave, 11.6 with
+    // eight, in a captured graph); and a wave brings 256 blocks of W at a time, for which it may wait twice.  Half of the device is
+    // enough below eight waves (16,000 x 256 bf16 by 256: 9.2 us with 125 workgroups of four, 10.3 with 250 of two), not with them
+    // (32,000 x 128 fp32 by 256: 17.6 us with 125 of eight, 12.9 with 250 of four).
     const int tiles = (a.n + 31) / 32, ks = stream_steps(a.k);
     int waves = 2 * STREAM_WAVES, groups;
     int64_t row_tiles;

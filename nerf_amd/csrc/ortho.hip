@@ -239,6 +239,10 @@ __global__ __launch_bounds__(256) void ortho_prep_kernel(const OrthoTable* __res
 // their way while one is worked on (LDS-DMA: no registers hold them).  16-byte chunk c of row r lies at place
 // c ^ (r / 2 % 8), so that the sixteen rows a ds_read_b128 phase touches (256 bytes of banks) lie apart; LDS-DMA
 // writes lane after lane, so it is the source address that is permuted.
+// Bound by LDS reads where there are many tiles: a stage of a tile of 64 is 32 KB of fragments for its four waves and 192 cycles of
+// matrix instructions, of a tile of 128 96 KB and 768 cycles; LDS gives a CU at most 128 bytes a cycle.  (2048 x 2048 by 2048: 49.9 us, 50.2
+// without loads of stages, 41.6 without products.)  Rows of X are not divided over workgroups: a matrix with a side of up to 64 has one for
+// its Gram matrix, which goes over the other side by itself (64 x 32768: 1.4 ms, 16 x 32768: 0.8).
 template <int T, int WAVES, int STAGES>
 struct SplitTile {
     static constexpr int FP = T / 64, FQ = T / (16 * WAVES); // 32 x 32 fragments per wave and side
