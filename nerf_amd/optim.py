@@ -183,6 +183,8 @@ class Muon(Adam):
             if kind and any(p.dim() != 2 for p in tensors):
                 raise ValueError("nerf_amd.optim.Muon: a group of matrices holds 2-D parameters only")
             matrix = [p.dim() == 2 and min(p.shape) >= self.MATRIX_SIDE if kind is None else bool(kind) for p in tensors]
+            if any(is_matrix and max(p.shape) > 32768 for p, is_matrix in zip(tensors, matrix)):
+                raise ValueError('nerf_amd.optim.Muon: matrices have sides of up to 32768 (a group with "muon": False gets Adam\'s step)')
             for muon in (True, False):
                 chosen = [p for p, is_matrix in zip(members, matrix) if is_matrix == muon]
                 if chosen:

@@ -35,3 +35,13 @@ def test_named_parameters_are_split_as_plain_ones_are(monkeypatch):
     assert [g["muon"] for g in plain.param_groups] == [True, False]
     with pytest.raises(ValueError, match="2-D"):
         Muon([{"params": [("0.bias", model[0].bias)], "muon": True}])
+
+
+def test_a_side_that_no_step_takes_fails_at_once():
+    from nerf_amd.optim import Muon
+    long = torch.nn.Parameter(torch.zeros(32769, 16))
+    for group in ([long], [{"params": [long], "muon": True}], [("table", long)]):
+        with pytest.raises(ValueError, match="32768"):
+            Muon(group)
+    with pytest.raises(RuntimeError, match="ROCm"):                       # Adam's may be of any size
+        Muon([{"params": [long], "muon": False}])
